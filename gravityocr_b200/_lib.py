@@ -25,7 +25,8 @@ EXPORTS = ("gr_version", "gr_status_string", "gr_set_pdl", "gr_set_attention_tc"
            "gr_attention_workspace_bytes", "gr_linear_default_splits", "gr_linear_plan", "gr_linear", "gr_embed_rows",
            "gr_residual_norm", "gr_bd_attention", "gr_accept_commit", "gr_draft_override", "gr_pack_gate_up",
            "gr_bd_attention_noalloc", "gr_bd_attention_ordered", "gr_gather_rows", "gr_logits_process",
-           "gr_sample_rows", "gr_commit_sampled", "gr_penalty_cumulate")
+           "gr_sample_rows", "gr_commit_sampled", "gr_penalty_cumulate", "gr_qk_norm_rope_write", "gr_kv_read",
+           "gr_kv8_attention_workspace_bytes", "gr_kv8_attention_plan", "gr_kv8_attention", "gr_token_logprobs")
 FILTER_JOINT, FILTER_SEQUENTIAL, FILTER_TORCH = range(3)
 PEN_REPETITION, PEN_FREQUENCY, PEN_PRESENCE, PEN_MIN_NEW_TOKENS = range(4)
 COIN_ACCEPT, COIN_FINAL, COIN_FIRST, COIN_PREFILL = range(4)
@@ -83,6 +84,20 @@ class Sampling(ctypes.Structure):
     ]
 
 
+class KvCache(ctypes.Structure):
+    """gr_kv_cache: one layer's paged K/V cache in bf16, e4m3 or int8 (made by ``kv_cache``)."""
+    _fields_ = [
+        ("format", ctypes.c_int),
+        ("n_kv_heads", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+        ("n_pages", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_exp", ctypes.c_void_p),
+        ("v_exp", ctypes.c_void_p),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -114,6 +129,15 @@ _SIGS = {
     "gr_bd_attention_ordered": (_I, [_P, _P, _P, _L, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _Z, _P,
                                      _P]),
 }
+_SIGS.update({
+    "gr_qk_norm_rope_write": (_I, [_P, _L, _I, _I, ctypes.POINTER(KvCache), _P, _P, ctypes.c_double, _P, _P, _P, _P, _I, _I,
+                                   _P, _P, _P, _P]),
+    "gr_kv_read": (_I, [ctypes.POINTER(KvCache), _P, _L, _P, _P, _P, _P]),
+    "gr_kv8_attention_workspace_bytes": (_Z, [_I, _I, _I, _I, _I]),
+    "gr_kv8_attention_plan": (_I, [_I, _I, _I, _I, _I, _P]),
+    "gr_kv8_attention": (_I, [_P, ctypes.POINTER(KvCache), _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _Z, _P, _P]),
+    "gr_token_logprobs": (_I, [_P, _I, _L, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P]),
+})
 GR_ERR_SCRATCH_LIMIT = 8
 NOALLOC_SCRATCH_BYTES = 8 << 20
 
@@ -304,3 +328,182 @@ def commit_sampled(bs: int, K: int, am, accept, sample, seeds, rpi, seq_lens, pr
 def penalty_cumulate(bs: int, tokens, stride: int, counts, add: int, smp: Sampling, stream=None) -> None:
     _check(load().gr_penalty_cumulate(bs, tokens.data_ptr(), stride, _ptr(counts), add, ctypes.byref(smp),
                                       _stream(stream)), "gr_penalty_cumulate")
+
+
+# ---------------------------------------------------------------------- 8-bit K/V cache
+KV_BF16, KV_E4M3, KV_INT8 = range(3)
+_KV_FORMATS = {torch.bfloat16: KV_BF16, torch.float8_e4m3fn: KV_E4M3, torch.int8: KV_INT8}
+
+
+def _same_device(first: torch.Tensor, **others: Optional[torch.Tensor]) -> None:
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"{name} is on {t.device}, the call's other tensors on {first.device}")
+
+
+def _numel(t: torch.Tensor, n: int, name: str) -> None:
+    if t.numel() != n:
+        raise RuntimeError(f"{name} holds {t.numel()} elements, the call needs {n}")
+
+
+def _status_ok(status: Optional[torch.Tensor]) -> None:
+    if status is not None:
+        _need(status, torch.int32, "status")
+        if status.numel() < 1:
+            raise RuntimeError("status is empty")
+
+
+def kv_cache(k: torch.Tensor, v: torch.Tensor, k_exp: Optional[torch.Tensor] = None,
+             v_exp: Optional[torch.Tensor] = None) -> KvCache:
+    """One layer's cache over the caller's tensors: k / v [pages, kv_heads, 16, 128] in bf16, float8_e4m3fn or int8 (the
+    dtype is the format), and for the 8-bit formats k_exp / v_exp int8 [pages, kv_heads, 16].  The handle keeps the
+    tensors alive."""
+    if k.dtype not in _KV_FORMATS:
+        raise RuntimeError(f"no cache format for {k.dtype}")
+    _need(k, k.dtype, "k")
+    _need(v, k.dtype, "v")
+    if k.dim() != 4 or tuple(k.shape[2:]) != (16, 128) or v.shape != k.shape:
+        raise RuntimeError(f"k / v must be [pages, kv_heads, 16, 128], got {tuple(k.shape)} / {tuple(v.shape)}")
+    c = KvCache()
+    c.format = _KV_FORMATS[k.dtype]
+    if (c.format == KV_BF16) != (k_exp is None) or (k_exp is None) != (v_exp is None):
+        raise RuntimeError("8-bit caches need k_exp and v_exp, a bf16 cache takes neither")
+    for t, name in ((k_exp, "k_exp"), (v_exp, "v_exp")):
+        if t is not None:
+            _need(t, torch.int8, name)
+            if t.shape != k.shape[:3]:
+                raise RuntimeError(f"{name} must be {tuple(k.shape[:3])}, got {tuple(t.shape)}")
+    _same_device(k, v=v, k_exp=k_exp, v_exp=v_exp)
+    c.n_pages, c.n_kv_heads, c.page_size = k.shape[0], k.shape[1], 16
+    c.k, c.v, c.k_exp, c.v_exp = _ptr(k), _ptr(v), _ptr(k_exp), _ptr(v_exp)
+    c.tensors = (k, v, k_exp, v_exp)
+    return c
+
+
+def qk_norm_rope_write(qkv: torch.Tensor, n_q_heads: int, cache: KvCache, row_slot: torch.Tensor, q_out: torch.Tensor,
+                       inv_freq: Optional[torch.Tensor], rotary_dim: int, *, row_pos=None, row_pos3=None,
+                       mrope_section=None, rope_half: bool = False, q_norm=None, k_norm=None, eps: float = 1e-5,
+                       status=None, stream=None) -> None:
+    """Projected rows qkv [m, >= (n_q_heads + 2 kv_heads) * 128] bf16 (a row stride is allowed): per-head norms of q and k
+    (optional), the rotation, q to q_out, k and v to the cache at row_slot (gr_qk_norm_rope_write)."""
+    if not qkv.is_cuda or qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+        raise RuntimeError("qkv must be a CUDA bf16 [m, width] tensor with unit column stride")
+    m, heads = qkv.shape[0], n_q_heads + 2 * cache.n_kv_heads
+    if m < 1 or n_q_heads < 1 or qkv.shape[1] < heads * 128:
+        raise RuntimeError(f"qkv {tuple(qkv.shape)} does not hold {heads} heads of 128")
+    _need(row_slot, torch.int64, "row_slot")
+    _need(q_out, torch.bfloat16, "q_out")
+    _numel(row_slot, m, "row_slot")
+    _numel(q_out, m * n_q_heads * 128, "q_out")
+    for t, n, dt, name in ((row_pos, m, torch.int32, "row_pos"), (row_pos3, 3 * m, torch.int32, "row_pos3"),
+                           (inv_freq, rotary_dim // 2, torch.float32, "inv_freq"), (q_norm, 128, torch.bfloat16, "q_norm"),
+                           (k_norm, 128, torch.bfloat16, "k_norm")):
+        if t is not None:
+            _need(t, dt, name)
+            _numel(t, n, name)
+    _status_ok(status)
+    _same_device(qkv, cache=cache.tensors[0], row_slot=row_slot, q_out=q_out, row_pos=row_pos, row_pos3=row_pos3,
+                 inv_freq=inv_freq, q_norm=q_norm, k_norm=k_norm, status=status)
+    sec = None if mrope_section is None else (ctypes.c_int32 * 3)(*mrope_section)
+    with torch.cuda.device(qkv.device):
+        rc = load().gr_qk_norm_rope_write(qkv.data_ptr(), qkv.stride(0) if m > 1 else max(qkv.stride(0), qkv.shape[1]), m,
+                                          n_q_heads, ctypes.byref(cache), _ptr(q_norm), _ptr(k_norm), eps,
+                                          _ptr(row_pos), _ptr(row_pos3), sec, _ptr(inv_freq), rotary_dim,
+                                          1 if rope_half else 0, row_slot.data_ptr(), q_out.data_ptr(), _ptr(status),
+                                          _stream(stream))
+    _check(rc, "gr_qk_norm_rope_write")
+
+
+def kv_read(cache: KvCache, slots: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, *, status=None,
+            stream=None) -> None:
+    """Cache rows at ``slots`` (int64 [n]) back in bf16: k_out / v_out [n, kv_heads * 128] (gr_kv_read)."""
+    _need(slots, torch.int64, "slots")
+    _need(k_out, torch.bfloat16, "k_out")
+    _need(v_out, torch.bfloat16, "v_out")
+    n = slots.numel()
+    _numel(k_out, n * cache.n_kv_heads * 128, "k_out")
+    _numel(v_out, n * cache.n_kv_heads * 128, "v_out")
+    _status_ok(status)
+    _same_device(slots, cache=cache.tensors[0], k_out=k_out, v_out=v_out, status=status)
+    with torch.cuda.device(slots.device):
+        rc = load().gr_kv_read(ctypes.byref(cache), slots.data_ptr(), n, k_out.data_ptr(), v_out.data_ptr(), _ptr(status),
+                               _stream(stream))
+    _check(rc, "gr_kv_read")
+
+
+def kv8_attention_workspace_bytes(bs: int, K: int, n_q_heads: int, n_kv_heads: int, max_splits: int) -> int:
+    return int(load().gr_kv8_attention_workspace_bytes(bs, K, n_q_heads, n_kv_heads, max_splits))
+
+
+def kv8_attention_split(bs: int, K: int, max_len: int, n_q_heads: int, n_kv_heads: int):
+    """(chunk, splits) of kv8_attention for requests of up to ``max_len`` tokens, the K new rows included."""
+    out = (ctypes.c_int32 * 2)()
+    _check(load().gr_kv8_attention_plan(bs, K, max_len, n_q_heads, n_kv_heads, out), "gr_kv8_attention_plan")
+    return out[0], out[1]
+
+
+def kv8_attention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, seq_lens: torch.Tensor, bs: int, K: int,
+                  draft: int, base_add: int, n_q_heads: int, chunk: int, max_splits: int, out: torch.Tensor,
+                  workspace: Optional[torch.Tensor], *, status=None, stream=None) -> None:
+    """``bd_attention`` over an 8-bit cache; K = 1 is the attention of one new token (gr_kv8_attention)."""
+    _need(q, torch.bfloat16, "q")
+    _need(out, torch.bfloat16, "out")
+    _need(page_table, torch.int32, "page_table")
+    _need(seq_lens, torch.int64, "seq_lens")
+    if q.numel() < bs * K * n_q_heads * 128 or out.numel() < bs * K * n_q_heads * 128:
+        raise RuntimeError(f"q / out hold fewer than bs * K = {bs * K} rows of {n_q_heads} heads")
+    if page_table.dim() != 2 or page_table.shape[0] < bs or seq_lens.numel() < bs:
+        raise RuntimeError(f"page_table {tuple(page_table.shape)} / seq_lens {tuple(seq_lens.shape)} hold fewer than {bs} requests")
+    _status_ok(status)
+    if workspace is not None:
+        _need(workspace, workspace.dtype, "workspace")
+    _same_device(q, cache=cache.tensors[0], page_table=page_table, seq_lens=seq_lens, out=out, workspace=workspace,
+                 status=status)
+    with torch.cuda.device(q.device):
+        rc = load().gr_kv8_attention(q.data_ptr(), ctypes.byref(cache), page_table.data_ptr(), page_table.shape[1],
+                                     seq_lens.data_ptr(), bs, K, int(draft), base_add, n_q_heads, chunk, max_splits,
+                                     out.data_ptr(), _ptr(workspace),
+                                     0 if workspace is None else workspace.numel() * workspace.element_size(),
+                                     _ptr(status), _stream(stream))
+    _check(rc, "gr_kv8_attention")
+
+
+# ---------------------------------------------------------------------- log probabilities
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor,
+                   rank: torch.Tensor, *, top_logprob: Optional[torch.Tensor] = None,
+                   top_ids: Optional[torch.Tensor] = None, temperature: Optional[torch.Tensor] = None, status=None,
+                   stream=None) -> None:
+    """Log probability, rank and entropy of ids [rows] under softmax(logits / temperature), and the best alternatives into
+    top_logprob / top_ids [rows, n].  logits: fp32 or bf16 [rows, vocab]; a row stride is allowed (gr_token_logprobs)."""
+    if not logits.is_cuda or logits.dtype not in (torch.float32, torch.bfloat16) or logits.dim() != 2 or (
+            logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise RuntimeError("logits must be a CUDA fp32 or bf16 [rows, vocab] tensor with unit column stride")
+    rows, vocab = logits.shape
+    _need(ids, torch.int64, "ids")
+    _need(logprob, torch.float32, "logprob")
+    _need(entropy, torch.float32, "entropy")
+    _need(rank, torch.int32, "rank")
+    for t, name in ((ids, "ids"), (logprob, "logprob"), (entropy, "entropy"), (rank, "rank")):
+        _numel(t, rows, name)
+    if temperature is not None:
+        _need(temperature, torch.float32, "temperature")
+        _numel(temperature, rows, "temperature")
+    n_top = 0
+    if (top_logprob is None) != (top_ids is None):
+        raise RuntimeError("top_logprob and top_ids come together")
+    if top_ids is not None:
+        _need(top_logprob, torch.float32, "top_logprob")
+        _need(top_ids, torch.int32, "top_ids")
+        if top_ids.dim() != 2 or top_ids.shape[0] != rows or top_logprob.shape != top_ids.shape:
+            raise RuntimeError(f"top_logprob / top_ids must be [{rows}, n]")
+        n_top = top_ids.shape[1]
+    _status_ok(status)
+    _same_device(logits, ids=ids, logprob=logprob, entropy=entropy, rank=rank, top_logprob=top_logprob, top_ids=top_ids,
+                 temperature=temperature, status=status)
+    with torch.cuda.device(logits.device):
+        rc = load().gr_token_logprobs(logits.data_ptr(), int(logits.dtype == torch.bfloat16),
+                                      logits.stride(0) if rows > 1 else max(logits.stride(0), vocab), rows, vocab,
+                                      ids.data_ptr(), _ptr(temperature), n_top, logprob.data_ptr(), entropy.data_ptr(),
+                                      rank.data_ptr(), _ptr(top_logprob), _ptr(top_ids), _ptr(status),
+                                      _stream(stream))
+    _check(rc, "gr_token_logprobs")

@@ -22,7 +22,8 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libgravity_b200.so")
 TIMELINE_LIB = os.path.join(HERE, "libgravity_b200_timeline.so")
-SOURCES = ["linear.cu", "attention.cu", "attention_tc.cu", "rowwise.cu", "sampling.cu", "capi.cu"]
+SOURCES = ["linear.cu", "attention.cu", "attention_tc.cu", "rowwise.cu", "sampling.cu", "kv8.cu",
+           "attention_kv8.cu", "logprobs.cu", "capi.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -1,5 +1,6 @@
 // extern "C" entry points of libgravity_b200.so (declared in include/gravity_b200.h): argument checks, tile and
 // split heuristics, TMA tensor-map encoding (cached per buffer) and the launches.
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <map>
@@ -795,6 +796,212 @@ int gr_pack_gate_up(const void* src, void* dst, int intermediate, int hidden, vo
                              hidden, static_cast<cudaStream_t>(stream)) == cudaSuccess
              ? GR_OK
              : GR_ERR_CUDA;
+}
+
+// ------------------------------------------------------------------ 8-bit K/V cache, log probabilities
+static bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+static int check_cache(const gr_kv_cache* c) {
+  if (!c || c->format < GR_KV_BF16 || c->format > GR_KV_INT8 || c->n_kv_heads <= 0 || c->page_size != 16 ||
+      c->n_pages <= 0 || !c->k || !c->v || !aligned(c->k, 16) || !aligned(c->v, 16))
+    return GR_ERR_ARG;
+  if (c->format != GR_KV_BF16 && (!c->k_exp || !c->v_exp || !aligned(c->k_exp, 16) || !aligned(c->v_exp, 16)))
+    return GR_ERR_ARG;
+  // cache rows are counted in 32 bits by the TMA coordinates
+  if (c->n_pages > (INT32_MAX / 16) / c->n_kv_heads) return GR_ERR_UNSUPPORTED;
+  return GR_OK;
+}
+
+// 1-byte codes as rows of 128, a box of one (page, head): 16 rows, 128-byte swizzle.
+static int tensor_map_codes(const void* base, uint64_t rows, CUtensorMap* out) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return GR_ERR_TMA;
+  const cuuint64_t dims[2] = {128, rows};
+  const cuuint64_t strides[1] = {128};
+  const cuuint32_t box[2] = {128, 16};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? GR_OK
+             : GR_ERR_TMA;
+}
+
+int gr_qk_norm_rope_write(const void* qkv, int64_t ld_qkv, int m, int n_q_heads, const gr_kv_cache* cache,
+                          const void* q_norm, const void* k_norm, double eps, const int32_t* row_pos,
+                          const int32_t* row_pos3, const int32_t* mrope_section, const float* inv_freq, int rotary_dim,
+                          int rope_half, const int64_t* row_slot, void* q_out, int32_t* status, void* stream) {
+  const int rc = check_cache(cache);
+  if (rc) return rc;
+  if (!qkv || m <= 0 || n_q_heads <= 0 || !row_slot || !q_out || !(eps >= 0.0)) return GR_ERR_ARG;
+  if (n_q_heads > 1024 || cache->n_kv_heads > 1024) return GR_ERR_UNSUPPORTED;
+  if (ld_qkv < static_cast<int64_t>(n_q_heads + 2 * cache->n_kv_heads) * 128 || ld_qkv % 4 || !aligned(qkv, 8) ||
+      !aligned(q_out, 8) || !aligned(q_norm, 8) || !aligned(k_norm, 8))
+    return GR_ERR_ARG;
+  if (rotary_dim < 0 || rotary_dim > 128 || rotary_dim % 8) return GR_ERR_ARG;
+  if (rotary_dim > 0 && (!inv_freq || (!row_pos && !row_pos3))) return GR_ERR_ARG;
+  if (row_pos && row_pos3) return GR_ERR_ARG;
+  if (row_pos3 && (!mrope_section || mrope_section[0] < 0 || mrope_section[1] < 0 || mrope_section[2] < 0 ||
+                   static_cast<int64_t>(mrope_section[0]) + mrope_section[1] + mrope_section[2] != rotary_dim / 2))
+    return GR_ERR_ARG;
+  KvWriteParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.qkv = static_cast<const __nv_bfloat16*>(qkv);
+  p.ld_qkv = ld_qkv;
+  p.m = m;
+  p.n_q_heads = n_q_heads;
+  p.n_kv_heads = cache->n_kv_heads;
+  p.sms = num_sms();
+  p.q_norm = static_cast<const __nv_bfloat16*>(q_norm);
+  p.k_norm = static_cast<const __nv_bfloat16*>(k_norm);
+  p.eps = eps;
+  p.row_pos = row_pos;
+  p.row_pos3 = row_pos3;
+  p.mrope_s0 = row_pos3 ? mrope_section[0] : 0;
+  p.mrope_s1 = row_pos3 ? mrope_section[1] : 0;
+  p.inv_freq = inv_freq;
+  p.rotary_dim = rotary_dim;
+  p.row_slot = row_slot;
+  p.n_slots = cache->n_pages * 16;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.k = cache->k;
+  p.v = cache->v;
+  p.k_exp = cache->k_exp;
+  p.v_exp = cache->v_exp;
+  p.status = status;
+  return launch_qk_norm_rope_write(p, cache->format, rope_half != 0, static_cast<cudaStream_t>(stream), g_pdl) ==
+                 cudaSuccess
+             ? GR_OK
+             : GR_ERR_CUDA;
+}
+
+int gr_kv_read(const gr_kv_cache* cache, const int64_t* slots, int64_t n, void* k_out, void* v_out, int32_t* status,
+               void* stream) {
+  const int rc = check_cache(cache);
+  if (rc) return rc;
+  if (!slots || n <= 0 || !k_out || !v_out || !aligned(k_out, 16) || !aligned(v_out, 16)) return GR_ERR_ARG;
+  if (n > INT32_MAX || cache->n_kv_heads > 1024) return GR_ERR_UNSUPPORTED;
+  KvReadParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.k = cache->k;
+  p.v = cache->v;
+  p.k_exp = cache->k_exp;
+  p.v_exp = cache->v_exp;
+  p.n_kv_heads = cache->n_kv_heads;
+  p.n_slots = cache->n_pages * 16;
+  p.slots = slots;
+  p.n = n;
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.v_out = static_cast<__nv_bfloat16*>(v_out);
+  p.status = status;
+  return launch_kv_read(p, cache->format, static_cast<cudaStream_t>(stream), g_pdl) == cudaSuccess ? GR_OK
+                                                                                                  : GR_ERR_CUDA;
+}
+
+size_t gr_kv8_attention_workspace_bytes(int bs, int K, int n_q_heads, int n_kv_heads, int max_splits) {
+  if (bs <= 0 || K <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads || max_splits <= 0) return 0;
+  return kv8_attention_ws_bytes(bs, n_q_heads / n_kv_heads * K, n_kv_heads, max_splits, nullptr, nullptr);
+}
+
+int gr_kv8_attention_plan(int bs, int K, int max_len, int n_q_heads, int n_kv_heads, int32_t* out) {
+  if (!out || bs <= 0 || K <= 0 || max_len <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads)
+    return GR_ERR_ARG;
+  const int64_t units = static_cast<int64_t>(bs) * n_kv_heads;
+  // two CTAs an SM: the (request, head) pairs times the splits of the longest request make about one such wave
+  const int64_t per = (2LL * num_sms() + units - 1) / units;
+  int64_t chunk = (static_cast<int64_t>(max_len) + per - 1) / per;
+  if (chunk > 1024 && units >= num_sms()) chunk = 1024;  // many requests of mixed lengths: even pieces
+  const int64_t least = (static_cast<int64_t>(max_len) + kKv8MaxSplits - 1) / kKv8MaxSplits;
+  if (chunk < least) chunk = least;
+  if (chunk < 128) chunk = 128;
+  chunk = (chunk + 31) / 32 * 32;
+  out[0] = static_cast<int32_t>(chunk);
+  out[1] = static_cast<int32_t>((max_len + chunk - 1) / chunk);
+  return GR_OK;
+}
+
+int gr_kv8_attention(const void* q, const gr_kv_cache* cache, const int32_t* page_table, int pt_stride,
+                     const int64_t* seq_lens, int bs, int K, int draft, int base_add, int n_q_heads, int chunk,
+                     int max_splits, void* out, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  const int rc = check_cache(cache);
+  if (rc) return rc;
+  if (cache->format == GR_KV_BF16) return GR_ERR_UNSUPPORTED;
+  if (!q || !page_table || !seq_lens || !out || bs <= 0 || K <= 0 || pt_stride <= 0 || n_q_heads <= 0 ||
+      n_q_heads % cache->n_kv_heads || draft < 0 || draft > 2 || chunk <= 0 || chunk % 32 || max_splits <= 0 ||
+      max_splits > kKv8MaxSplits || !aligned(q, 16) || !aligned(out, 16))
+    return GR_ERR_ARG;
+  const int64_t rows = static_cast<int64_t>(n_q_heads / cache->n_kv_heads) * K;
+  if (rows > 128 || bs > 65535 || cache->n_kv_heads > 65535 ||
+      static_cast<int64_t>(bs) * cache->n_kv_heads > kKv8TicketPairs ||
+      pt_stride > (INT32_MAX - 8192) / 16 || chunk > INT32_MAX / 2)
+    return GR_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(chunk) * max_splits < K) return GR_ERR_ARG;
+  KvAttnParams p;
+  std::memset(&p, 0, sizeof(p));
+  if (max_splits > 1) {
+    size_t o_off, ml_off;
+    const size_t need = kv8_attention_ws_bytes(bs, static_cast<int>(rows), cache->n_kv_heads, max_splits, &o_off, &ml_off);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16)) return GR_ERR_ARG;
+    uint8_t* w = static_cast<uint8_t*>(workspace);
+    p.ws_ticket = reinterpret_cast<int*>(w);
+    p.ws_o = reinterpret_cast<float*>(w + o_off);
+    p.ws_ml = reinterpret_cast<float*>(w + ml_off);
+  }
+  const uint64_t code_rows = static_cast<uint64_t>(cache->n_pages) * cache->n_kv_heads * 16;
+  CUtensorMap tmk, tmv;
+  int e = tensor_map_codes(cache->k, code_rows, &tmk);
+  if (e) return e;
+  e = tensor_map_codes(cache->v, code_rows, &tmv);
+  if (e) return e;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.k_exp = cache->k_exp;
+  p.v_exp = cache->v_exp;
+  p.n_pages = static_cast<int>(cache->n_pages);
+  p.page_table = page_table;
+  p.pt_stride = pt_stride;
+  p.seq_lens = seq_lens;
+  p.bs = bs;
+  p.K = K;
+  p.draft = draft;
+  p.base_add = base_add;
+  p.n_q_heads = n_q_heads;
+  p.n_kv_heads = cache->n_kv_heads;
+  p.chunk = chunk;
+  p.max_splits = max_splits;
+  p.scale_log2 = (1.0f / sqrtf(128.0f)) * 1.4426950408889634f;
+  p.status = status;
+  return launch_kv8_attention(tmk, tmv, p, cache->format, static_cast<cudaStream_t>(stream), g_pdl) == cudaSuccess
+             ? GR_OK
+             : GR_ERR_CUDA;
+}
+
+int gr_token_logprobs(const void* logits, int is_bf16, int64_t ld, int rows, int vocab, const int64_t* ids,
+                      const float* temperature, int n_top, float* logprob, float* entropy, int32_t* rank,
+                      float* top_logprob, int32_t* top_ids, int32_t* status, void* stream) {
+  if (!logits || rows <= 0 || vocab <= 0 || ld < vocab || !ids || !logprob || !entropy || !rank || n_top < 0 ||
+      n_top > kLogprobMaxTop || n_top > vocab || (n_top > 0 && (!top_logprob || !top_ids)) ||
+      !aligned(logits, is_bf16 ? 2 : 4))
+    return GR_ERR_ARG;
+  if (vocab > (1 << 30)) return GR_ERR_UNSUPPORTED;
+  LogprobParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.logits = logits;
+  p.ld = ld;
+  p.rows = rows;
+  p.vocab = vocab;
+  p.ids = ids;
+  p.temperature = temperature;
+  p.n_top = n_top;
+  p.logprob = logprob;
+  p.entropy = entropy;
+  p.rank = rank;
+  p.top_logprob = top_logprob;
+  p.top_ids = top_ids;
+  p.sms = num_sms();
+  p.status = status;
+  return launch_token_logprobs(p, is_bf16 != 0, static_cast<cudaStream_t>(stream), g_pdl) == cudaSuccess ? GR_OK
+                                                                                                         : GR_ERR_CUDA;
 }
 
 }  // extern "C"

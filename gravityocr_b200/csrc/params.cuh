@@ -130,6 +130,75 @@ struct OverrideParams {
   const int32_t* rounds;
 };
 
+struct KvWriteParams {
+  const __nv_bfloat16* qkv;
+  int64_t ld_qkv;
+  int m, n_q_heads, n_kv_heads;
+  int groups;              // warps that share a row's heads
+  int sms;
+  const __nv_bfloat16* q_norm;
+  const __nv_bfloat16* k_norm;
+  double eps;
+  const int32_t* row_pos;
+  const int32_t* row_pos3;
+  int mrope_s0, mrope_s1;
+  const float* inv_freq;
+  int rotary_dim;
+  const int64_t* row_slot;
+  int64_t n_slots;
+  __nv_bfloat16* q_out;
+  void* k;
+  void* v;
+  int8_t* k_exp;
+  int8_t* v_exp;
+  int32_t* status;
+};
+struct KvReadParams {
+  const void* k;
+  const void* v;
+  const int8_t* k_exp;
+  const int8_t* v_exp;
+  int n_kv_heads;
+  int64_t n_slots;
+  const int64_t* slots;
+  int64_t n;
+  __nv_bfloat16* k_out;
+  __nv_bfloat16* v_out;
+  int32_t* status;
+};
+struct KvAttnParams {
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  const int8_t* k_exp;
+  const int8_t* v_exp;
+  int n_pages;
+  const int32_t* page_table;
+  int pt_stride;
+  const int64_t* seq_lens;
+  int bs, K, draft, base_add, n_q_heads, n_kv_heads;
+  int chunk, max_splits, groups;
+  float scale_log2;
+  float* ws_o;
+  float* ws_ml;
+  int* ws_ticket;
+  int32_t* status;
+};
+struct LogprobParams {
+  const void* logits;
+  int64_t ld;
+  int rows, vocab;
+  const int64_t* ids;
+  const float* temperature;
+  int n_top;
+  float* logprob;
+  float* entropy;
+  int32_t* rank;
+  float* top_logprob;
+  int32_t* top_ids;
+  int sms;
+  int32_t* status;
+};
+
 // Host-side set-up that belongs to one device context (function attributes, occupancy answers): done once per device,
 // under a lock, by the first launch that runs with that device current.
 constexpr int kMaxDevices = 64;
@@ -190,6 +259,15 @@ cudaError_t launch_sample_rows(const SampleParams& p, cudaStream_t s);
 // Largest vocabulary sample_rows takes: a warp adds at most 4,095 entries per pass to its 32-bit bucket words.
 constexpr int kSampleMaxVocab = 65024;
 cudaError_t launch_penalty_cumulate(const SampleParams& p, cudaStream_t s);
+cudaError_t launch_qk_norm_rope_write(KvWriteParams p, int format, bool half, cudaStream_t s, bool pdl);
+cudaError_t launch_kv_read(const KvReadParams& p, int format, cudaStream_t s, bool pdl);
+size_t kv8_attention_ws_bytes(int bs, int rows, int n_kv_heads, int max_splits, size_t* o_off, size_t* ml_off);
+cudaError_t launch_kv8_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, KvAttnParams p, int format,
+                                 cudaStream_t stream, bool pdl);
+constexpr int kKv8TicketPairs = 16384;  // (request, K/V head) pairs of one call
+constexpr int kKv8MaxSplits = 128;
+cudaError_t launch_token_logprobs(const LogprobParams& p, bool bf16, cudaStream_t stream, bool pdl);
+constexpr int kLogprobMaxTop = 64;
 cudaError_t launch_pack_gate_up(const __nv_bfloat16* src, __nv_bfloat16* dst, int I, int H, cudaStream_t s);
 
 }  // namespace gr

@@ -273,6 +273,66 @@ int gr_commit_sampled(int bs, int K, const int32_t* am, const int32_t* accept, c
 int gr_penalty_cumulate(int bs, const int32_t* tokens, int stride, const int32_t* counts, int add,
                         const gr_sampling* s, void* stream);
 
+/* ------------------------------------------------------------------ 8-bit K/V cache
+ * A paged cache in bf16, or with 8-bit rows: a row is one (token, K/V head), 128 codes x_i and one exponent e, and stands
+ * for x_i * 2^e.  e is the smallest exponent in [-40, 40] with max|x| <= top * 2^e, top = 448 (e4m3) or 127 (int8);
+ * codes are x * 2^-e rounded half to even and saturated at +-top.  A row with a NaN or an infinity is stored as e = -128
+ * and zero codes and reads back as NaN.  No counterpart in the reference, whose cache dtype is the serving framework's. */
+enum gr_kv_format { GR_KV_BF16 = 0, GR_KV_E4M3 = 1, GR_KV_INT8 = 2 };
+
+/* One layer's cache.  Device pointers, 16-byte aligned. */
+typedef struct gr_kv_cache {
+  int format;             /* gr_kv_format */
+  int n_kv_heads;
+  int page_size;          /* 16 */
+  int64_t n_pages;
+  void* k;                /* [n_pages, n_kv_heads, 16, 128] bf16, or 1-byte codes */
+  void* v;
+  int8_t* k_exp;          /* [n_pages, n_kv_heads, 16]; NULL for GR_KV_BF16 */
+  int8_t* v_exp;
+} gr_kv_cache;
+
+/* From m projected rows qkv [m, ld_qkv] bf16 (q heads | k heads | v heads, 128 each; ld_qkv % 4 == 0, 8-byte aligned) in
+ * one pass: q and k heads take their RMS norm (q_norm / k_norm bf16 [128], or NULL for none), x * w / sqrt(mean x^2 + eps);
+ * then the rotation of their first rotary_dim elements (a multiple of 8, 0..128; rope_half 0: pairs (2i, 2i + 1); 1: pairs
+ * (i, i + rotary_dim / 2)) by the angle position * inv_freq[i], formed in 64 bits; q goes to q_out bf16 [m, n_q_heads *
+ * 128], k and v rows to the cache at row_slot (page * 16 + offset).  Positions are row_pos [m], or row_pos3 [m][3] with
+ * mrope_section (three pair counts, as gr_epilogue); both NULL only with rotary_dim 0.  A negative slot writes q only; a
+ * slot past the cache sets GR_ERR_BAD_PAGE and writes q only.  No two rows may share a slot.  Inputs and outputs may not
+ * overlap. */
+int gr_qk_norm_rope_write(const void* qkv, int64_t ld_qkv, int m, int n_q_heads, const gr_kv_cache* cache,
+                          const void* q_norm, const void* k_norm, double eps, const int32_t* row_pos,
+                          const int32_t* row_pos3, const int32_t* mrope_section, const float* inv_freq, int rotary_dim,
+                          int rope_half, const int64_t* row_slot, void* q_out, int32_t* status, void* stream);
+
+/* The rows at n slots, back in bf16 (exact for the 8-bit formats): k_out / v_out bf16 [n, n_kv_heads * 128].  A negative slot
+ * leaves its output rows as they are; a slot past the cache does too and sets GR_ERR_BAD_PAGE. */
+int gr_kv_read(const gr_kv_cache* cache, const int64_t* slots, int64_t n, void* k_out, void* v_out, int32_t* status,
+               void* stream);
+
+/* gr_bd_attention over an 8-bit cache (GR_KV_BF16 is GR_ERR_UNSUPPORTED: gr_bd_attention reads that): the same rows, masks
+ * (draft 0, 1, 2) and page tables.  K = 1 is one decode token.  A row that sees nothing (seq_lens[b] + base_add + j < 0: a
+ * padding request has seq_lens -K - base_add) gives zeros.  Lengths past the page table, and page ids past the cache, set
+ * GR_ERR_BAD_PAGE.  chunk: a multiple of 32; max_splits <= 128, chunk * max_splits >= the longest length + K.
+ * workspace: gr_kv8_attention_workspace_bytes, zero-filled once (needed for max_splits > 1), one call at a time. */
+size_t gr_kv8_attention_workspace_bytes(int bs, int K, int n_q_heads, int n_kv_heads, int max_splits);
+int gr_kv8_attention(const void* q, const gr_kv_cache* cache, const int32_t* page_table, int pt_stride,
+                     const int64_t* seq_lens, int bs, int K, int draft, int base_add, int n_q_heads, int chunk,
+                     int max_splits, void* out, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* Chunk and split count for requests of up to max_len tokens (the K rows included): out[0], out[1]. */
+int gr_kv8_attention_plan(int bs, int K, int max_len, int n_q_heads, int n_kv_heads, int32_t* out);
+
+/* Log probabilities of ids [rows] under softmax(logits / temperature): logprob [rows], rank [rows] (1 + the tokens that come
+ * before it, by logit, then by id), entropy [rows] (nats), and the n_top (0..64, <= vocab) best tokens, equal logits by id:
+ * top_logprob / top_ids [rows, n_top].  logits: fp32, or bf16 when is_bf16, [rows, ld], ld >= vocab; temperature [rows] > 0,
+ * or NULL for 1.  -inf logits (masked tokens) have probability 0.  id -1: no token asked (NaN, rank 0); any other id outside
+ * the vocabulary sets GR_ERR_BAD_ID.  A row with a NaN or +inf logit, or with every logit -inf, has no distribution: its
+ * outputs are NaN, rank 0, ids -1, and GR_ERR_NO_TOKEN is set; a temperature that is not > 0 gives the same with GR_ERR_ARG.
+ * The reference refuses requests that ask for log probabilities. */
+int gr_token_logprobs(const void* logits, int is_bf16, int64_t ld, int rows, int vocab, const int64_t* ids,
+                      const float* temperature, int n_top, float* logprob, float* entropy, int32_t* rank,
+                      float* top_logprob, int32_t* top_ids, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
