@@ -1,495 +1,691 @@
 // Attention of one to a few new tokens per request over the paged 8-bit K/V cache (rows as kv8_dev.cuh defines them), split
-// over the cache's length and joined.
+// over the cache's length and joined, on tcgen05 without unpacking a code.
 //
-// Rows of one request and one K/V head: the GQA group's G query heads x K window rows (row r = g * K + j), in m16 tiles;
-// visibility as in attention_dev.cuh (row_limit).  With one new token and G = 2 there are 2 rows: the work is reading
-// the cache, 258 bytes a token and head, so everything below serves that stream.
+// Rows of one request and one K/V head: the GQA group's G query heads x K window rows (row r = g * K + j); visibility as
+// in attention_dev.cuh (row_limit).  With one new token there are G rows: the work is reading the cache, 258 bytes per
+// token and head, so the kernel is built to add nothing to that stream.  Both products take the codes as they lie in
+// shared memory after TMA, as the tensor core's A operand, and the few query rows as its N side:
+//   S [128 tokens x N1] = K [128 tokens x 128] Q^T        A: K tile, K-major
+//   O [128 dims x N2]   = V^T [128 dims x 128 tokens] P^T  A: V tile, MN-major; P as its threads write it, MN-major
+// A TMEM lane is then a token (S) or a dimension (O): one thread per token does that token's softmax for every row, with
+// the token's two exponents as plain scalars, and one thread per dimension accumulates O in fp32 registers.
 //
-// A CTA covers cache positions [split * chunk, (split + 1) * chunk) of one (request, K/V head).  It is made of independent
-// warp groups, one warp per m16 tile of rows; a group owns a ring of 32-token stages (two pages: 4 KB of K codes, 4 KB of
-// V codes by 2-D TMA in the 128-byte swizzle, 64 bytes of exponents by bulk copies) and its own online softmax over the
-// tiles it takes, so no barrier joins the warps until the end.
+// The 8-bit B operands hold a row in several 8-bit parts, one column each, whose products are summed in fp32:
+//   e4m3  q = q0 + q1 / 16, exact to 2^-22 of the row's largest element (q has 8 significant bits, a part 4);
+//         p = p0 + p1 / 16 + p2 / 256, 2^-12 relative; accumulated in fp32.
+//   int8  q in three signed digits to base 256 (2^-22 of the row's largest element), p in two: 2^-16 of the tile's largest
+//         weight, accumulated exactly in int32 and added in fp32.
+//   (bf16 rounding of the output is 2^-9 relative.)
+// Scales: a row's q is brought to a fixed binade by a power of two; with a token's 2^ek, 2^ev:
+//   w = s * coef_r * 2^ek + ev (base 2),  M_r = max w,  p = 2^(w - M_r),  O = sum p code_v,  l = sum p 2^-ev,  out = O / l.
+// |ev| <= 40 keeps l: a token whose p underflows has a score 46 binades below the best.
 //
-// Codes become halves in registers (exact) right before mma.sync m16n8k16, f16 in, fp32 accumulated.  Which cache element a
-// lane holds is a free permutation of the products' inner index, so both operands are read with 16-byte shared loads
-// and no transposition beyond byte shuffles:
-//   S = Q K^T: the lane with quad index c holds dims 16c..16c+15 and 64+16c..64+16c+15 of its token (and of its two Q rows);
-//   O = P V:   it holds tokens c, c+4, c+8, c+12 of a page, exactly the columns of S it has, for 16 dims of one 16-dim chunk.
-// Conflict-free: the 8 lanes of a shared-load phase touch 8 different 16-byte chunks of the swizzled tile.
 //
-// Scales: a row's q is brought to [2^14, 2^15) by a power of two (halves hold it exactly down to 2^-28 of its largest
-// element), the key's 2^ek multiplies the score, and the value's 2^ev joins the softmax weight:
-//   w = s * scale * log2(e) + ev,  M = max w,  P = 2^(w - M + 15),  O = sum P code_v,  l = sum 2^(w - ev - M + 15),
-//   out = O / l.  P <= 2^15 is rounded to half: 2^-12 relative down to 2^-29 of the largest weight, and the tokens that
-//   fall below 2^-40 of it add nothing.  l's terms stay within fp32: |ev| <= 40.
+// P is measured from its own tile's maximum T_r, not the running one: its parts then resolve the tile's weights whatever the
+// rest of the sequence holds (a first token that takes most of the attention would otherwise push every later weight
+// below int8's two digits), and O and l take a tile in fp32 with the factor 2^(T_r - M_r).
+//
+// CTA: (split, K/V head and block of at most 40 rows, request).  One thread per token (then per dimension) and row group: up
+// to 16 rows four warps take all of them, above that eight warps take half the rows each.  One warp issues the MMAs, one the
+// TMA copies (8 pages a 128-token tile, 2 KB of K and 2 KB of V each; ~85 cycles an issue, which on the MMA warp would sit
+// between a tile's two products).  Per tile: S -> weights -> P to shared memory -> O -> registers.  K and V have rings of
+// their own, so a tile's K half is refilled as soon as its scores exist, and the two or three CTAs of an SM cover each
+// other's latencies.
 #include "kv8_dev.cuh"
 
 namespace gr {
 
-constexpr int kQTile = 32;                                  // tokens per stage: two pages
-constexpr int kQStageBytes = 2 * kQTile * 128;              // K codes, V codes
-constexpr int kQExpBytes = 2 * kQTile;                      // K exponents, V exponents
-constexpr int kQStages = 3;
-constexpr int kQMaxWarps = 8;
-constexpr size_t kQTicketBytes = 65536;                     // tickets of 16384 (request, K/V head) pairs
+constexpr int kQTile = 128;                                 // tokens per tile: eight pages
+constexpr int kQHalf = kQTile * 128;                        // K or V codes of a tile
+constexpr int kQStages = 2;                                 // K and V rings (the product barriers are as many)
+constexpr int kQMaxRows = 40;                               // rows of a CTA
+constexpr size_t kQTicketBytes = kKv8TicketPairs * sizeof(int);
 
-__device__ __forceinline__ void mma_16816_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void bulk_load16(void* dst, const void* src, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];" ::"r"(
-                   smem_u32(dst)),
-               "l"(reinterpret_cast<uint64_t>(src)), "r"(smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-// Two codes (bytes 2h, 2h + 1 of w) as a half2.
-template <int FMT, int H>
-__device__ __forceinline__ uint32_t kv_half2(uint32_t w) {
-  if (FMT == GR_KV_E4M3) return e4m3x2_to_half2(H ? w >> 16 : w);
-  const uint32_t a = __byte_perm(w, 0x64646464u, H ? 0x4342 : 0x4140);  // w holds x ^ 0x80 bytes
-  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&a), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <int FMT>
-__device__ __forceinline__ uint32_t kv_biased(uint32_t w) {
-  return FMT == GR_KV_INT8 ? w ^ 0x80808080u : w;
-}
-
-struct KvAttnSmem {  // offsets from the 1024-aligned start
-  int ring, exps, scales, bars, total;
+// RT rows in H groups of RH.  Columns: S has part k of row r at group * q_parts * RH + k * RH + r (within its group), P
+// likewise with every group padded to 16 columns.
+template <int FMT, int RT, int H>
+struct KvAttnShape {
+  static constexpr int RH = RT / H;
+  static constexpr int q_parts = FMT == GR_KV_E4M3 ? 2 : 3;
+  static constexpr int p_parts = FMT == GR_KV_E4M3 ? 3 : 2;
+  static constexpr int p_cols = (p_parts * RH + 15) / 16 * 16;
+  static constexpr int n1 = (q_parts * RT + 15) / 16 * 16;
+  static constexpr int n2 = p_cols * H;
+  static constexpr int tmem_cols = n1 + n2 <= 32 ? 32 : (n1 + n2 <= 64 ? 64 : (n1 + n2 <= 128 ? 128 : 256));
+  static constexpr int threads = 128 * H + 64;
+  static constexpr int ctas = RT > 16 ? 2 : 3;              // per SM
+  // shared memory, from a 1024-aligned start
+  static constexpr int k = 0;
+  static constexpr int v = k + kQStages * kQHalf;
+  static constexpr int q = v + kQStages * kQHalf;           // [n1][128], 128-byte swizzle
+  static constexpr int p = q + n1 * 128;                    // [n2 / 16][128 tokens][16]
+  static constexpr int xm = p + n2 * 128;                   // [RT][4] warp maxima of a tile; at the end, warp sums of l
+  static constexpr int coef = xm + RT * 16;                 // [RT] score scale
+  static constexpr int ref = coef + RT * 4;                 // [RT] off - T_r
+  static constexpr int alpha = ref + RT * 4;                // [RT] factor of the sums so far
+  static constexpr int beta = alpha + RT * 4;               // [RT] factor of the tile's sums
+  static constexpr int lim = beta + RT * 4;                 // [RT] row limits
+  static constexpr int pages = lim + RT * 4;                // [kKv8MaxChunk / 16] first code row of each page
+  static constexpr int bars = (pages + kKv8MaxChunk / 4 + 15) / 16 * 16;
+  static constexpr int bytes = 1024 + bars + (2 * kQStages + 5) * 8 + 16;
+  static_assert(RH % 4 == 0 && n1 <= 256 && n1 + n2 <= 256, "rows are handled by fours");
 };
-__host__ __device__ inline KvAttnSmem kv_attn_smem(int groups, int n_mt) {
-  KvAttnSmem s;
-  const int ring = groups * kQStages * kQStageBytes;
-  const int merge = groups * n_mt * 16 * 130 * 4;  // O [rows][128], m and l, of every group (reuses the ring)
-  s.ring = 0;
-  s.exps = ring > merge ? ring : (merge + 1023) / 1024 * 1024;
-  s.scales = s.exps + groups * kQStages * kQExpBytes;
-  s.bars = s.scales + groups * n_mt * kQTile * 8;
-  s.total = s.bars + groups * kQStages * 16 + 16;
-  return s;
+
+// One thread of the warp, the same each time; all 32 lanes take part.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+template <int FMT>
+__device__ __forceinline__ void tc_mma_codes(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  if (FMT == GR_KV_E4M3)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Instruction descriptor of the 8-bit kinds: fp32 / int32 result, e4m3 or signed 8-bit inputs, M = 128; both operands
+// K-major or both MN-major.
+template <int FMT>
+__device__ constexpr uint32_t idesc_codes(int n, bool mn) {
+  return (FMT == GR_KV_E4M3 ? (1u << 4) : ((2u << 4) | (1u << 7) | (1u << 10))) | (mn ? (1u << 15) | (1u << 16) : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// N consecutive TMEM columns of this thread's lane (N a multiple of 4); wait with tmem_ld_done.
+template <int N>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t addr, uint32_t* r) {
+  if constexpr (N >= 16) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+    if constexpr (N > 16) tmem_ld_cols<N - 16>(addr + 16, r + 16);
+  } else if constexpr (N >= 8) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
+    if constexpr (N > 8) tmem_ld_cols<N - 8>(addr + 8, r + 8);
+  } else {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+  }
+}
+// Completes this thread's TMEM loads; no use of r can be scheduled before it.
+template <int N>
+__device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+// 1.5 * 2^23 + x as a float, |x| < 2^22: an integer becomes a float by an addition (the conversion unit is 8 times slower).
+constexpr float kIntBias = 12582912.f;
+__device__ __forceinline__ float int_biased(uint32_t x) { return __uint_as_float(x + 0x4B400000u); }
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));  // NaNs are ignored
+  return r;
+}
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ bool named_any(int id, int threads, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(x)), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+// MN-major operand without a swizzle: [16 MN elements][K index] blocks, each K index 16 bytes; 128 bytes to the next 8 K
+// indices (leading), block_bytes to the next 16 MN elements (stride).
+__device__ __forceinline__ uint64_t smem_desc_mn16(uint32_t addr, uint32_t block_bytes) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(128 >> 4) << 16) |
+         (static_cast<uint64_t>(block_bytes >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+// Four q values, scaled into the format's binade, to q_parts words of four codes.
+template <int FMT>
+__device__ __forceinline__ void split_q(const float (&x)[4], uint32_t* part) {
+  if (FMT == GR_KV_E4M3) {  // |x| < 256
+    part[0] = kv_pack<GR_KV_E4M3>(x);
+    float rest[4];
+    const uint32_t h01 = e4m3x2_to_half2(part[0]), h23 = e4m3x2_to_half2(part[0] >> 16);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h01));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&h23));
+    rest[0] = (x[0] - a.x) * 16.f;
+    rest[1] = (x[1] - a.y) * 16.f;
+    rest[2] = (x[2] - b.x) * 16.f;
+    rest[3] = (x[3] - b.y) * 16.f;
+    part[1] = kv_pack<GR_KV_E4M3>(rest);
+  } else {  // |x| < 2^22: digits in [-128, 127]
+    part[0] = part[1] = part[2] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t t = (static_cast<uint32_t>(__float2int_rn(x[i])) + 0x808080u) ^ 0x808080u;
+      part[0] |= ((t >> 16) & 0xffu) << (8 * i);
+      part[1] |= ((t >> 8) & 0xffu) << (8 * i);
+      part[2] |= (t & 0xffu) << (8 * i);
+    }
+  }
 }
 
-template <int FMT>
-__global__ void __launch_bounds__(32 * kQMaxWarps) kv8_attention_kernel(const __grid_constant__ CUtensorMap tmk,
-                                                                       const __grid_constant__ CUtensorMap tmv,
-                                                                       const KvAttnParams p) {
+template <int FMT, int RT, int H>
+__global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_kernel(
+    const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const KvAttnParams p) {
+  using Sh = KvAttnShape<FMT, RT, H>;
+  constexpr int RH = Sh::RH;
+  constexpr int kMmaWarp = 4 * H, kCopyWarp = kMmaWarp + 1, kSoft = 128 * H;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-  const int G = p.n_q_heads / p.n_kv_heads;
-  const int R = G * p.K;
-  const int n_mt = (R + 15) / 16;
-  const int R_pad = n_mt * 16;
-  const int NG = p.groups;
-  const KvAttnSmem lay = kv_attn_smem(NG, n_mt);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int grp = warp / n_mt, mt = warp - grp * n_mt;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + lay.bars) + grp * kQStages;
-  uint64_t* empty = full + NG * kQStages;
-  int* flag = reinterpret_cast<int*>(smem + lay.bars + NG * kQStages * 16);
-  if (mt == 0 && lane == 0) {
-    for (int s = 0; s < kQStages; ++s) {
-      mbar_init(full + s, 1);
-      mbar_init(empty + s, n_mt);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + Sh::bars);
+  uint64_t* v_full = k_full + kQStages;
+  uint64_t* s_full = v_full + kQStages;
+  // products completed, one barrier per stage parity: a waiter two tiles behind must not mistake the phase
+  uint64_t* o_full = s_full + 2;
+  uint64_t* p_full = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_full + 1);
+  int* flag = reinterpret_cast<int*>(tmem_slot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < 2 * kQStages; ++s) mbar_init(k_full + s, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(s_full + s, 1);
+      mbar_init(o_full + s, 1);
     }
+    mbar_init(p_full, kMmaWarp);
     fence_mbar_init();
-  }
-  if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmk);
     tma_prefetch_desc(&tmv);
-    pdl_trigger();
   }
+  // TMEM is taken before the dependent launch is released: a CTA of a later kernel (which may wait for this grid) can
+  // then never hold the columns this CTA is waiting for
+  if (warp == kMmaWarp) tmem_alloc(tmem_slot, Sh::tmem_cols);
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (tid == 0) pdl_trigger();
   pdl_wait();
 
+  const int split = blockIdx.x, b = blockIdx.z;
+  const int kvh = blockIdx.y / p.row_blocks, blk = blockIdx.y - kvh * p.row_blocks;
+  const int G = p.n_q_heads / p.n_kv_heads;
+  const int R_all = G * p.K;
+  const int r0 = blk * p.rows_per_block;
+  const int R = min(p.rows_per_block, R_all - r0);  // this CTA's rows r0 .. r0 + R - 1
   const int64_t base64 = p.seq_lens[b] + p.base_add;
   const int64_t cap = static_cast<int64_t>(p.pt_stride) * 16;
   const int64_t end64 = base64 + p.K;
-  if (end64 > cap && threadIdx.x == 0 && split == 0) report(p.status, GR_ERR_BAD_PAGE);
+  if (end64 > cap && tid == 0 && split == 0) report(p.status, GR_ERR_BAD_PAGE);
   const int base = static_cast<int>(min(max(base64, static_cast<int64_t>(-p.K)), cap));
   const int L = static_cast<int>(min(max(end64, static_cast<int64_t>(0)), cap));  // the last row's limit
-  const int n_active = max(1, (L + p.chunk - 1) / p.chunk);
-  if (split >= n_active) return;
+  const int n_active = min(p.max_splits, max(1, (L + p.chunk - 1) / p.chunk));
+  const bool active = split < n_active;  // uniform over the CTA
   const int kv_beg = split * p.chunk;
   const int kv_end = min(L, kv_beg + p.chunk);
-  const int n_tiles = kv_end > kv_beg ? (kv_end - kv_beg + kQTile - 1) / kQTile : 0;
-  const int my_tiles = n_tiles > grp ? (n_tiles - grp + NG - 1) / NG : 0;
-  const int* pt = p.page_table + static_cast<int64_t>(b) * p.pt_stride;
-  const int last_page = (L - 1) >> 4;
-
-  // ---- producer: lanes 0-7 of the group's first warp issue a stage (K and V tiles of two pages, their exponents)
-  uint8_t* ring = smem + lay.ring + grp * kQStages * kQStageBytes;
-  uint8_t* exps = smem + lay.exps + grp * kQStages * kQExpBytes;
-  const bool producer = mt == 0;
-  auto page_of = [&](int i) {  // page id of this lane's copy in the group's tile i (in range: checked here)
-    if (!producer || lane >= 8 || i >= my_tiles) return 0;
-    const int slot = min(((kv_beg + (grp + i * NG) * kQTile) >> 4) + (lane & 1), last_page);
-    const int pg = __ldg(pt + slot);
-    if (static_cast<unsigned>(pg) >= static_cast<unsigned>(p.n_pages)) {
-      report(p.status, GR_ERR_BAD_PAGE);
-      return 0;
-    }
-    return pg;
-  };
-  auto issue = [&](int i, int pg) {
-    const int st = i % kQStages;
-    if (lane == 0) mbar_arrive_expect_tx(full + st, kQStageBytes + kQExpBytes);
-    __syncwarp();
-    uint8_t* stage = ring + st * kQStageBytes;
-    const int half = lane & 1;
-    const int64_t row = (static_cast<int64_t>(pg) * p.n_kv_heads + kvh) * 16;
-    if (lane < 2) tma_load_2d(stage + half * 2048, &tmk, full + st, 0, static_cast<int>(row));
-    else if (lane < 4) tma_load_2d(stage + kQTile * 128 + half * 2048, &tmv, full + st, 0, static_cast<int>(row));
-    else if (lane < 6) bulk_load16(exps + st * kQExpBytes + half * 16, p.k_exp + row, full + st);
-    else if (lane < 8) bulk_load16(exps + st * kQExpBytes + kQTile + half * 16, p.v_exp + row, full + st);
-  };
-  if (producer) {
-    for (int i = 0; i < kQStages - 1; ++i)
-      if (i < my_tiles) issue(i, page_of(i));
-  }
-  int next_page = page_of(kQStages - 1);
-
-  // ---- this lane's two query rows, as halves
-  const int c = lane & 3, n = lane >> 2;
-  const int j0 = mt * 16 + n;
-  uint32_t qf[2][16];   // [row][k-step * 2 + half of the step's 4 dims]
-  float coef[2];
-  int lim[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = j0 + 8 * h;
-    const int g = r / p.K, j = r - g * p.K;
-    float x[32];
-    if (r < R) {
-      const __nv_bfloat16* src = p.q + ((static_cast<int64_t>(b) * p.K + j) * p.n_q_heads + kvh * G + g) * 128;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src + (u >> 1) * 64 + c * 16) + (u & 1));
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[u * 8 + 2 * e] = __uint_as_float(w[e] << 16);
-          x[u * 8 + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-        }
-      }
-      lim[h] = p.draft ? ((j == 0 && p.draft == 1) ? base + 1 : base + p.K) : base + j + 1;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) x[e] = 0.f;
-      lim[h] = L;
-    }
-    uint32_t am = 0;
-#pragma unroll
-    for (int e = 0; e < 32; ++e) am = max(am, __float_as_uint(x[e]) & 0x7fffffffu);
-    am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
-    am = max(am, __shfl_xor_sync(0xffffffffu, am, 2));
-    const int sh = max(-112, min(112, static_cast<int>(am >> 23) - 127 - 14));  // q * 2^-sh lies in [2^14, 2^15)
-    const float f = exp2i(-sh);
-    coef[h] = exp2i(sh) * p.scale_log2;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) qf[h][e] = pack_half(x[2 * e] * f, x[2 * e + 1] * f);
-  }
-  const int min_lim = p.draft == 2 ? base + p.K : base + 1;
-
-  float o[16][4];
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float2* scales = reinterpret_cast<float2*>(smem + lay.scales) + warp * kQTile;
-  const int krow = (n >> 1) + (n & 1) * 4;                 // the token (of 8) this lane's K column stands for
-  const int vchunk = (n >> 1) | ((n & 1) << 2);            // the 16-dim chunk this lane's V column stands for
-  bool dead = false;
-
-  for (int i = 0; i < my_tiles; ++i) {
-    const int st = i % kQStages;
-    // refill the stage of the tile before this one, once every warp of the group has read it
-    if (producer && i + kQStages - 1 < my_tiles) {
-      const int nx = i + kQStages - 1;
-      if (i > 0 && n_mt > 1 && !mbar_wait(empty + nx % kQStages, ((i - 1) / kQStages) & 1, p.status, GR_ERR_TIMEOUT))
-        dead = true;
-      __syncwarp();
-      issue(nx, next_page);
-      next_page = page_of(nx + 1);
-    }
-    if (!mbar_wait(full + st, (i / kQStages) & 1, p.status, GR_ERR_TIMEOUT)) dead = true;
-    const uint8_t* kt = ring + st * kQStageBytes;
-    const uint8_t* vt = kt + kQTile * 128;
-    const int8_t* et = reinterpret_cast<const int8_t*>(exps + st * kQExpBytes);
-    const int t0 = kv_beg + (grp + i * NG) * kQTile;
-    const bool partial = t0 + kQTile > min(min_lim, kv_end);
-    {
-      const int ev = et[kQTile + lane];
-      scales[lane] = make_float2(kv_scale(et[lane]), ev == kKvExpBad ? __int_as_float(0x7fc00000) : static_cast<float>(ev));
-    }
-    __syncwarp();
-
-    // S: 4 column tiles of 8 tokens
-    float s[4][4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
-      const int row = t * 8 + krow;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(kt + sw128(row, c + 4 * h));
-        const uint32_t w[4] = {kv_biased<FMT>(raw.x), kv_biased<FMT>(raw.y), kv_biased<FMT>(raw.z),
-                               kv_biased<FMT>(raw.w)};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int ks = h * 4 + e;
-          const uint32_t a[4] = {qf[0][2 * ks], qf[1][2 * ks], qf[0][2 * ks + 1], qf[1][2 * ks + 1]};
-          mma_16816_f16(s[t], a, kv_half2<FMT, 0>(w[e]), kv_half2<FMT, 1>(w[e]));
-        }
-      }
-    }
-    // weights: w = s * coef * 2^ek + ev; column e of tile t is token t * 8 + c + 4 * (e & 1), row e >> 1
-    float ev[4][2];
-    float mx[2] = {m[0], m[1]};
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float2 f = scales[t * 8 + c + 4 * e];
-        ev[t][e] = f.y;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float w = fmaf(s[t][2 * h + e], coef[h] * f.x, f.y);
-          if (partial) {
-            const int tok = t0 + t * 8 + c + 4 * e;
-            if (tok >= lim[h] || tok >= kv_end) w = -INFINITY;
-          }
-          s[t][2 * h + e] = w;
-          mx[h] = fmaxf(mx[h], w);
-        }
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-    }
-    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float al = m[h] == -INFINITY ? 0.f : ex2_approx(m[h] - mx[h]);
-        m[h] = mx[h];
-        l[h] *= al;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          o[x][2 * h] *= al;
-          o[x][2 * h + 1] *= al;
-        }
-      }
-    }
-    const float r0 = (m[0] == -INFINITY ? 0.f : m[0]) - 15.f, r1 = (m[1] == -INFINITY ? 0.f : m[1]) - 15.f;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float w0 = s[t][e] - r0, w1 = s[t][2 + e] - r1;
-        float l0 = ex2_approx(w0 - ev[t][e]), l1 = ex2_approx(w1 - ev[t][e]);
-        if (partial) {  // a hidden token's exponent may be that of a bad row, or of no row
-          if (w0 == -INFINITY) l0 = 0.f;
-          if (w1 == -INFINITY) l1 = 0.f;
-        }
-        l[0] += l0;
-        l[1] += l1;
-        s[t][e] = ex2_approx(w0);
-        s[t][2 + e] = ex2_approx(w1);
-      }
-    }
-    // O += P V, a page (16 tokens) at a time
-#pragma unroll
-    for (int pg = 0; pg < 2; ++pg) {
-      uint32_t a[4];
-      a[0] = pack_half(s[2 * pg][0], s[2 * pg][1]);
-      a[1] = pack_half(s[2 * pg][2], s[2 * pg][3]);
-      a[2] = pack_half(s[2 * pg + 1][0], s[2 * pg + 1][1]);
-      a[3] = pack_half(s[2 * pg + 1][2], s[2 * pg + 1][3]);
-      uint4 raw[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int row = pg * 16 + u * 4 + c;
-        raw[u] = *reinterpret_cast<const uint4*>(vt + sw128(row, vchunk));
-        if (partial && t0 + row >= kv_end) raw[u] = make_uint4(0, 0, 0, 0);  // unwritten slots: any bytes, NaN codes too
-      }
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t v0 = kv_biased<FMT>(w == 0 ? raw[0].x : (w == 1 ? raw[0].y : (w == 2 ? raw[0].z : raw[0].w)));
-        const uint32_t v1 = kv_biased<FMT>(w == 0 ? raw[1].x : (w == 1 ? raw[1].y : (w == 2 ? raw[1].z : raw[1].w)));
-        const uint32_t v2 = kv_biased<FMT>(w == 0 ? raw[2].x : (w == 1 ? raw[2].y : (w == 2 ? raw[2].z : raw[2].w)));
-        const uint32_t v3 = kv_biased<FMT>(w == 0 ? raw[3].x : (w == 1 ? raw[3].y : (w == 2 ? raw[3].z : raw[3].w)));
-        // bytes (dim, token pair): x holds dims 0, 1 of tokens c, c+4, y of tokens c+8, c+12
-        const uint32_t x0 = __byte_perm(v0, v1, 0x5140), y0 = __byte_perm(v2, v3, 0x5140);
-        const uint32_t x1 = __byte_perm(v0, v1, 0x7362), y1 = __byte_perm(v2, v3, 0x7362);
-        mma_16816_f16(o[4 * w], a, kv_half2<FMT, 0>(x0), kv_half2<FMT, 0>(y0));
-        mma_16816_f16(o[4 * w + 1], a, kv_half2<FMT, 1>(x0), kv_half2<FMT, 1>(y0));
-        mma_16816_f16(o[4 * w + 2], a, kv_half2<FMT, 0>(x1), kv_half2<FMT, 0>(y1));
-        mma_16816_f16(o[4 * w + 3], a, kv_half2<FMT, 1>(x1), kv_half2<FMT, 1>(y1));
-      }
-    }
-    __syncwarp();
-    if (n_mt > 1 && lane == 0) mbar_arrive(empty + st);
-  }
-  if (dead && producer) {  // a wait ran out: give the copies in flight another limit each before the ring is reused
-    for (int i = max(0, my_tiles - kQStages); i < my_tiles; ++i)
-      mbar_wait(full + i % kQStages, (i / kQStages) & 1, p.status, GR_ERR_TIMEOUT);
-  }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-  }
-
-  // ---- join the groups through shared memory (the ring is idle)
-  __syncthreads();
-  float* part = reinterpret_cast<float*>(smem + lay.ring);      // [NG][R_pad][128]
-  float* part_ml = part + NG * R_pad * 128;                     // [NG][R_pad][2]
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float* dst = part + (grp * R_pad + j0 + 8 * h) * 128;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      *reinterpret_cast<float4*>(dst + c * 16 + u * 4) =
-          make_float4(o[4 * u][2 * h], o[4 * u + 1][2 * h], o[4 * u + 2][2 * h], o[4 * u + 3][2 * h]);
-      *reinterpret_cast<float4*>(dst + 64 + c * 16 + u * 4) =
-          make_float4(o[4 * u][2 * h + 1], o[4 * u + 1][2 * h + 1], o[4 * u + 2][2 * h + 1], o[4 * u + 3][2 * h + 1]);
-    }
-    if (c == 0) {
-      part_ml[(grp * R_pad + j0 + 8 * h) * 2] = m[h];
-      part_ml[(grp * R_pad + j0 + 8 * h) * 2 + 1] = l[h];
-    }
-  }
-  __syncthreads();
-  const int nthr = blockDim.x;
+  const int n_tiles = active && kv_end > kv_beg ? (kv_end - kv_beg + kQTile - 1) / kQTile : 0;
   const int64_t slot0 = (static_cast<int64_t>(b) * p.n_kv_heads + kvh) * p.max_splits;
-  auto store_out = [&](int r, int d4, float4 a, float inv) {
-    const int g = r / p.K, j = r - g * p.K;
-    __nv_bfloat16* dst = p.out + ((static_cast<int64_t>(b) * p.K + j) * p.n_q_heads + kvh * G + g) * 128 + d4 * 4;
-    uint2 pk;
-    pk.x = pack_bf16(a.x * inv, a.y * inv);
-    pk.y = pack_bf16(a.z * inv, a.w * inv);
-    *reinterpret_cast<uint2*>(dst) = pk;
-  };
-  for (int it = threadIdx.x; it < R * 32; it += nthr) {
-    const int r = it >> 5, d4 = it & 31;
-    float M = -INFINITY;
-    for (int g = 0; g < NG; ++g) M = fmaxf(M, part_ml[(g * R_pad + r) * 2]);
-    const float Ms = M == -INFINITY ? 0.f : M;
-    float lsum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int g = 0; g < NG; ++g) {
-      const float w = ex2_approx(part_ml[(g * R_pad + r) * 2] - Ms);
-      const float4 v = *reinterpret_cast<const float4*>(part + (g * R_pad + r) * 128 + d4 * 4);
-      lsum += w * part_ml[(g * R_pad + r) * 2 + 1];
-      acc.x += w * v.x;
-      acc.y += w * v.y;
-      acc.z += w * v.z;
-      acc.w += w * v.w;
+
+  // ---- first code row of each of the chunk's pages; page ids are checked here
+  int* pages = reinterpret_cast<int*>(smem + Sh::pages);
+  for (int k = tid; k < n_tiles * 8; k += Sh::threads) {
+    int id = (kv_beg >> 4) + k <= (kv_end - 1) >> 4
+                 ? __ldg(p.page_table + static_cast<int64_t>(b) * p.pt_stride + (kv_beg >> 4) + k) : 0;
+    if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.n_pages)) {
+      report(p.status, GR_ERR_BAD_PAGE);
+      id = 0;
     }
-    if (n_active == 1) {
-      store_out(r, d4, acc, lsum == 0.f ? 0.f : 1.f / lsum);
-    } else {
-      __stcg(reinterpret_cast<float4*>(p.ws_o + ((slot0 + split) * R_pad + r) * 128) + d4, acc);
-      if (d4 == 0) __stcg(reinterpret_cast<float2*>(p.ws_ml) + (slot0 + split) * R_pad + r, make_float2(M, lsum));
-    }
+    pages[k] = (id * p.n_kv_heads + kvh) * 16;
   }
-  if (n_active == 1) return;
+  if (active && warp < kMmaWarp) {
+    // ---- query rows to shared memory, in parts: a warp per row, every load ahead of the first use
+    float* coef = reinterpret_cast<float*>(smem + Sh::coef);
+    int* lim = reinterpret_cast<int*>(smem + Sh::lim);
+    constexpr int per_warp = (RT + kMmaWarp - 1) / kMmaWarp;
+    uint2 raw[per_warp];
+#pragma unroll
+    for (int u = 0; u < per_warp; ++u) {
+      const int r = warp + u * kMmaWarp;
+      raw[u] = make_uint2(0u, 0u);
+      if (r < R) {
+        const int g = (r0 + r) / p.K, j = (r0 + r) - g * p.K;
+        raw[u] = __ldg(reinterpret_cast<const uint2*>(
+            p.q + ((static_cast<int64_t>(b) * p.K + j) * p.n_q_heads + kvh * G + g) * 128) + lane);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < per_warp; ++u) {
+      const int r = warp + u * kMmaWarp;
+      if (r >= RT) break;
+      float x[4] = {__uint_as_float(raw[u].x << 16), __uint_as_float(raw[u].x & 0xffff0000u),
+                    __uint_as_float(raw[u].y << 16), __uint_as_float(raw[u].y & 0xffff0000u)};
+      uint32_t am = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) am = max(am, __float_as_uint(x[i]) & 0x7fffffffu);
+      am = __reduce_max_sync(0xffffffffu, am);
+      // the largest |q| to [2^7, 2^8) (e4m3) or [2^21, 2^22) (int8); a row with a NaN or an infinity scores NaN
+      const int sh = max(-100, min(100, static_cast<int>(am >> 23) - 127 - (FMT == GR_KV_E4M3 ? 7 : 21)));
+      const float f = am >= 0x7f800000u ? 0.f : exp2i(-sh);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = f == 0.f ? 0.f : x[i] * f;
+      uint32_t part[3];
+      split_q<FMT>(x, part);
+#pragma unroll
+      for (int k = 0; k < Sh::q_parts; ++k) {
+        const int col = (r / RH) * Sh::q_parts * RH + k * RH + r % RH;
+        *reinterpret_cast<uint32_t*>(smem + Sh::q + sw128(col, lane >> 2) + (lane & 3) * 4) = part[k];
+      }
+      if (lane == 0) {
+        const int j = (r0 + r) % p.K;
+        coef[r] = f == 0.f ? __int_as_float(0x7fc00000) : exp2i(sh) * p.scale_log2;
+        lim[r] = r < R ? min(kv_end, p.draft ? ((j == 0 && p.draft == 1) ? base + 1 : base + p.K) : base + j + 1) : 0;
+      }
+    }
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+
+  if (warp == kCopyWarp) {
+    // ---- copies, by one elected thread (the compiler keeps their operands uniform)
+    const int n_pages = (kv_end - kv_beg + 15) >> 4;
+    auto copy = [&](const CUtensorMap* map, int at, uint64_t* bars, int i) {
+      if (elect_one()) {
+        uint64_t* bar = bars + i % kQStages;
+        const int n = min(8, n_pages - i * 8);
+        mbar_arrive_expect_tx(bar, n * 2048);
+        uint8_t* dst = smem + at + (i % kQStages) * kQHalf;
+        const int4 a = *reinterpret_cast<const int4*>(pages + i * 8), c = *reinterpret_cast<const int4*>(pages + i * 8 + 4);
+        const int row[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < n) tma_load_2d(dst + k * 2048, map, bar, 0, row[k]);
+      }
+      __syncwarp();
+    };
+    int nk = 0, nv = 0;  // tiles whose copies are issued
+    for (bool ok = true; ok && nv < n_tiles;) {
+      // a K stage is free once its tile's scores exist, a V stage once its tile's second product has completed
+      if (nk >= kQStages) ok = mbar_wait(s_full + (nk & 1), ((nk - 2) >> 1) & 1, p.status, GR_ERR_TIMEOUT);
+      if (ok) copy(&tmk, Sh::k, k_full, nk++);
+      if (ok && nv >= kQStages) ok = mbar_wait(o_full + (nv & 1), ((nv - 2) >> 1) & 1, p.status, GR_ERR_TIMEOUT);
+      if (ok) copy(&tmv, Sh::v, v_full, nv++);
+    }
+    // no copy may still be landing in shared memory when the CTA leaves (after a wait that ran out, too)
+    for (int i = max(0, nk - kQStages); i < nk; ++i)
+      mbar_wait(k_full + i % kQStages, (i / kQStages) & 1, p.status, GR_ERR_TIMEOUT);
+    for (int i = max(0, nv - kQStages); i < nv; ++i)
+      mbar_wait(v_full + i % kQStages, (i / kQStages) & 1, p.status, GR_ERR_TIMEOUT);
+  } else if (warp == kMmaWarp) {
+    // ---- MMAs, by one elected thread
+    bool ok = true;
+    constexpr uint32_t id_s = idesc_codes<FMT>(Sh::n1, false), id_o = idesc_codes<FMT>(Sh::n2, true);
+    const uint64_t kd = smem_desc_sw128(smem_u32(smem + Sh::k));
+    const uint64_t vd = smem_desc_sw128_mn(smem_u32(smem + Sh::v), kQHalf);
+    const uint64_t qd = smem_desc_sw128(smem_u32(smem + Sh::q));
+    const uint64_t pd = smem_desc_mn16(smem_u32(smem + Sh::p), kQTile * 16);
+    for (int i = 0; i < n_tiles; ++i) {
+      const uint32_t so = (static_cast<uint32_t>(i % kQStages) * kQHalf) >> 4;
+      ok = ok && mbar_wait(k_full + i % kQStages, (i / kQStages) & 1, p.status, GR_ERR_TIMEOUT);
+      tc_fence_after();
+      if (ok && elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // 32 dims a step: 32 bytes of a row
+          tc_mma_codes<FMT>(tmem, kd + so + 2 * k, qd + 2 * k, id_s, k != 0);
+        tc_commit(s_full + (i & 1));
+      }
+      __syncwarp();
+      ok = ok && mbar_wait(v_full + i % kQStages, (i / kQStages) & 1, p.status, GR_ERR_TIMEOUT);
+      ok = ok && mbar_wait(p_full, i & 1, p.status, GR_ERR_TIMEOUT);
+      tc_fence_after();
+      if (ok && elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // 32 tokens a step: 4 KB of V rows, 512 bytes of P
+          tc_mma_codes<FMT>(tmem + Sh::n1, vd + so + 256 * k, pd + 32 * k, id_o, k != 0);
+        tc_commit(o_full + (i & 1));
+      }
+      __syncwarp();
+    }
+  } else if (active) {
+    // ---- one thread per token (weights), then per dimension (output), for the rows of its group
+    const int t128 = tid & 127, grp = H == 1 ? 0 : warp >> 2, rb = grp * RH;
+    const float* coef = reinterpret_cast<const float*>(smem + Sh::coef) + rb;
+    const int* lim = reinterpret_cast<const int*>(smem + Sh::lim) + rb;
+    float* refs = reinterpret_cast<float*>(smem + Sh::ref);
+    float* alphas = reinterpret_cast<float*>(smem + Sh::alpha);
+    float* betas = reinterpret_cast<float*>(smem + Sh::beta);
+    float* xm = reinterpret_cast<float*>(smem + Sh::xm);
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t t_s = t_lane + grp * Sh::q_parts * RH, t_o = t_lane + Sh::n1 + grp * Sh::p_cols;
+    uint8_t* ps = smem + Sh::p + grp * Sh::p_cols * kQTile;
+    constexpr float off = FMT == GR_KV_E4M3 ? 8.f : 14.994309f;  // weights up to 2^8, or 32639 (two digits' largest)
+    const int min_lim = min(kv_end, p.draft == 2 ? base + p.K : base + 1);
+    float o[RH], l[RH];
+#pragma unroll
+    for (int r = 0; r < RH; ++r) o[r] = l[r] = 0.f;
+    // this token's exponents, loaded a tile ahead
+    int next_ek = 0, next_ev = 0;
+    auto load_exps = [&](int i) {
+      const int t = i * kQTile + t128;
+      if (kv_beg + t < kv_end) {
+        const int at = pages[t >> 4] + (t & 15);
+        next_ek = __ldg(p.k_exp + at);
+        next_ev = __ldg(p.v_exp + at);
+      }
+    };
+    load_exps(0);
+    float m_row = -INFINITY;  // threads 0 .. RT - 1: the row's running maximum
+    bool ok = true;
+    for (int i = 0; i < n_tiles; ++i) {
+      const int t0 = kv_beg + i * kQTile, tok = t0 + t128;
+      const bool partial = t0 + kQTile > min_lim;
+      ok = ok && mbar_wait(s_full + (i & 1), (i >> 1) & 1, p.status, GR_ERR_TIMEOUT);
+      tc_fence_after();
+      const int ek = next_ek, ve = next_ev;
+      load_exps(i + 1);
+      const float fk = kv_scale(ek);
+      const float ev = ve == kKvExpBad ? __int_as_float(0x7fc00000) : static_cast<float>(ve);
+      const float unv = ve == kKvExpBad ? 1.f : exp2i(-ve);
+      float w[RH];
+      {
+        uint32_t s[Sh::q_parts * RH];
+        tmem_ld_cols<Sh::q_parts * RH>(t_s, s);
+        tmem_ld_done(s);
+#pragma unroll
+        for (int r = 0; r < RH; ++r) {
+          float x;
+          if (FMT == GR_KV_E4M3) {
+            x = fmaf(__uint_as_float(s[RH + r]), 1.f / 16, __uint_as_float(s[r]));
+          } else {  // digits * 65536, 256, 1; the two constants leave exactly with the first product's
+            x = fmaf(int_biased(s[r]), 65536.f, -kIntBias * 65536.f - kIntBias * 256.f);
+            x = fmaf(int_biased(s[RH + r]), 256.f, x) + (int_biased(s[2 * RH + r]) - kIntBias);
+          }
+          w[r] = fmaf(x, coef[r] * fk, ev);
+        }
+      }
+      if (partial) {
+#pragma unroll
+        for (int r = 0; r < RH; ++r)
+          if (tok >= lim[r]) w[r] = -INFINITY;
+        // an unwritten slot's value codes may be NaN codes: out of the product
+        ok = ok && mbar_wait(v_full + i % kQStages, (i / kQStages) & 1, p.status, GR_ERR_TIMEOUT);
+        if (grp == 0 && tok >= kv_end) {
+          uint4* row = reinterpret_cast<uint4*>(smem + Sh::v + (i % kQStages) * kQHalf + t128 * 128);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) row[k] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      // row maxima over the tile's 128 tokens: by warp, then one thread per row
+      {
+        float mine = 0.f;
+#pragma unroll
+        for (int r = 0; r < RH; ++r) {
+          const float x = warp_max(w[r]);
+          if (lane == r) mine = x;
+        }
+        if (lane < RH) xm[(rb + lane) * 4 + (warp & 3)] = mine;
+      }
+      named_sync(1, kSoft);
+      bool raised = false;
+      if (tid < RT) {
+        const float4 x = *reinterpret_cast<const float4*>(xm + tid * 4);
+        const float mt = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));  // -inf: no token of this tile is seen
+        const float mn = fmaxf(mt, m_row);
+        raised = mn > m_row;
+        alphas[tid] = raised ? ex2_approx(m_row - mn) : 1.f;  // 0 from -inf
+        betas[tid] = mt == -INFINITY ? 1.f : ex2_approx(mt - mn);
+        refs[tid] = off - (mt == -INFINITY ? 0.f : mt);
+        m_row = mn;
+      }
+      if (named_any(1, kSoft, raised)) {
+#pragma unroll
+        for (int r = 0; r < RH; ++r) {
+          o[r] *= alphas[rb + r];
+          l[r] *= alphas[rb + r];
+        }
+      }
+      // weights; P to shared memory, 16 (part, row) columns of a token in a vector
+      uint32_t pw[Sh::p_cols / 4];
+#pragma unroll
+      for (int k = 0; k < Sh::p_cols / 4; ++k) pw[k] = 0;
+#pragma unroll
+      for (int r = 0; r < RH; r += 4) {
+        float x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[k] = ex2_approx(w[r + k] + refs[rb + r + k]);
+          // a hidden token's exponent may be that of a bad row, or of no row: its weight is 0, and 2^-ev is finite
+          l[r + k] = fmaf(x[k] * unv, betas[rb + r + k], l[r + k]);
+        }
+        if (FMT == GR_KV_E4M3) {
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+            pw[(k * RH + r) / 4] = __byte_perm(lo, hi, 0x5410);
+            if (k < 2) {
+              const uint32_t h01 = e4m3x2_to_half2(lo), h23 = e4m3x2_to_half2(hi);
+              const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h01));
+              const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&h23));
+              x[0] = (x[0] - a.x) * 16.f;
+              x[1] = (x[1] - a.y) * 16.f;
+              x[2] = (x[2] - c.x) * 16.f;
+              x[3] = (x[3] - c.y) * 16.f;
+            }
+          }
+        } else {
+          // two signed digits: the low 16 bits of x + 2^23 + 0x8080 are x + 0x8080, each byte less 0x80 a digit
+          uint32_t t[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) t[k] = __float_as_uint(x[k] + 8421504.f);
+          const uint32_t a = __byte_perm(t[0], t[1], 0x5140), c = __byte_perm(t[2], t[3], 0x5140);  // lo lo hi hi
+          pw[r / 4] = __byte_perm(a, c, 0x7632) ^ 0x80808080u;
+          pw[(RH + r) / 4] = __byte_perm(a, c, 0x5410) ^ 0x80808080u;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < Sh::p_cols / 16; ++k)
+        *reinterpret_cast<uint4*>(ps + (k * kQTile + t128) * 16) =
+            make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]);
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
+      ok = ok && mbar_wait(o_full + (i & 1), (i >> 1) & 1, p.status, GR_ERR_TIMEOUT);
+      tc_fence_after();
+      {
+        uint32_t x[Sh::p_parts * RH];
+        tmem_ld_cols<Sh::p_parts * RH>(t_o, x);
+        tmem_ld_done(x);
+#pragma unroll
+        for (int r = 0; r < RH; ++r) {
+          float y;
+          if (FMT == GR_KV_E4M3)
+            y = fmaf(fmaf(__uint_as_float(x[2 * RH + r]), 1.f / 16, __uint_as_float(x[RH + r])), 1.f / 16,
+                     __uint_as_float(x[r]));
+          else
+            y = fmaf(int_biased(x[r]), 256.f, -kIntBias * 256.f - kIntBias) + int_biased(x[RH + r]);
+          o[r] = fmaf(y, betas[rb + r], o[r]);
+        }
+      }
+    }
+    // ---- l over the 128 tokens, then this split's result
+    named_sync(1, kSoft);
+#pragma unroll
+    for (int r = 0; r < RH; ++r) {
+      const float x = warp_sum(l[r]);
+      if (lane == 0) xm[(rb + r) * 4 + (warp & 3)] = x;
+    }
+    named_sync(1, kSoft);
+    if (n_active > 1 && tid < R) {
+      const float4 x = *reinterpret_cast<const float4*>(xm + tid * 4);
+      __stcg(reinterpret_cast<float2*>(p.ws_ml) + (slot0 + split) * R_all + r0 + tid,
+             make_float2(m_row, (x.x + x.y) + (x.z + x.w)));
+    }
+#pragma unroll
+    for (int r = 0; r < RH; ++r) {
+      if (rb + r >= R) break;
+      if (n_active == 1) {
+        const float4 x = *reinterpret_cast<const float4*>(xm + (rb + r) * 4);
+        const float sum = (x.x + x.y) + (x.z + x.w);
+        const int g = (r0 + rb + r) / p.K, j = (r0 + rb + r) - g * p.K;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        p.out[((static_cast<int64_t>(b) * p.K + j) * p.n_q_heads + kvh * G + g) * 128 + t128] =
+            __float2bfloat16(o[r] * inv);
+      } else {
+        __stcg(p.ws_o + ((slot0 + split) * R_all + r0 + rb + r) * 128 + t128, o[r]);
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Sh::tmem_cols);
+  }
+  if (!active || n_active == 1) return;
 
   // ---- the last split to arrive joins them, in split order
   __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int* tk = p.ws_ticket + b * p.n_kv_heads + kvh;
+  if (tid == 0) {
+    int* tk = p.ws_ticket + (static_cast<int64_t>(b) * p.n_kv_heads + kvh) * p.row_blocks + blk;
     const bool last = atomicAdd(tk, 1) == n_active - 1;
     if (last) *tk = 0;
     *flag = last;
   }
   __syncthreads();
-  if (!*flag) return;
+  if (!*flag || warp >= kMmaWarp) return;
   __threadfence();
-  for (int r = warp; r < R; r += nthr >> 5) {
-    const float2* ml = reinterpret_cast<const float2*>(p.ws_ml);
-    float M = -INFINITY;
-    for (int s2 = lane; s2 < n_active; s2 += 32) M = fmaxf(M, __ldcg(ml + (slot0 + s2) * R_pad + r).x);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-    const float Ms = M == -INFINITY ? 0.f : M;
-    float lsum = 0.f;
+  // a warp per row; one or two rows share the four warps, each taking a part of the splits
+  const int parts = R >= 3 ? 1 : (R == 2 ? 2 : 4);
+  float4* pool = reinterpret_cast<float4*>(smem + Sh::k);  // [warps][32] partial sums
+  for (int rr = warp / parts; rr < (parts > 1 ? 4 / parts : R); rr += kMmaWarp / parts) {
+    const int part = warp % parts;
+    const int r = r0 + rr;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s2 = 0; s2 < n_active; ++s2) {
-      const float2 x = __ldcg(ml + (slot0 + s2) * R_pad + r);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_o + ((slot0 + s2) * R_pad + r) * 128) + lane);
-      const float w = ex2_approx(x.x - Ms);
-      lsum += w * x.y;
-      acc.x += w * v.x;
-      acc.y += w * v.y;
-      acc.z += w * v.z;
-      acc.w += w * v.w;
+    float lsum = 0.f;
+    {
+      const float2* ml = reinterpret_cast<const float2*>(p.ws_ml);
+      float2 x[kKv8MaxSplits / 32];
+      float M = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kKv8MaxSplits / 32; ++k) {
+        const int s2 = lane + 32 * k;
+        x[k] = s2 < n_active ? __ldcg(ml + (slot0 + s2) * R_all + r) : make_float2(-INFINITY, 0.f);
+        M = fmaxf(M, x[k].x);
+      }
+      M = warp_max(M);
+      const float Ms = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int k = 0; k < kKv8MaxSplits / 32; ++k) {
+        x[k].x = ex2_approx(x[k].x - Ms);
+        lsum += x[k].x * x[k].y;
+      }
+      lsum = warp_sum(lsum);
+#pragma unroll
+      for (int k = 0; k < kKv8MaxSplits / 32; ++k) {
+        if (32 * k >= n_active) break;
+        const int n = min(32, n_active - 32 * k);
+#pragma unroll 8
+        for (int u = part; u < n; u += parts) {
+          const float4 v =
+              __ldcg(reinterpret_cast<const float4*>(p.ws_o + ((slot0 + 32 * k + u) * R_all + r) * 128) + lane);
+          const float w = __shfl_sync(0xffffffffu, x[k].x, u);
+          acc.x += w * v.x;
+          acc.y += w * v.y;
+          acc.z += w * v.z;
+          acc.w += w * v.w;
+        }
+      }
     }
-    store_out(r, lane, acc, lsum == 0.f ? 0.f : 1.f / lsum);
+    if (parts > 1) {
+      pool[warp * 32 + lane] = acc;
+      named_sync(1, 128);
+      if (part == 0) {
+        for (int k = 1; k < parts; ++k) {
+          const float4 v = pool[(warp + k) * 32 + lane];
+          acc.x += v.x;
+          acc.y += v.y;
+          acc.z += v.z;
+          acc.w += v.w;
+        }
+      }
+      named_sync(1, 128);
+    }
+    if (part == 0) {
+      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+      const int g = r / p.K, j = r - g * p.K;
+      uint2 pk;
+      pk.x = pack_bf16(acc.x * inv, acc.y * inv);
+      pk.y = pack_bf16(acc.z * inv, acc.w * inv);
+      *reinterpret_cast<uint2*>(p.out + ((static_cast<int64_t>(b) * p.K + j) * p.n_q_heads + kvh * G + g) * 128 +
+                                lane * 4) = pk;
+    }
   }
 }
 
 size_t kv8_attention_ws_bytes(int bs, int rows, int n_kv_heads, int max_splits, size_t* o_off, size_t* ml_off) {
-  const size_t r_pad = static_cast<size_t>((rows + 15) / 16) * 16;
-  const size_t slots = static_cast<size_t>(bs) * n_kv_heads * max_splits;
+  const size_t n = static_cast<size_t>(bs) * n_kv_heads * max_splits * rows;
   if (o_off) *o_off = kQTicketBytes;
-  if (ml_off) *ml_off = kQTicketBytes + slots * r_pad * 512;
-  return kQTicketBytes + slots * r_pad * 520;
+  if (ml_off) *ml_off = kQTicketBytes + n * 512;
+  return kQTicketBytes + n * 520;
 }
 
-template <int FMT>
+// Rows of a CTA: at most kQMaxRows, the row blocks of a head as even as possible.
+void kv8_attention_blocks(int rows, int* blocks, int* per_block) {
+  *blocks = (rows + kQMaxRows - 1) / kQMaxRows;
+  *per_block = (rows + *blocks - 1) / *blocks;
+}
+
+template <int FMT, int RT, int H>
 static cudaError_t launch_kv8_attention_t(const CUtensorMap& tmk, const CUtensorMap& tmv, const KvAttnParams& p,
-                                          int warps, size_t smem, cudaStream_t stream, bool pdl) {
+                                          cudaStream_t stream, bool pdl) {
+  auto kern = kv8_attention_kernel<FMT, RT, H>;
+  using Sh = KvAttnShape<FMT, RT, H>;
   static PerDeviceOnce configured;
-  cudaError_t e = once_per_device(configured, [] {
-    cudaError_t r = cudaFuncSetAttribute(kv8_attention_kernel<FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         227 * 1024);
+  cudaError_t e = once_per_device(configured, [&] {
+    cudaError_t r = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::bytes);
     if (r != cudaSuccess) return r;
-    return cudaFuncSetAttribute(kv8_attention_kernel<FMT>, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    return cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
   });
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.max_splits, p.n_kv_heads, p.bs);
-  cfg.blockDim = dim3(32 * warps);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3(p.max_splits, p.n_kv_heads * p.row_blocks, p.bs);
+  cfg.blockDim = dim3(Sh::threads);
+  cfg.dynamicSmemBytes = Sh::bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv8_attention_kernel<FMT>, tmk, tmv, p);
+  return cudaLaunchKernelEx(&cfg, kern, tmk, tmv, p);
 }
-
-// Warp groups of a CTA: as many as fit eight warps, four at most.
-int kv8_attention_groups(int rows) {
-  const int n_mt = (rows + 15) / 16;
-  const int g = kQMaxWarps / n_mt;
-  return g > 4 ? 4 : g;
+template <int FMT>
+static cudaError_t launch_kv8_attention_f(const CUtensorMap& tmk, const CUtensorMap& tmv, const KvAttnParams& p,
+                                          cudaStream_t stream, bool pdl) {
+  if (p.rows_per_block <= 4) return launch_kv8_attention_t<FMT, 4, 1>(tmk, tmv, p, stream, pdl);
+  if (p.rows_per_block <= 8) return launch_kv8_attention_t<FMT, 8, 1>(tmk, tmv, p, stream, pdl);
+  if (p.rows_per_block <= 16) return launch_kv8_attention_t<FMT, 16, 1>(tmk, tmv, p, stream, pdl);
+  return launch_kv8_attention_t<FMT, kQMaxRows, 2>(tmk, tmv, p, stream, pdl);
 }
 
 cudaError_t launch_kv8_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, KvAttnParams p, int format,
                                  cudaStream_t stream, bool pdl) {
-  const int rows = p.n_q_heads / p.n_kv_heads * p.K;
-  const int n_mt = (rows + 15) / 16;
-  p.groups = kv8_attention_groups(rows);
-  const size_t smem = 1024 + kv_attn_smem(p.groups, n_mt).total;
-  return format == GR_KV_E4M3 ? launch_kv8_attention_t<GR_KV_E4M3>(tmk, tmv, p, p.groups * n_mt, smem, stream, pdl)
-                              : launch_kv8_attention_t<GR_KV_INT8>(tmk, tmv, p, p.groups * n_mt, smem, stream, pdl);
+  kv8_attention_blocks(p.n_q_heads / p.n_kv_heads * p.K, &p.row_blocks, &p.rows_per_block);
+  return format == GR_KV_E4M3 ? launch_kv8_attention_f<GR_KV_E4M3>(tmk, tmv, p, stream, pdl)
+                              : launch_kv8_attention_f<GR_KV_INT8>(tmk, tmv, p, stream, pdl);
 }
 
 }  // namespace gr

@@ -1,5 +1,6 @@
 // extern "C" entry points of libgravity_b200.so (declared in include/gravity_b200.h): argument checks, tile and
 // split heuristics, TMA tensor-map encoding (cached per buffer) and the launches.
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -904,17 +905,21 @@ size_t gr_kv8_attention_workspace_bytes(int bs, int K, int n_q_heads, int n_kv_h
 }
 
 int gr_kv8_attention_plan(int bs, int K, int max_len, int n_q_heads, int n_kv_heads, int32_t* out) {
-  if (!out || bs <= 0 || K <= 0 || max_len <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads)
+  if (!out || bs <= 0 || K <= 0 || max_len <= 0 || max_len > kKv8MaxChunk * kKv8MaxSplits || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads)
     return GR_ERR_ARG;
-  const int64_t units = static_cast<int64_t>(bs) * n_kv_heads;
-  // two CTAs an SM: the (request, head) pairs times the splits of the longest request make about one such wave
-  const int64_t per = (2LL * num_sms() + units - 1) / units;
+  // the (request, head, row block) triples times the splits of the longest request make about one wave of the CTAs
+  // that fit: three an SM, two where a CTA holds more than 16 rows
+  int blocks, per_block;
+  kv8_attention_blocks(n_q_heads / n_kv_heads * K, &blocks, &per_block);
+  const int64_t units = static_cast<int64_t>(bs) * n_kv_heads * blocks;
+  const int64_t per = std::max<int64_t>(1, (per_block > 16 ? 2LL : 3LL) * num_sms() / units);
   int64_t chunk = (static_cast<int64_t>(max_len) + per - 1) / per;
   if (chunk > 1024 && units >= num_sms()) chunk = 1024;  // many requests of mixed lengths: even pieces
   const int64_t least = (static_cast<int64_t>(max_len) + kKv8MaxSplits - 1) / kKv8MaxSplits;
   if (chunk < least) chunk = least;
   if (chunk < 128) chunk = 128;
   chunk = (chunk + 31) / 32 * 32;
+  if (chunk > kKv8MaxChunk) chunk = kKv8MaxChunk;
   out[0] = static_cast<int32_t>(chunk);
   out[1] = static_cast<int32_t>((max_len + chunk - 1) / chunk);
   return GR_OK;
@@ -927,13 +932,14 @@ int gr_kv8_attention(const void* q, const gr_kv_cache* cache, const int32_t* pag
   if (rc) return rc;
   if (cache->format == GR_KV_BF16) return GR_ERR_UNSUPPORTED;
   if (!q || !page_table || !seq_lens || !out || bs <= 0 || K <= 0 || pt_stride <= 0 || n_q_heads <= 0 ||
-      n_q_heads % cache->n_kv_heads || draft < 0 || draft > 2 || chunk <= 0 || chunk % 32 || max_splits <= 0 ||
+      n_q_heads % cache->n_kv_heads || draft < 0 || draft > 2 || chunk <= 0 || chunk % 32 || chunk > kKv8MaxChunk || max_splits <= 0 ||
       max_splits > kKv8MaxSplits || !aligned(q, 16) || !aligned(out, 16))
     return GR_ERR_ARG;
   const int64_t rows = static_cast<int64_t>(n_q_heads / cache->n_kv_heads) * K;
-  if (rows > 128 || bs > 65535 || cache->n_kv_heads > 65535 ||
-      static_cast<int64_t>(bs) * cache->n_kv_heads > kKv8TicketPairs ||
-      pt_stride > (INT32_MAX - 8192) / 16 || chunk > INT32_MAX / 2)
+  if (rows > 128) return GR_ERR_UNSUPPORTED;
+  int blocks, per_block;
+  kv8_attention_blocks(static_cast<int>(rows), &blocks, &per_block);
+  if (static_cast<int64_t>(bs) * cache->n_kv_heads * blocks > kKv8TicketPairs || pt_stride > (INT32_MAX - 8192) / 16)
     return GR_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(chunk) * max_splits < K) return GR_ERR_ARG;
   KvAttnParams p;

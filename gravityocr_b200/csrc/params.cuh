@@ -176,7 +176,8 @@ struct KvAttnParams {
   int pt_stride;
   const int64_t* seq_lens;
   int bs, K, draft, base_add, n_q_heads, n_kv_heads;
-  int chunk, max_splits, groups;
+  int chunk, max_splits;
+  int row_blocks, rows_per_block;  // a CTA's share of a K/V head's query rows
   float scale_log2;
   float* ws_o;
   float* ws_ml;
@@ -264,8 +265,10 @@ cudaError_t launch_kv_read(const KvReadParams& p, int format, cudaStream_t s, bo
 size_t kv8_attention_ws_bytes(int bs, int rows, int n_kv_heads, int max_splits, size_t* o_off, size_t* ml_off);
 cudaError_t launch_kv8_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, KvAttnParams p, int format,
                                  cudaStream_t stream, bool pdl);
-constexpr int kKv8TicketPairs = 16384;  // (request, K/V head) pairs of one call
+void kv8_attention_blocks(int rows, int* blocks, int* per_block);
+constexpr int kKv8TicketPairs = 16384;  // (request, K/V head, row block) triples of one call
 constexpr int kKv8MaxSplits = 128;
+constexpr int kKv8MaxChunk = 8192;      // cache tokens of a split
 cudaError_t launch_token_logprobs(const LogprobParams& p, bool bf16, cudaStream_t stream, bool pdl);
 constexpr int kLogprobMaxTop = 64;
 cudaError_t launch_pack_gate_up(const __nv_bfloat16* src, __nv_bfloat16* dst, int I, int H, cudaStream_t s);

@@ -83,7 +83,7 @@ def _attend(cache=None, **kw):
 
 @pytest.mark.parametrize("kw", [dict(q=None), dict(q=P + 8), dict(pt=None), dict(stride=0), dict(seq=None), dict(bs=0),
                                 dict(K=0), dict(draft=3), dict(draft=-1), dict(nq=12), dict(nq=0), dict(chunk=0),
-                                dict(chunk=100), dict(splits=0), dict(splits=129, ws=P, n_ws=1 << 40),
+                                dict(chunk=100), dict(chunk=8224), dict(splits=0), dict(splits=129, ws=P, n_ws=1 << 40),
                                 dict(splits=2), dict(splits=2, ws=P, n_ws=65536), dict(splits=2, ws=P + 4, n_ws=1 << 30),
                                 dict(out=None), dict(out=P + 2), dict(K=33, nq=16, chunk=32)])
 def test_attention_refuses(kw):
@@ -114,17 +114,17 @@ def test_logprobs_refuses(kw):
 
 
 @pytest.mark.parametrize("bs", [1, 2, 7, 64, 500])
-@pytest.mark.parametrize("max_len", [1, 31, 32, 129, 4129, 131072, 2 ** 24 + 5])
+@pytest.mark.parametrize("max_len", [1, 31, 32, 129, 4129, 131072, 2 ** 20])
 @pytest.mark.parametrize("heads", [(16, 8), (5, 1), (32, 8)])
 def test_plan_covers_the_longest_request(bs, max_len, heads):
     chunk, splits = L.kv8_attention_split(bs, 1, max_len, *heads)
     assert chunk % 32 == 0 and 1 <= splits <= 128 and chunk * splits >= max_len > chunk * (splits - 1)
-    assert L.kv8_attention_workspace_bytes(bs, 1, *heads, splits) >= 65536 + bs * heads[1] * splits * 16 * 520
+    assert L.kv8_attention_workspace_bytes(bs, 1, *heads, splits) >= 65536 + bs * heads[0] * splits * 520
 
 
 def test_plan_refuses():
     lib, out = L.load(), (ctypes.c_int32 * 2)()
-    for a in [(0, 1, 9, 16, 8), (1, 0, 9, 16, 8), (1, 1, 0, 16, 8), (1, 1, 9, 15, 8), (1, 1, 9, 16, 0)]:
+    for a in [(1, 1, 2 ** 20 + 1, 16, 8), (0, 1, 9, 16, 8), (1, 0, 9, 16, 8), (1, 1, 0, 16, 8), (1, 1, 9, 15, 8), (1, 1, 9, 16, 0)]:
         assert lib.gr_kv8_attention_plan(*a, out) == ARG
     assert lib.gr_kv8_attention_plan(1, 1, 9, 16, 8, None) == ARG
     assert L.kv8_attention_workspace_bytes(1, 1, 15, 8, 1) == 0
