@@ -13,17 +13,18 @@
 // The 8-bit B operands hold a row in several 8-bit parts, one column each, whose products are summed in fp32:
 //   e4m3  q = q0 + q1 / 16, exact to 2^-22 of the row's largest element (q has 8 significant bits, a part 4);
 //         p = p0 + p1 / 16 + p2 / 256, 2^-12 relative; accumulated in fp32.
-//   int8  q in three signed digits to base 256 (2^-22 of the row's largest element), p in two: 2^-16 of the tile's largest
-//         weight, accumulated exactly in int32 and added in fp32.
+//   int8  q and p in two signed digits to base 256, rounded to 2^-16 of the row's largest element and of the tile's largest
+//         weight; accumulated exactly in int32, joined as hi * 256 + lo and added in fp32.
 //   (bf16 rounding of the output is 2^-9 relative.)
-// Scales: a row's q is brought to a fixed binade by a power of two; with a token's 2^ek, 2^ev:
-//   w = s * coef_r * 2^ek + ev (base 2),  M_r = max w,  p = 2^(w - M_r),  O = sum p code_v,  l = sum p 2^-ev,  out = O / l.
+// Scales: a row's q is brought to the parts' range by a factor that coef_r undoes; with a token's 2^ek, 2^ev:
+//   w = s * coef_r * 2^ek + ev (base 2),  p = 2^(w - M_r),  O = sum p code_v,  l = sum p 2^-ev,  out = O / l.
 // |ev| <= 40 keeps l: a token whose p underflows has a score 46 binades below the best.
 //
 //
 // P is measured from its own tile's maximum T_r, not the running one: its parts then resolve the tile's weights whatever the
 // rest of the sequence holds (a first token that takes most of the attention would otherwise push every later weight
-// below int8's two digits), and O and l take a tile in fp32 with the factor 2^(T_r - M_r).
+// below int8's two digits), and O and l take a tile in fp32 with the factor 2^(T_r - M_r).  M_r is the first tile's maximum,
+// raised only where a tile's is 2^64 above it: fp32 holds the rest, and the sums are hardly ever rescaled.
 //
 // CTA: (split, K/V head and block of at most 40 rows, request).  One thread per token (then per dimension) and row group: up
 // to 16 rows four warps take all of them, above that eight warps take half the rows each.  One warp issues the MMAs, one the
@@ -38,18 +39,18 @@ namespace gr {
 constexpr int kQTile = 128;                                 // tokens per tile: eight pages
 constexpr int kQHalf = kQTile * 128;                        // K or V codes of a tile
 constexpr int kQStages = 2;                                 // K and V rings (the product barriers are as many)
+constexpr int kQExpStages = 4;                              // tiles' exponents
 constexpr int kQMaxRows = 40;                               // rows of a CTA
 constexpr size_t kQTicketBytes = kKv8TicketPairs * sizeof(int);
 
-// RT rows in H groups of RH.  Columns: S has part k of row r at group * q_parts * RH + k * RH + r (within its group), P
+// RT rows in H groups of RH.  Columns: S has part k of row r at group * 2 * RH + k * RH + r (within its group), P
 // likewise with every group padded to 16 columns.
 template <int FMT, int RT, int H>
 struct KvAttnShape {
   static constexpr int RH = RT / H;
-  static constexpr int q_parts = FMT == GR_KV_E4M3 ? 2 : 3;
   static constexpr int p_parts = FMT == GR_KV_E4M3 ? 3 : 2;
   static constexpr int p_cols = (p_parts * RH + 15) / 16 * 16;
-  static constexpr int n1 = (q_parts * RT + 15) / 16 * 16;
+  static constexpr int n1 = (2 * RT + 15) / 16 * 16;
   static constexpr int n2 = p_cols * H;
   static constexpr int tmem_cols = n1 + n2 <= 32 ? 32 : (n1 + n2 <= 64 ? 64 : (n1 + n2 <= 128 ? 128 : 256));
   static constexpr int threads = 128 * H + 64;
@@ -59,7 +60,8 @@ struct KvAttnShape {
   static constexpr int v = k + kQStages * kQHalf;
   static constexpr int q = v + kQStages * kQHalf;           // [n1][128], 128-byte swizzle
   static constexpr int p = q + n1 * 128;                    // [n2 / 16][128 tokens][16]
-  static constexpr int xm = p + n2 * 128;                   // [RT][4] warp maxima of a tile; at the end, warp sums of l
+  static constexpr int exps = p + n2 * 128;                 // [kQExpStages][K, V][128]
+  static constexpr int xm = exps + kQExpStages * 2 * kQTile;                   // [4][RT] warp maxima of a tile; at the end, the sums l
   static constexpr int coef = xm + RT * 16;                 // [RT] score scale
   static constexpr int ref = coef + RT * 4;                 // [RT] off - T_r
   static constexpr int alpha = ref + RT * 4;                // [RT] factor of the sums so far
@@ -67,10 +69,18 @@ struct KvAttnShape {
   static constexpr int lim = beta + RT * 4;                 // [RT] row limits
   static constexpr int pages = lim + RT * 4;                // [kKv8MaxChunk / 16] first code row of each page
   static constexpr int bars = (pages + kKv8MaxChunk / 4 + 15) / 16 * 16;
-  static constexpr int bytes = 1024 + bars + (2 * kQStages + 5) * 8 + 16;
+  static constexpr int bytes = 1024 + bars + (2 * kQStages + kQExpStages + 5) * 8 + 16;
   static_assert(RH % 4 == 0 && n1 <= 256 && n1 + n2 <= 256, "rows are handled by fours");
 };
 
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src))
+               : "memory");
+}
+// Arrives on the barrier once this thread's copies so far have landed (one of the barrier's expected arrivals).
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 // One thread of the warp, the same each time; all 32 lanes take part.
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -128,7 +138,8 @@ __device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
-// 1.5 * 2^23 + x as a float, |x| < 2^22: an integer becomes a float by an addition (the conversion unit is 8 times slower).
+// 1.5 * 2^23 + x as a float, |x| < 2^22: an integer becomes a float by an addition.  (The conversion unit, 8 cycles a warp,
+// already has the weights' exponentials and the joining of O.)
 constexpr float kIntBias = 12582912.f;
 __device__ __forceinline__ float int_biased(uint32_t x) { return __uint_as_float(x + 0x4B400000u); }
 __device__ __forceinline__ float warp_max(float v) {
@@ -154,7 +165,7 @@ __device__ __forceinline__ uint64_t smem_desc_mn16(uint32_t addr, uint32_t block
   return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(128 >> 4) << 16) |
          (static_cast<uint64_t>(block_bytes >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
 }
-// Four q values, scaled into the format's binade, to q_parts words of four codes.
+// Four scaled q values to q_parts words of four codes.
 template <int FMT>
 __device__ __forceinline__ void split_q(const float (&x)[4], uint32_t* part) {
   if (FMT == GR_KV_E4M3) {  // |x| < 256
@@ -168,14 +179,13 @@ __device__ __forceinline__ void split_q(const float (&x)[4], uint32_t* part) {
     rest[2] = (x[2] - b.x) * 16.f;
     rest[3] = (x[3] - b.y) * 16.f;
     part[1] = kv_pack<GR_KV_E4M3>(rest);
-  } else {  // |x| < 2^22: digits in [-128, 127]
-    part[0] = part[1] = part[2] = 0;
+  } else {  // |x| <= 32639: digits in [-128, 127]
+    part[0] = part[1] = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t t = (static_cast<uint32_t>(__float2int_rn(x[i])) + 0x808080u) ^ 0x808080u;
-      part[0] |= ((t >> 16) & 0xffu) << (8 * i);
-      part[1] |= ((t >> 8) & 0xffu) << (8 * i);
-      part[2] |= (t & 0xffu) << (8 * i);
+      const uint32_t t = (static_cast<uint32_t>(__float2int_rn(x[i])) + 0x8080u) ^ 0x8080u;
+      part[0] |= ((t >> 8) & 0xffu) << (8 * i);
+      part[1] |= (t & 0xffu) << (8 * i);
     }
   }
 }
@@ -194,7 +204,8 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
   // products completed, one barrier per stage parity: a waiter two tiles behind must not mistake the phase
   uint64_t* o_full = s_full + 2;
   uint64_t* p_full = o_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_full + 1);
+  uint64_t* e_full = p_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(e_full + kQExpStages);
   int* flag = reinterpret_cast<int*>(tmem_slot + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -204,6 +215,7 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
       mbar_init(o_full + s, 1);
     }
     mbar_init(p_full, kMmaWarp);
+    for (int s = 0; s < kQExpStages; ++s) mbar_init(e_full + s, 32);
     fence_mbar_init();
     tma_prefetch_desc(&tmk);
     tma_prefetch_desc(&tmv);
@@ -249,47 +261,67 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
     pages[k] = (id * p.n_kv_heads + kvh) * 16;
   }
   if (active && warp < kMmaWarp) {
-    // ---- query rows to shared memory, in parts: a warp per row, every load ahead of the first use
+    // ---- query rows to shared memory, in parts: a warp per row, each step for all of a warp's rows (their latencies overlap)
     float* coef = reinterpret_cast<float*>(smem + Sh::coef);
     int* lim = reinterpret_cast<int*>(smem + Sh::lim);
     constexpr int per_warp = (RT + kMmaWarp - 1) / kMmaWarp;
     uint2 raw[per_warp];
+    int limit[per_warp];
+    float x[per_warp][4], f[per_warp], back[per_warp];
 #pragma unroll
     for (int u = 0; u < per_warp; ++u) {
       const int r = warp + u * kMmaWarp;
-      raw[u] = make_uint2(0u, 0u);
-      if (r < R) {
-        const int g = (r0 + r) / p.K, j = (r0 + r) - g * p.K;
-        raw[u] = __ldg(reinterpret_cast<const uint2*>(
-            p.q + ((static_cast<int64_t>(b) * p.K + j) * p.n_q_heads + kvh * G + g) * 128) + lane);
+      const int g = (r0 + min(r, R - 1)) / p.K, j = (r0 + min(r, R - 1)) - g * p.K;
+      raw[u] = __ldg(reinterpret_cast<const uint2*>(
+          p.q + ((static_cast<int64_t>(b) * p.K + j) * p.n_q_heads + kvh * G + g) * 128) + lane);
+      limit[u] = r < R ? min(kv_end, p.draft ? ((j == 0 && p.draft == 1) ? base + 1 : base + p.K) : base + j + 1) : 0;
+      if (r >= R) raw[u] = make_uint2(0u, 0u);
+    }
+#pragma unroll
+    for (int u = 0; u < per_warp; ++u) {
+      x[u][0] = __uint_as_float(raw[u].x << 16);
+      x[u][1] = __uint_as_float(raw[u].x & 0xffff0000u);
+      x[u][2] = __uint_as_float(raw[u].y << 16);
+      x[u][3] = __uint_as_float(raw[u].y & 0xffff0000u);
+      uint32_t am = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) am = max(am, __float_as_uint(x[u][i]) & 0x7fffffffu);
+      am = __reduce_max_sync(0xffffffffu, am);
+      // e4m3: the largest |q| to [2^7, 2^8), exactly; int8: to 32639, two digits' largest, rounded with the digits.  A row
+      // with a NaN or an infinity scores NaN.
+      if (FMT == GR_KV_E4M3) {
+        const int sh = max(-100, min(100, static_cast<int>(am >> 23) - 127 - 7));
+        f[u] = exp2i(-sh);
+        back[u] = exp2i(sh);
+      } else {
+        const float a = fmaxf(__uint_as_float(am), 1e-30f);
+        f[u] = __fdividef(32639.f, a) * 0.9999995f;  // not above 32639 after its rounding
+        back[u] = 1.f / f[u];
+      }
+      if (am >= 0x7f800000u) {
+        f[u] = 0.f;
+        back[u] = __int_as_float(0x7fc00000);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[u][i] = 0.f;
       }
     }
 #pragma unroll
     for (int u = 0; u < per_warp; ++u) {
       const int r = warp + u * kMmaWarp;
-      if (r >= RT) break;
-      float x[4] = {__uint_as_float(raw[u].x << 16), __uint_as_float(raw[u].x & 0xffff0000u),
-                    __uint_as_float(raw[u].y << 16), __uint_as_float(raw[u].y & 0xffff0000u)};
-      uint32_t am = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) am = max(am, __float_as_uint(x[i]) & 0x7fffffffu);
-      am = __reduce_max_sync(0xffffffffu, am);
-      // the largest |q| to [2^7, 2^8) (e4m3) or [2^21, 2^22) (int8); a row with a NaN or an infinity scores NaN
-      const int sh = max(-100, min(100, static_cast<int>(am >> 23) - 127 - (FMT == GR_KV_E4M3 ? 7 : 21)));
-      const float f = am >= 0x7f800000u ? 0.f : exp2i(-sh);
+      for (int i = 0; i < 4; ++i) x[u][i] *= f[u];
+      uint32_t part[2];
+      split_q<FMT>(x[u], part);
+      if (RT % kMmaWarp == 0 || r < RT) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = f == 0.f ? 0.f : x[i] * f;
-      uint32_t part[3];
-      split_q<FMT>(x, part);
-#pragma unroll
-      for (int k = 0; k < Sh::q_parts; ++k) {
-        const int col = (r / RH) * Sh::q_parts * RH + k * RH + r % RH;
-        *reinterpret_cast<uint32_t*>(smem + Sh::q + sw128(col, lane >> 2) + (lane & 3) * 4) = part[k];
-      }
-      if (lane == 0) {
-        const int j = (r0 + r) % p.K;
-        coef[r] = f == 0.f ? __int_as_float(0x7fc00000) : exp2i(sh) * p.scale_log2;
-        lim[r] = r < R ? min(kv_end, p.draft ? ((j == 0 && p.draft == 1) ? base + 1 : base + p.K) : base + j + 1) : 0;
+        for (int k = 0; k < 2; ++k) {
+          const int col = (r / RH) * 2 * RH + k * RH + r % RH;
+          *reinterpret_cast<uint32_t*>(smem + Sh::q + sw128(col, lane >> 2) + (lane & 3) * 4) = part[k];
+        }
+        if (lane == 0) {
+          coef[r] = back[u] * p.scale_log2;
+          lim[r] = limit[u];
+        }
       }
     }
     fence_proxy_async_smem();
@@ -327,8 +359,17 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
     for (int i = max(0, nv - kQStages); i < nv; ++i)
       mbar_wait(v_full + i % kQStages, (i / kQStages) & 1, p.status, GR_ERR_TIMEOUT);
   } else if (warp == kMmaWarp) {
-    // ---- MMAs, by one elected thread
+    // ---- MMAs, by one elected thread; the exponents' copies, 16 bytes a lane and two tiles ahead (plain loads by the
+    // threads that use them were waited for with the next TMEM load: a memory latency a tile)
     bool ok = true;
+    const int n_pages = (kv_end - kv_beg + 15) >> 4;
+    auto copy_exps = [&](int i) {
+      const int pg = i * 8 + (lane & 7);
+      if (lane < 16 && pg < n_pages)
+        cp_async16(smem + Sh::exps + (i % kQExpStages) * 2 * kQTile + lane * 16, (lane < 8 ? p.k_exp : p.v_exp) + pages[pg]);
+      cp_async_arrive(e_full + i % kQExpStages);
+    };
+    for (int i = 0; i < min(2, n_tiles); ++i) copy_exps(i);
     constexpr uint32_t id_s = idesc_codes<FMT>(Sh::n1, false), id_o = idesc_codes<FMT>(Sh::n2, true);
     const uint64_t kd = smem_desc_sw128(smem_u32(smem + Sh::k));
     const uint64_t vd = smem_desc_sw128_mn(smem_u32(smem + Sh::v), kQHalf);
@@ -345,6 +386,7 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
         tc_commit(s_full + (i & 1));
       }
       __syncwarp();
+      if (i + 2 < n_tiles) copy_exps(i + 2);  // tile i - 2's slot: its weights are long made
       ok = ok && mbar_wait(v_full + i % kQStages, (i / kQStages) & 1, p.status, GR_ERR_TIMEOUT);
       ok = ok && mbar_wait(p_full, i & 1, p.status, GR_ERR_TIMEOUT);
       tc_fence_after();
@@ -356,6 +398,7 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
       }
       __syncwarp();
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (active) {
     // ---- one thread per token (weights), then per dimension (output), for the rows of its group
     const int t128 = tid & 127, grp = H == 1 ? 0 : warp >> 2, rb = grp * RH;
@@ -366,24 +409,13 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
     float* betas = reinterpret_cast<float*>(smem + Sh::beta);
     float* xm = reinterpret_cast<float*>(smem + Sh::xm);
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t t_s = t_lane + grp * Sh::q_parts * RH, t_o = t_lane + Sh::n1 + grp * Sh::p_cols;
+    const uint32_t t_s = t_lane + grp * 2 * RH, t_o = t_lane + Sh::n1 + grp * Sh::p_cols;
     uint8_t* ps = smem + Sh::p + grp * Sh::p_cols * kQTile;
     constexpr float off = FMT == GR_KV_E4M3 ? 8.f : 14.994309f;  // weights up to 2^8, or 32639 (two digits' largest)
     const int min_lim = min(kv_end, p.draft == 2 ? base + p.K : base + 1);
     float o[RH], l[RH];
 #pragma unroll
     for (int r = 0; r < RH; ++r) o[r] = l[r] = 0.f;
-    // this token's exponents, loaded a tile ahead
-    int next_ek = 0, next_ev = 0;
-    auto load_exps = [&](int i) {
-      const int t = i * kQTile + t128;
-      if (kv_beg + t < kv_end) {
-        const int at = pages[t >> 4] + (t & 15);
-        next_ek = __ldg(p.k_exp + at);
-        next_ev = __ldg(p.v_exp + at);
-      }
-    };
-    load_exps(0);
     float m_row = -INFINITY;  // threads 0 .. RT - 1: the row's running maximum
     bool ok = true;
     for (int i = 0; i < n_tiles; ++i) {
@@ -391,26 +423,35 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
       const bool partial = t0 + kQTile > min_lim;
       ok = ok && mbar_wait(s_full + (i & 1), (i >> 1) & 1, p.status, GR_ERR_TIMEOUT);
       tc_fence_after();
-      const int ek = next_ek, ve = next_ev;
-      load_exps(i + 1);
+      ok = ok && mbar_wait(e_full + i % kQExpStages, (i / kQExpStages) & 1, p.status, GR_ERR_TIMEOUT);
+      const int8_t* ex = reinterpret_cast<const int8_t*>(smem + Sh::exps + (i % kQExpStages) * 2 * kQTile);
+      const int ek = ex[t128], ve = ex[kQTile + t128];
       const float fk = kv_scale(ek);
       const float ev = ve == kKvExpBad ? __int_as_float(0x7fc00000) : static_cast<float>(ve);
       const float unv = ve == kKvExpBad ? 1.f : exp2i(-ve);
       float w[RH];
       {
-        uint32_t s[Sh::q_parts * RH];
-        tmem_ld_cols<Sh::q_parts * RH>(t_s, s);
+        uint32_t s[2 * RH];
+        tmem_ld_cols<2 * RH>(t_s, s);
         tmem_ld_done(s);
 #pragma unroll
         for (int r = 0; r < RH; ++r) {
           float x;
           if (FMT == GR_KV_E4M3) {
             x = fmaf(__uint_as_float(s[RH + r]), 1.f / 16, __uint_as_float(s[r]));
-          } else {  // digits * 65536, 256, 1; the two constants leave exactly with the first product's
-            x = fmaf(int_biased(s[r]), 65536.f, -kIntBias * 65536.f - kIntBias * 256.f);
-            x = fmaf(int_biased(s[RH + r]), 256.f, x) + (int_biased(s[2 * RH + r]) - kIntBias);
+          } else {
+            // hi * 256 + lo by additions: 1.5 * 2^23 + x is a float's bits, and the biases (multiples of 256) leave exactly
+            x = fmaf(int_biased(s[r]), 256.f, -kIntBias * 257.f) + int_biased(s[RH + r]);
           }
-          w[r] = fmaf(x, coef[r] * fk, ev);
+          w[r] = x;
+        }
+#pragma unroll
+        for (int r = 0; r < RH; r += 4) {
+          const float4 c = *reinterpret_cast<const float4*>(coef + r);
+          w[r] = fmaf(w[r], c.x * fk, ev);
+          w[r + 1] = fmaf(w[r + 1], c.y * fk, ev);
+          w[r + 2] = fmaf(w[r + 2], c.z * fk, ev);
+          w[r + 3] = fmaf(w[r + 3], c.w * fk, ev);
         }
       }
       if (partial) {
@@ -426,26 +467,21 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
         }
       }
       // row maxima over the tile's 128 tokens: by warp, then one thread per row
-      {
-        float mine = 0.f;
 #pragma unroll
-        for (int r = 0; r < RH; ++r) {
-          const float x = warp_max(w[r]);
-          if (lane == r) mine = x;
-        }
-        if (lane < RH) xm[(rb + lane) * 4 + (warp & 3)] = mine;
+      for (int r = 0; r < RH; r += 4) {
+        const float4 x = make_float4(warp_max(w[r]), warp_max(w[r + 1]), warp_max(w[r + 2]), warp_max(w[r + 3]));
+        if (lane == 0) *reinterpret_cast<float4*>(xm + (warp & 3) * RT + rb + r) = x;
       }
       named_sync(1, kSoft);
       bool raised = false;
       if (tid < RT) {
-        const float4 x = *reinterpret_cast<const float4*>(xm + tid * 4);
-        const float mt = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));  // -inf: no token of this tile is seen
-        const float mn = fmaxf(mt, m_row);
-        raised = mn > m_row;
-        alphas[tid] = raised ? ex2_approx(m_row - mn) : 1.f;  // 0 from -inf
-        betas[tid] = mt == -INFINITY ? 1.f : ex2_approx(mt - mn);
+        const float mt = fmaxf(fmaxf(xm[tid], xm[RT + tid]), fmaxf(xm[2 * RT + tid], xm[3 * RT + tid]));
+        // mt = -inf: the row sees no token of this tile.  The sums' reference moves only when a tile is 2^64 above it.
+        raised = mt > m_row + 64.f;
+        alphas[tid] = raised ? ex2_approx(m_row - mt) : 1.f;  // 0 from -inf
+        if (raised) m_row = mt;
+        betas[tid] = mt == -INFINITY ? 1.f : ex2_approx(mt - m_row);
         refs[tid] = off - (mt == -INFINITY ? 0.f : mt);
-        m_row = mn;
       }
       if (named_any(1, kSoft, raised)) {
 #pragma unroll
@@ -460,13 +496,15 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
       for (int k = 0; k < Sh::p_cols / 4; ++k) pw[k] = 0;
 #pragma unroll
       for (int r = 0; r < RH; r += 4) {
-        float x[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          x[k] = ex2_approx(w[r + k] + refs[rb + r + k]);
-          // a hidden token's exponent may be that of a bad row, or of no row: its weight is 0, and 2^-ev is finite
-          l[r + k] = fmaf(x[k] * unv, betas[rb + r + k], l[r + k]);
-        }
+        const float4 rf = *reinterpret_cast<const float4*>(refs + rb + r);
+        const float4 bt = *reinterpret_cast<const float4*>(betas + rb + r);
+        float x[4] = {ex2_approx(w[r] + rf.x), ex2_approx(w[r + 1] + rf.y), ex2_approx(w[r + 2] + rf.z),
+                      ex2_approx(w[r + 3] + rf.w)};
+        // a hidden token's exponent may be that of a bad row, or of no row: its weight is 0, and 2^-ev is finite
+        l[r] = fmaf(x[0] * unv, bt.x, l[r]);
+        l[r + 1] = fmaf(x[1] * unv, bt.y, l[r + 1]);
+        l[r + 2] = fmaf(x[2] * unv, bt.z, l[r + 2]);
+        l[r + 3] = fmaf(x[3] * unv, bt.w, l[r + 3]);
         if (FMT == GR_KV_E4M3) {
 #pragma unroll
           for (int k = 0; k < 3; ++k) {
@@ -508,43 +546,62 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
         tmem_ld_cols<Sh::p_parts * RH>(t_o, x);
         tmem_ld_done(x);
 #pragma unroll
-        for (int r = 0; r < RH; ++r) {
-          float y;
-          if (FMT == GR_KV_E4M3)
-            y = fmaf(fmaf(__uint_as_float(x[2 * RH + r]), 1.f / 16, __uint_as_float(x[RH + r])), 1.f / 16,
-                     __uint_as_float(x[r]));
-          else
-            y = fmaf(int_biased(x[r]), 256.f, -kIntBias * 256.f - kIntBias) + int_biased(x[RH + r]);
-          o[r] = fmaf(y, betas[rb + r], o[r]);
+        for (int r1 = 0; r1 < RH; r1 += 4) {
+          const float4 bt = *reinterpret_cast<const float4*>(betas + rb + r1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = r1 + e;
+            float y;
+            if (FMT == GR_KV_E4M3)
+              y = fmaf(fmaf(__uint_as_float(x[2 * RH + r]), 1.f / 16, __uint_as_float(x[RH + r])), 1.f / 16,
+                       __uint_as_float(x[r]));
+            else
+              y = static_cast<float>(static_cast<int>(x[r]) * 256 + static_cast<int>(x[RH + r]));
+            o[r] = fmaf(y, e == 0 ? bt.x : (e == 1 ? bt.y : (e == 2 ? bt.z : bt.w)), o[r]);
+          }
         }
       }
     }
     // ---- l over the 128 tokens, then this split's result
-    named_sync(1, kSoft);
+    float* part = reinterpret_cast<float*>(smem + Sh::k);  // [RT][128]; the last tile's scores are done with the ring
 #pragma unroll
-    for (int r = 0; r < RH; ++r) {
-      const float x = warp_sum(l[r]);
-      if (lane == 0) xm[(rb + r) * 4 + (warp & 3)] = x;
+    for (int r = 0; r < RH; ++r) part[(rb + r) * kQTile + t128] = l[r];
+    named_sync(1, kSoft);
+    {
+      constexpr int per_warp = (RT + kMmaWarp - 1) / kMmaWarp;
+      float sum[per_warp];
+#pragma unroll
+      for (int u = 0; u < per_warp; ++u) {
+        const float4 x = *reinterpret_cast<const float4*>(part + min(warp + u * kMmaWarp, RT - 1) * kQTile + lane * 4);
+        sum[u] = (x.x + x.y) + (x.z + x.w);
+      }
+#pragma unroll
+      for (int w = 16; w > 0; w >>= 1) {
+#pragma unroll
+        for (int u = 0; u < per_warp; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], w);
+      }
+#pragma unroll
+      for (int u = 0; u < per_warp; ++u)
+        if (lane == 0 && warp + u * kMmaWarp < RT) xm[warp + u * kMmaWarp] = sum[u];
     }
     named_sync(1, kSoft);
-    if (n_active > 1 && tid < R) {
-      const float4 x = *reinterpret_cast<const float4*>(xm + tid * 4);
-      __stcg(reinterpret_cast<float2*>(p.ws_ml) + (slot0 + split) * R_all + r0 + tid,
-             make_float2(m_row, (x.x + x.y) + (x.z + x.w)));
-    }
+    if (n_active > 1 && tid < R)
+      __stcg(reinterpret_cast<float2*>(p.ws_ml) + (slot0 + split) * R_all + r0 + tid, make_float2(m_row, xm[tid]));
+    if (n_active == 1) {
 #pragma unroll
-    for (int r = 0; r < RH; ++r) {
-      if (rb + r >= R) break;
-      if (n_active == 1) {
-        const float4 x = *reinterpret_cast<const float4*>(xm + (rb + r) * 4);
-        const float sum = (x.x + x.y) + (x.z + x.w);
+      for (int r = 0; r < RH; ++r) {
+        if (rb + r >= R) break;
+        const float sum = xm[rb + r];
         const int g = (r0 + rb + r) / p.K, j = (r0 + rb + r) - g * p.K;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         p.out[((static_cast<int64_t>(b) * p.K + j) * p.n_q_heads + kvh * G + g) * 128 + t128] =
             __float2bfloat16(o[r] * inv);
-      } else {
-        __stcg(p.ws_o + ((slot0 + split) * R_all + r0 + rb + r) * 128 + t128, o[r]);
       }
+    } else {
+      float* dst = p.ws_o + ((slot0 + split) * R_all + r0 + rb) * 128 + t128;
+#pragma unroll
+      for (int r = 0; r < RH; ++r)
+        if (rb + r < R) __stcg(dst + r * 128, o[r]);
     }
     tc_fence_before();
   }
@@ -567,71 +624,98 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
   __syncthreads();
   if (!*flag || warp >= kMmaWarp) return;
   __threadfence();
-  // a warp per row; one or two rows share the four warps, each taking a part of the splits
-  const int parts = R >= 3 ? 1 : (R == 2 ? 2 : 4);
-  float4* pool = reinterpret_cast<float4*>(smem + Sh::k);  // [warps][32] partial sums
-  for (int rr = warp / parts; rr < (parts > 1 ? 4 / parts : R); rr += kMmaWarp / parts) {
-    const int part = warp % parts;
-    const int r = r0 + rr;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float lsum = 0.f;
-    {
-      const float2* ml = reinterpret_cast<const float2*>(p.ws_ml);
-      float2 x[kKv8MaxSplits / 32];
-      float M = -INFINITY;
+  const float2* ml = reinterpret_cast<const float2*>(p.ws_ml);
+  float* wgt = reinterpret_cast<float*>(smem + Sh::k);  // [rows][kKv8MaxSplits] weights / sum of the splits
+  constexpr int per_warp = (RT + kMmaWarp - 1) / kMmaWarp;
+  constexpr int per_lane = kKv8MaxSplits / 32;
+  auto weights = [&](int r, float2 (&x)[per_lane]) {
+    float M = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < kKv8MaxSplits / 32; ++k) {
+    for (int k = 0; k < per_lane; ++k) M = fmaxf(M, x[k].x);
+    M = warp_max(M);
+    if (M == -INFINITY) M = 0.f;
+#pragma unroll
+    for (int k = 0; k < per_lane; ++k) {
+      x[k].x = ex2_approx(x[k].x - M);
+      sum += x[k].x * x[k].y;
+    }
+    sum = warp_sum(sum);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < per_lane; ++k)
+      if (lane + 32 * k < n_active) wgt[r * kKv8MaxSplits + lane + 32 * k] = x[k].x * inv;
+  };
+#pragma unroll
+  for (int u0 = 0; u0 < per_warp; u0 += 2) {  // two rows' loads at a time
+    float2 x[2][per_lane];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = warp + (u0 + u) * kMmaWarp;
+#pragma unroll
+      for (int k = 0; k < per_lane; ++k) {
         const int s2 = lane + 32 * k;
-        x[k] = s2 < n_active ? __ldcg(ml + (slot0 + s2) * R_all + r) : make_float2(-INFINITY, 0.f);
-        M = fmaxf(M, x[k].x);
+        x[u][k] = r < R && s2 < n_active ? __ldcg(ml + (slot0 + s2) * R_all + r0 + r) : make_float2(-INFINITY, 0.f);
       }
-      M = warp_max(M);
-      const float Ms = M == -INFINITY ? 0.f : M;
+    }
 #pragma unroll
-      for (int k = 0; k < kKv8MaxSplits / 32; ++k) {
-        x[k].x = ex2_approx(x[k].x - Ms);
-        lsum += x[k].x * x[k].y;
-      }
-      lsum = warp_sum(lsum);
-#pragma unroll
-      for (int k = 0; k < kKv8MaxSplits / 32; ++k) {
-        if (32 * k >= n_active) break;
-        const int n = min(32, n_active - 32 * k);
+    for (int u = 0; u < 2; ++u)
+      if (warp + (u0 + u) * kMmaWarp < R) weights(warp + (u0 + u) * kMmaWarp, x[u]);
+  }
+  named_sync(1, kSoft);
+  auto store4 = [&](int it, float4 a) {
+    const int r = r0 + (it >> 5);
+    const int g = r / p.K, j = r - g * p.K;
+    uint2 pk;
+    pk.x = pack_bf16(a.x, a.y);
+    pk.y = pack_bf16(a.z, a.w);
+    *reinterpret_cast<uint2*>(p.out + ((static_cast<int64_t>(b) * p.K + j) * p.n_q_heads + kvh * G + g) * 128 +
+                              (it & 31) * 4) = pk;
+  };
+  auto add = [&](float4& a, int it, int s2) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_o + ((slot0 + s2) * R_all + r0 + (it >> 5)) * 128) +
+                            (it & 31));
+    const float w = wgt[(it >> 5) * kKv8MaxSplits + s2];
+    a.x += w * v.x;
+    a.y += w * v.y;
+    a.z += w * v.z;
+    a.w += w * v.w;
+  };
+  if (R * 32 * 2 <= kSoft) {
+    // one or two rows: the splits are shared between the threads, too
+    const int parts = kSoft / (R * 32), it = tid % (R * 32), part = tid / (R * 32);
+    float4* pool = reinterpret_cast<float4*>(smem + Sh::v);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (part < parts) {
 #pragma unroll 8
-        for (int u = part; u < n; u += parts) {
-          const float4 v =
-              __ldcg(reinterpret_cast<const float4*>(p.ws_o + ((slot0 + 32 * k + u) * R_all + r) * 128) + lane);
-          const float w = __shfl_sync(0xffffffffu, x[k].x, u);
-          acc.x += w * v.x;
-          acc.y += w * v.y;
-          acc.z += w * v.z;
-          acc.w += w * v.w;
-        }
-      }
+      for (int s2 = part; s2 < n_active; s2 += parts) add(a, it, s2);
     }
-    if (parts > 1) {
-      pool[warp * 32 + lane] = acc;
-      named_sync(1, 128);
-      if (part == 0) {
-        for (int k = 1; k < parts; ++k) {
-          const float4 v = pool[(warp + k) * 32 + lane];
-          acc.x += v.x;
-          acc.y += v.y;
-          acc.z += v.z;
-          acc.w += v.w;
-        }
-      }
-      named_sync(1, 128);
-    }
+    pool[tid] = a;
+    named_sync(1, kSoft);
     if (part == 0) {
-      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
-      const int g = r / p.K, j = r - g * p.K;
-      uint2 pk;
-      pk.x = pack_bf16(acc.x * inv, acc.y * inv);
-      pk.y = pack_bf16(acc.z * inv, acc.w * inv);
-      *reinterpret_cast<uint2*>(p.out + ((static_cast<int64_t>(b) * p.K + j) * p.n_q_heads + kvh * G + g) * 128 +
-                                lane * 4) = pk;
+      for (int k = 1; k < parts; ++k) {
+        const float4 v = pool[k * R * 32 + it];
+        a.x += v.x;
+        a.y += v.y;
+        a.z += v.z;
+        a.w += v.w;
+      }
+      store4(it, a);
     }
+    return;
+  }
+  for (int it0 = tid; it0 < R * 32; it0 += 4 * kSoft) {  // four (row, 4 dims) items' loads at a time
+    float4 a[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) a[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+    for (int s2 = 0; s2 < n_active; ++s2) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (it0 + u * kSoft < R * 32) add(a[u], it0 + u * kSoft, s2);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (it0 + u * kSoft < R * 32) store4(it0 + u * kSoft, a[u]);
   }
 }
 

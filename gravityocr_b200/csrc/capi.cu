@@ -907,14 +907,15 @@ size_t gr_kv8_attention_workspace_bytes(int bs, int K, int n_q_heads, int n_kv_h
 int gr_kv8_attention_plan(int bs, int K, int max_len, int n_q_heads, int n_kv_heads, int32_t* out) {
   if (!out || bs <= 0 || K <= 0 || max_len <= 0 || max_len > kKv8MaxChunk * kKv8MaxSplits || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads)
     return GR_ERR_ARG;
-  // the (request, head, row block) triples times the splits of the longest request make about one wave of the CTAs
-  // that fit: three an SM, two where a CTA holds more than 16 rows
+  // the (request, head, row block) triples times the splits of the longest request make about one wave of two CTAs an SM
+  // (131,071 tokens of one request: 37 splits 50 us, 55 splits 54 us); many requests of mixed lengths go in even pieces of
+  // at most 1,536 tokens (64 requests of 288-4,128 tokens: 52 us, against 54 at 1,024 and 56 uncut)
   int blocks, per_block;
   kv8_attention_blocks(n_q_heads / n_kv_heads * K, &blocks, &per_block);
   const int64_t units = static_cast<int64_t>(bs) * n_kv_heads * blocks;
-  const int64_t per = std::max<int64_t>(1, (per_block > 16 ? 2LL : 3LL) * num_sms() / units);
+  const int64_t per = std::max<int64_t>(1, 2LL * num_sms() / units);
   int64_t chunk = (static_cast<int64_t>(max_len) + per - 1) / per;
-  if (chunk > 1024 && units >= num_sms()) chunk = 1024;  // many requests of mixed lengths: even pieces
+  if (chunk > 1536 && units >= num_sms()) chunk = 1536;
   const int64_t least = (static_cast<int64_t>(max_len) + kKv8MaxSplits - 1) / kKv8MaxSplits;
   if (chunk < least) chunk = least;
   if (chunk < 128) chunk = 128;

@@ -274,13 +274,14 @@ def _check_attention(c, out, draft=0):
             continue
         # |out - ref| <= half a bf16 step, and of sum p |v|: the rounding of p to three e4m3 parts (2^-12), fp32 sums over the
         # tokens (16 at a time, and a few joins), and twice the relative error of a weight, which is the absolute error of
-        # its score: 128 products of fp32 accumulation (twice, for truncating accumulators), q's parts (2^-21 of its
-        # largest element) and the exponent's argument
+        # its score: 128 products of fp32 accumulation (twice, for truncating accumulators), the exponent's argument, and q's
+        # parts: 2^-21 of its largest element for e4m3, 0.5 / 32639 of it for int8's two digits
         n, G = k.shape[0], nq // nkv
         av = R.attention(q, k, v.abs(), c["lens"][b], draft)
         ka = k.abs().repeat_interleave(G, 1)
         mag = torch.einsum("jhd,thd->jht", q.abs(), ka).amax(-1, keepdim=True) / math.sqrt(128)
-        parts = 2.0 ** -21 * q.abs().amax(-1, keepdim=True) * ka.sum(-1).amax(0)[None, :, None] / math.sqrt(128)
+        int8 = c["cache"][0].dtype == torch.int8
+        parts = (0.5 / 32639 if int8 else 2.0 ** -21) * q.abs().amax(-1, keepdim=True) * ka.sum(-1).amax(0)[None, :, None] / math.sqrt(128)
         arg = 1.45 * mag + 100.0
         rel = HALF + (n / 16 + 40) * 2.0 ** -23 + 2 * (256 * 2.0 ** -24 * mag + parts + 2.0 ** -22 + 4 * 2.0 ** -24 * arg)
         err = (got[b] - ref).abs()
@@ -288,7 +289,7 @@ def _check_attention(c, out, draft=0):
         # top 2^ev < 2 max|v| of the largest one's row: 2^-26 for three e4m3 parts (any signs); int8's two digits round to
         # 2^-16 of it independently, so their sum over n tokens stays within 6 / sqrt(3) * 2^-15 * sqrt(n)
         loud = R.attention(q, k, v.abs().amax(-1, keepdim=True).expand(v.shape), c["lens"][b], draft)
-        floor = 2.0 ** -13 * math.sqrt(n) if c["cache"][0].dtype == torch.int8 else 2.0 ** -25 * n
+        floor = 2.0 ** -13 * math.sqrt(n) if int8 else 2.0 ** -25 * n
         tol = BF16 * ref.abs() + rel * av + floor * loud
         assert (err <= tol).all(), (b, float((err / tol.clamp_min(1e-30)).max()))
 
