@@ -1,5 +1,7 @@
 """Token log probabilities on a B200 against the 64-bit oracle: ranks and ids have to be equal, the numbers stay within
 bounds derived from the arithmetic."""
+import math
+
 import pytest
 import torch
 
@@ -31,7 +33,8 @@ def _check(logits, ids, n, temperature=None):
     # a fp32 sum of at most 256 terms a thread and 16 joins: below 2^-16 R; the rest are roundings of the result
     r = torch.expm1(-wtop[:, 0])
     slack = 2.0 ** -16 * r / (1 + r)
-    assert ((lp.double().cpu() - wlp).abs() <= slack + 2.0 ** -21 * wlp.abs()).all()
+    lp = lp.double().cpu()
+    assert ((lp == wlp) | ((lp - wlp).abs() <= slack + 2.0 ** -21 * wlp.abs())).all()   # (-inf equals -inf)
     # H = log1p(R) - W / (1 + R): two terms >= 0, W's terms with the same errors and one more product
     assert ((ent.double().cpu() - went).abs() <= 2.0 ** -14 * went + 1e-30).all()
     if n:
@@ -130,6 +133,28 @@ def test_masked_tokens(vocab):
     fin = torch.isfinite(w[0])
     assert ((lp.double().cpu() - w[0])[fin].abs() <= 2.0 ** -16 + 2.0 ** -21 * w[0][fin].abs()).all()
     assert torch.equal(lp.cpu()[~fin].double(), w[0][~fin])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab,rows", [(100, 2), (59392, 3), (59392, 200)])
+def test_masks_of_the_lowest_value(dtype, vocab, rows):
+    """Masks of the type's lowest value: some tokens, all of them (a uniform row), mixed with -inf, all but very low ones."""
+    low = torch.finfo(dtype).min
+    x, ids = _logits(rows, vocab, dtype, 5)
+    x[0, ::2] = low
+    x[0, 1] = float("-inf")
+    x[1, :] = low
+    _check(x, ids, 10)
+    x[0, :] = float("-inf")
+    x[0, 3:9] = low
+    x[1, :] = low
+    x[1, vocab // 2:] = -3e30
+    lp, ent, rank, top, tid = _call(x, torch.full_like(ids, 4), 10)
+    assert abs(float(ent[0]) - math.log(6)) < 1e-6 and abs(float(lp[0]) + math.log(6)) < 1e-6 and int(rank[0]) == 2
+    assert tid[0].tolist() == [3, 4, 5, 6, 7, 8, 0, 1, 2, 9]
+    n = vocab - vocab // 2
+    assert abs(float(ent[1]) - math.log(n)) < 1e-5 and float(lp[1]) < -1e38 and int(rank[1]) == n + 5
+    assert tid[1].tolist() == list(range(vocab // 2, vocab // 2 + 10))
 
 
 def test_peaked_rows_keep_their_digits():
