@@ -4,25 +4,31 @@
 // With m = max l, d_v = (l_v - m) / T and the sums over every token but the (first) best one
 //   R = sum e^{d_v},  W = sum d_v e^{d_v}:   log p_v = d_v - log1p(R),   H = log1p(R) - W / (1 + R).
 // Leaving the best token's own 1 out of R keeps a peaked row exact (its log p is -R, not log(1 + 2^-24 ..)), and both terms
-// of H are >= 0, so neither cancels.  A thread keeps (m, R, W) of its elements online, 16 of them at a time: their maximum
-// first, then one exponential each; two such states join by scaling the lower one by e^{(m_lo - m_hi) / T} after its own
-// best token has joined its sums.
-//   rank = 1 + the tokens that come before the given one, by logit, then by id.
-// Best n: a thread also keeps its best element.  The n-th best of the bests of 64 groups of threads bounds the row's n-th
-// best from below, so only threads whose best reaches the bound look at their elements again (a few KB, from L2), and
-// what they find above it is ranked by counting.
+// of H are >= 0, so neither cancels.
+//
+// Stream: a thread sums e^{(l - ref) / T} and its product with the exponent, 16 logits at a time, against a reference of its
+// own that moves only when a batch's maximum is 2^24 above it; it keeps its largest logit, and counts the tokens that come
+// before the given one (rank = 1 + those, by logit, then by id).  About nine instructions a logit; a running maximum with
+// its token left out on the way cost twice that.  At the end the thread that holds the best token is left out of the
+// sums, and a warp reads that thread's logits again (they are in L2) to sum them without it.
+// Best n: every batch's maximum goes to a cell in shared memory (a thread's batches share 16).  The n-th largest of the largest
+// logits of 64 groups of threads bounds the row's n-th best from below, so only cells that reach the bound are read
+// again, and what is found above it is ranked by counting.  (Cells, not threads, because 592 rows in flight outgrow the L2:
+// reading every such thread's logits again cost 20% more DRAM traffic.)
 // Bound: reading the row.  Few rows are shared between the CTAs of a cluster, whose states, counts and best lists the first
 // one joins through distributed shared memory.
 #include "params.cuh"
 
 namespace gr {
 
-constexpr int kLpThreads = 512;
-constexpr int kLpWarps = kLpThreads / 32;
+constexpr int kLpThreadsFew = 512;        // where the CTAs of a cluster share a row
+constexpr int kLpThreadsMany = 256;       // a CTA a row: four an SM, so one's selection overlaps the others' reading
 constexpr int kLpGroups = 64;             // groups of threads whose bests bound the n-th best; n <= kLpGroups
 constexpr int kLpCand = 1024;             // candidates kept at once
+constexpr uint32_t kLpAhead = 48 << 10;   // bytes of a later row fetched to L2 while this one is finished
+constexpr int kLpCells = 16;              // cells of a thread: batch i counts in cell i % kLpCells
+constexpr int kLpHot = 512;               // cells read again one by one; more (ties) and every thread scans its own logits
 constexpr int kLpMaxCluster = 8;
-constexpr float kLpFloor = -1e20f;        // logits count as at least this: e = 0 there, and (l - m) / T stays finite
 
 struct LpState {
   float m, R, W;  // max logit (-inf: no token yet); sums without the max token, W in units of log2
@@ -50,16 +56,23 @@ __device__ __forceinline__ LpState lp_join(const LpState& a, const LpState& b, f
   r.W = hi.W + f * (lo.W + (lo.R + 1.f) * d);
   return r;
 }
+__device__ __forceinline__ float lp_warp_max(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));  // NaNs are ignored
+  return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// Order of (logit, id) pairs as one integer: higher logit first, then the lower id.  0: no token.
-__device__ __forceinline__ uint64_t lp_key(float x, int id) {
+// Order of logits as integers (one zero), and of (logit, id) pairs: higher logit first, then the lower id.  0: no token.
+__device__ __forceinline__ uint32_t lp_order(float x) {
   const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);
-  const uint32_t o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  return (static_cast<uint64_t>(o) << 32) | (0xffffffffu - static_cast<uint32_t>(id));
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t lp_key(float x, int id) {
+  return (static_cast<uint64_t>(lp_order(x)) << 32) | (0xffffffffu - static_cast<uint32_t>(id));
 }
 __device__ __forceinline__ int lp_key_id(uint64_t k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
 __device__ __forceinline__ float lp_key_logit(uint64_t k) {
@@ -67,7 +80,32 @@ __device__ __forceinline__ float lp_key_logit(uint64_t k) {
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
 
-// 16 logits of a thread: 16-byte loads raw[], their maximum, and their values raised to kLpFloor (NaNs kept).
+// 16-byte loads of logits: their maximum (NaNs ignored), and how many are >= t.
+// Two fp32 numbers in a register pair (add, mul and fma take both at once).
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 template <typename T>
 struct LpVec;
 template <>
@@ -79,10 +117,6 @@ struct LpVec<float> {
   }
   static __device__ __forceinline__ float max_of(const uint4& v) {
     return fmaxf(fmaxf(get(v, 0), get(v, 1)), fmaxf(get(v, 2), get(v, 3)));
-  }
-  static __device__ __forceinline__ void values(const uint4& v, float* x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = max_nan(get(v, i), kLpFloor);
   }
   // how many are >= t
   static __device__ __forceinline__ int count(const uint4& v, float t) {
@@ -107,16 +141,6 @@ struct LpVec<__nv_bfloat16> {
     const float2 m = __bfloat1622float2(__hmax2(__hmax2(pair(v.x), pair(v.y)), __hmax2(pair(v.z), pair(v.w))));
     return fmaxf(m.x, m.y);
   }
-  static __device__ __forceinline__ void values(const uint4& v, float* x) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 c = __hmax2_nan(pair(w[i]), __float2bfloat162_rn(kLpFloor));
-      const uint32_t u = *reinterpret_cast<const uint32_t*>(&c);
-      x[2 * i] = __uint_as_float(u << 16);
-      x[2 * i + 1] = __uint_as_float(u & 0xffff0000u);
-    }
-  }
   static __device__ __forceinline__ int count(const uint4& v, float t) {
     const __nv_bfloat162 tt = __float2bfloat162_rn(t);  // t is a bf16 number
     const __nv_bfloat162 n = __hadd2(__hadd2(__hge2(pair(v.x), tt), __hge2(pair(v.y), tt)),
@@ -131,89 +155,83 @@ struct LpVec<__nv_bfloat16> {
 };
 
 struct LpThread {
-  LpState s;
-  int best_id;
-  int before;  // tokens that come before the given one
+  float ref, S, W;  // reference logit (-inf: none yet), sum of e = 2^d, sum of e d, d = (l - ref) k
+  float best;       // largest logit
+  int before;       // tokens that come before the given one
 };
+constexpr float kLpRaise = 24.f;
+// The sums of a thread or a warp seen from another reference, at or above its own.
+__device__ __forceinline__ void lp_move(float& S, float& W, float ref, float to, float k) {
+  if (ref == -INFINITY) return;  // nothing yet (or NaN, which stays)
+  float d;
+  const float f = lp_shift(ref, to, k, d);
+  W = f * fmaf(S, d, W);
+  S *= f;
+}
+__device__ __forceinline__ void lp_add(float x, float ref, float k, float& S, float& W) {
+  const float d = max_nan((x - ref) * k, -1e30f);  // a masked token: e = 0, and e d = 0 stays a number
+  const float e = ex2_approx(d);
+  S += e;
+  W = fmaf(e, d, W);
+}
+__device__ __forceinline__ void lp_raise(LpThread& t, float bm, float k) {
+  if (bm == -INFINITY || (bm - t.ref) * k <= kLpRaise) return;
+  lp_move(t.S, t.W, t.ref, bm, k);
+  t.ref = bm;
+}
 // One element on its own.
 __device__ __forceinline__ void lp_one(LpThread& t, float x, int id, float k, float mine, int my_id) {
   t.before += (x > mine || (x == mine && id < my_id)) ? 1 : 0;
-  if (x != x) {
-    t.s.R = x;
-    return;
-  }
-  if (x > t.s.m || t.best_id < 0) t.best_id = id;
-  if (x == -INFINITY) return;
-  LpState e;
-  e.m = x;
-  e.R = e.W = 0.f;
-  t.s = lp_join(t.s, e, k);
+  t.best = fmaxf(t.best, x);
+  lp_raise(t, x, k);
+  lp_add(x, t.ref == -INFINITY ? 0.f : t.ref, k, t.S, t.W);
 }
-// A batch of loads, id0[u] the id of load u's first element.  Best tokens below kLpFloor are left to lp_one (see the kernel).
-template <typename T>
-__device__ __forceinline__ void lp_batch(LpThread& t, const uint4 (&raw)[LpVec<T>::B], const int (&id0)[LpVec<T>::B],
-                                         float k, float mine, float mine_next, int my_id) {
+// A batch of loads NT apart, id0 the id of the first one's first element; the first `valid` hold logits, the rest
+// -inf, which adds nothing to the sums and must not be counted.  Returns the batch's maximum.
+template <typename T, int NT>
+__device__ __forceinline__ float lp_batch(LpThread& t, const uint4 (&raw)[LpVec<T>::B], int id0, int valid, float k, float mine, float mine_next, int my_id) {
   using V = LpVec<T>;
-  float x[V::B * V::N];
   float bm = V::max_of(raw[0]);
 #pragma unroll
   for (int u = 1; u < V::B; ++u) bm = fmaxf(bm, V::max_of(raw[u]));
+  t.best = fmaxf(t.best, bm);
+  lp_raise(t, bm, k);
+  const float ref = t.ref == -INFINITY ? 0.f : t.ref;  // nothing but masked tokens yet: e = 0 for each
+  const uint64_t kk = f2_pack(k, k), minus = f2_pack(-ref, -ref);
+  uint64_t S2 = f2_pack(t.S, 0.f), W2 = f2_pack(t.W, 0.f);
 #pragma unroll
-  for (int u = 0; u < V::B; ++u) V::values(raw[u], x + u * V::N);
-  if (bm > t.s.m || t.best_id < 0) {  // a new best token: the old one joins the sums, the new one stays out
-    int at = -1;
+  for (int u = 0; u < V::B; ++u)
 #pragma unroll
-    for (int i = V::B * V::N - 1; i >= 0; --i)
-      if (V::get(raw[i / V::N], i % V::N) == bm) at = i;
-    if (at >= 0) {
-      t.best_id = 0;
-#pragma unroll
-      for (int u = 0; u < V::B; ++u)
-        if (at / V::N == u) t.best_id = id0[u] + at % V::N;
-      if (bm > -INFINITY) {
-        LpState e;
-        e.m = bm;
-        e.R = e.W = 0.f;
-        t.s = lp_join(t.s, e, k);
-#pragma unroll
-        for (int i = 0; i < V::B * V::N; ++i)
-          if (i == at) x[i] = kLpFloor;
-      }
+    for (int i = 0; i < V::N; i += 2) {
+      float d0, d1;
+      f2_unpack(f2_mul(f2_add(f2_pack(V::get(raw[u], i), V::get(raw[u], i + 1)), minus), kk), d0, d1);
+      d0 = max_nan(d0, -1e30f);  // a masked token: e = 0, and e d = 0 stays a number
+      d1 = max_nan(d1, -1e30f);
+      const uint64_t e = f2_pack(ex2_approx(d0), ex2_approx(d1));
+      S2 = f2_add(S2, e);
+      W2 = f2_fma(e, f2_pack(d0, d1), W2);
     }
-  }
-  const float m = t.s.m == -INFINITY ? 0.f : fmaxf(t.s.m, kLpFloor);  // nothing but masked tokens yet: e = 0 for each
+  float a, b;
+  f2_unpack(S2, a, b);
+  t.S = a + b;
+  f2_unpack(W2, a, b);
+  t.W = a + b;
+  // tokens before the given one count when equal to it
+  if (my_id < id0 || my_id >= id0 + (V::B - 1) * NT * V::N + V::N) {
+    const float least = my_id < id0 ? mine_next : mine;
 #pragma unroll
-  for (int i = 0; i < V::B * V::N; ++i) {
-    const float d = (x[i] - m) * k;
-    const float e = ex2_approx(d);
-    t.s.R += e;
-    t.s.W = fmaf(e, d, t.s.W);
-  }
+    for (int u = 0; u < V::B; ++u)
+      if (u < valid) t.before += V::count(raw[u], least);
+  } else {
 #pragma unroll
-  for (int u = 0; u < V::B; ++u) {
-    // tokens before the given one count when equal to it
-    if (my_id >= id0[u] && my_id < id0[u] + V::N) {
+    for (int u = 0; u < V::B; ++u)
 #pragma unroll
       for (int i = 0; i < V::N; ++i) {
         const float y = V::get(raw[u], i);
-        t.before += (y > mine || (y == mine && id0[u] + i < my_id)) ? 1 : 0;
+        t.before += u < valid && (y > mine || (y == mine && id0 + u * NT * V::N + i < my_id)) ? 1 : 0;
       }
-    } else {
-      t.before += V::count(raw[u], id0[u] < my_id ? mine : mine_next);
-    }
   }
-}
-
-__device__ __forceinline__ LpState lp_warp_join(LpState s, float k) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    LpState t;
-    t.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-    t.R = __shfl_xor_sync(0xffffffffu, s.R, o);
-    t.W = __shfl_xor_sync(0xffffffffu, s.W, o);
-    s = lp_join(s, t, k);
-  }
-  return s;
+  return bm;
 }
 
 __device__ __forceinline__ uint32_t lp_cluster_rank() {
@@ -242,33 +260,26 @@ struct LpPart {  // a CTA's part of the row
   int before;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LogprobParams p) {
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LogprobParams p) {
   using V = LpVec<T>;
-  __shared__ LpState s_state[kLpWarps];
-  __shared__ int s_before[kLpWarps];
-  __shared__ uint64_t s_group[kLpGroups];
+  constexpr int kWarps = NT / 32;
+  __shared__ float s_max[kWarps], s_S[kWarps], s_W[kWarps];
+  __shared__ int s_before[kWarps];
+  __shared__ uint32_t s_group[kLpGroups];
   __shared__ uint64_t s_cand[kLpCand];
   __shared__ uint64_t s_top[kLpGroups];
   __shared__ __align__(16) LpPart s_part;
   __shared__ uint64_t s_bound;
-  __shared__ int s_n_cand, s_n_hot;
-  __shared__ int s_hot[kLpThreads];
+  __shared__ int s_n_cand, s_n_hot, s_arg;
+  __shared__ uint16_t s_hot[kLpHot];
+  __shared__ float s_cell[kLpCells][NT];
   if (threadIdx.x == 0) pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = lp_cluster_rank(), ctas = lp_cluster_size();
   const int64_t row = blockIdx.x / ctas;
   const T* base = static_cast<const T*>(p.logits) + row * p.ld;
-  const float temp = p.temperature ? p.temperature[row] : 1.f;
-  const float k = 1.4426950408889634f / temp;
-  const int64_t want = p.ids[row];
-  const bool asked = want >= 0 && want < p.vocab;
-  const int my_id = asked ? static_cast<int>(want) : -1;
-  const float mine = asked ? V::one(base + my_id) + 0.f : INFINITY;  // + 0: one zero
-  const float mine_next = V::next(mine);
-  const int n = p.n_top;
-
   // elements [0, head), vectors, elements [tail, vocab): rows need not start on a 16-byte boundary.  The row's first CTA
   // takes both ends; the vectors are cut evenly.
   const int head = min(p.vocab, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / sizeof(T)));
@@ -279,118 +290,175 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
   const int v_beg = min(n_vec, static_cast<int>(rank) * per), v_end = min(n_vec, v_beg + per);
   const bool ends = rank == 0;
 
+  // the first loads of the stream, then what the sums need: the given token's logit is two latencies away
+  constexpr int step = V::B * NT;
+  uint4 next[V::B];
+  const bool full = v_beg + tid + step - NT < v_end;
+  if (full) {
+#pragma unroll
+    for (int u = 0; u < V::B; ++u) next[u] = __ldg(vec + v_beg + tid + u * NT);
+  }
+  const float temp = p.temperature ? p.temperature[row] : 1.f;
+  const float k = 1.4426950408889634f / temp;
+  const int64_t want = p.ids[row];
+  const bool asked = want >= 0 && want < p.vocab;
+  const int my_id = asked ? static_cast<int>(want) : -1;
+  const float mine = asked ? V::one(base + my_id) + 0.f : INFINITY;  // + 0: one zero
+  const float mine_next = V::next(mine);
+  const int n = p.n_top;
+  if (tid == 0) {
+    s_n_cand = s_n_hot = 0;
+    s_arg = NT;
+    s_bound = 1;
+  }
   LpThread t;
-  auto clear = [&] {
-    t.s.m = -INFINITY;
-    t.s.R = t.s.W = 0.f;
-    t.best_id = -1;
-    t.before = 0;
-  };
-  clear();
+  t.ref = t.best = -INFINITY;
+  t.S = t.W = 0.f;
+  t.before = 0;
   if (ends && tid < head) lp_one(t, V::one(base + tid), tid, k, mine, my_id);
   {
     constexpr uint32_t hidden = V::N == 4 ? 0xff800000u : 0xff80ff80u;  // -inf: what a load past the end counts as
-    uint4 next[V::B];
-    auto load = [&](int v0) {
-#pragma unroll
-      for (int u = 0; u < V::B; ++u) {
-        const int v = v0 + u * kLpThreads;
-        next[u] = v < v_end ? __ldg(vec + v) : make_uint4(hidden, hidden, hidden, hidden);
-      }
+    int v0 = v_beg + tid, i = 0;
+    auto cell = [&](float bm) {
+      float& c = s_cell[i % kLpCells][tid];
+      c = i < kLpCells ? bm : fmaxf(c, bm);
+      ++i;
     };
-    load(v_beg + tid);
-    for (int v0 = v_beg + tid; v0 < v_end; v0 += V::B * kLpThreads) {
+    // full batches, the next one's loads in flight; then the rest
+    for (; v0 + step - NT < v_end; v0 += step) {
       uint4 raw[V::B];
-      int id0[V::B];
+#pragma unroll
+      for (int u = 0; u < V::B; ++u) raw[u] = next[u];
+      const int ahead = v0 + 2 * step - NT < v_end ? v0 + step : v0;  // the last batch loads itself again
+#pragma unroll
+      for (int u = 0; u < V::B; ++u) next[u] = __ldg(vec + ahead + u * NT);
+      cell(lp_batch<T, NT>(t, raw, head + v0 * V::N, V::B, k, mine, mine_next, my_id));
+    }
+    if (v0 < v_end) {
+      uint4 raw[V::B];
 #pragma unroll
       for (int u = 0; u < V::B; ++u) {
-        const int v = v0 + u * kLpThreads;
-        raw[u] = next[u];
-        id0[u] = v < v_end ? head + v * V::N : 0x7fff0000;
+        const int v = v0 + u * NT;
+        raw[u] = v < v_end ? __ldg(vec + v) : make_uint4(hidden, hidden, hidden, hidden);
       }
-      load(v0 + V::B * kLpThreads);
-      lp_batch<T>(t, raw, id0, k, mine, mine_next, my_id);
+      cell(lp_batch<T, NT>(t, raw, head + v0 * V::N, (v_end - v0 + NT - 1) / NT, k, mine, mine_next, my_id));
     }
   }
   if (ends && tail + tid < p.vocab) lp_one(t, V::one(base + tail + tid), tail + tid, k, mine, my_id);
-  if (__syncthreads_or(t.s.m < 0.1f * kLpFloor && t.s.m > -INFINITY)) {
-    // a thread's best logit lies near or below the floor (a mask of the type's lowest value, say): one by one
-    clear();
-    if (ends && tid < head) lp_one(t, V::one(base + tid), tid, k, mine, my_id);
-    for (int v = v_beg + tid; v < v_end; v += kLpThreads)
-      for (int i = 0; i < V::N; ++i) {
-        const int id = head + v * V::N + i;
-        lp_one(t, V::one(base + id), id, k, mine, my_id);
-      }
-    if (ends && tail + tid < p.vocab) lp_one(t, V::one(base + tail + tid), tail + tid, k, mine, my_id);
+  if (NT == kLpThreadsMany && tid == 0 && row + p.ahead < p.rows) {
+    // CTAs that started together reach their selection together: meanwhile the row that will follow on this SM comes to L2
+    const T* after = base + p.ahead * p.ld;
+    const uintptr_t from = (reinterpret_cast<uintptr_t>(after) + 15) & ~uintptr_t(15);
+    const uintptr_t bytes = (reinterpret_cast<uintptr_t>(after + p.vocab) - from) & ~uintptr_t(15);
+    if (reinterpret_cast<uintptr_t>(after + p.vocab) > from + 16)
+      l2_prefetch(reinterpret_cast<const void*>(from), static_cast<uint32_t>(bytes < kLpAhead ? bytes : kLpAhead));
   }
+  const bool any = v_beg + tid < v_end || (ends && (tid < head || tail + tid < p.vocab));
+  const uint32_t my_best = any ? lp_order(t.best) : 0;
 
-  // this CTA's state and rank count, and the bests of its groups of threads
-  const LpState ws = lp_warp_join(t.s, k);
+  // the part's largest logit, the thread that holds it (one of those that do), the groups' largest
+  const float wm = lp_warp_max(t.best);
+  if (lane == 0) s_max[warp] = wm;
+  if (tid < kLpGroups) s_top[tid] = 0;
+  uint32_t gb = my_best;
+#pragma unroll
+  for (int o = NT / kLpGroups / 2; o > 0; o >>= 1) gb = max(gb, __shfl_xor_sync(0xffffffffu, gb, o));
+  if (tid % (NT / kLpGroups) == 0) s_group[tid / (NT / kLpGroups)] = gb;
+  __syncthreads();
+  const float m = lp_warp_max(s_max[lane % kWarps]);
+  if (any && t.best == m) atomicMin(&s_arg, tid);
+  if (n > 0 && tid < kLpGroups) {
+    // the n-th largest of the groups'
+    const uint32_t mineg = s_group[tid];
+    int above = 0;
+#pragma unroll 16
+    for (int i = 0; i < kLpGroups; ++i) above += (s_group[i] > mineg || (s_group[i] == mineg && i < tid)) ? 1 : 0;
+    if (above == n - 1 && mineg) s_bound = static_cast<uint64_t>(mineg) << 32;
+  }
+  __syncthreads();
+  const int arg = s_arg;
+  uint64_t bound = s_bound;
+  // sums from m: every thread's but the best token's own, which one warp makes anew without that token
+  if (tid == arg && m > -INFINITY) t.S = t.W = 0.f;
+  else lp_move(t.S, t.W, t.ref, m, k);
+  const float S = warp_sum(t.S), W = warp_sum(t.W);
   const int wb = __reduce_add_sync(0xffffffffu, t.before);
   if (lane == 0) {
-    s_state[warp] = ws;
+    s_S[warp] = S;
+    s_W[warp] = W;
     s_before[warp] = wb;
   }
-  const uint64_t my_best = t.best_id >= 0 ? lp_key(t.s.m, t.best_id) : 0;
-  if (tid == 0) s_n_cand = s_n_hot = 0;
-  if (tid < kLpGroups) s_top[tid] = 0;
-  uint64_t gb = my_best;
-#pragma unroll
-  for (int o = kLpThreads / kLpGroups / 2; o > 0; o >>= 1) gb = max(gb, __shfl_xor_sync(0xffffffffu, gb, o));
-  if (tid % (kLpThreads / kLpGroups) == 0) s_group[tid / (kLpThreads / kLpGroups)] = gb;
+  if (n > 0 && v_beg + tid < v_end && (static_cast<uint64_t>(my_best) << 32 | 0xffffffffu) >= bound) {
+    const int cells = min(kLpCells, (v_end - v_beg - tid + V::B * NT - 1) / (V::B * NT));
+    for (int c = 0; c < cells; ++c)
+      if ((static_cast<uint64_t>(lp_order(s_cell[c][tid])) << 32 | 0xffffffffu) >= bound) {
+        const int at = atomicAdd(&s_n_hot, 1);
+        if (at < kLpHot) s_hot[at] = static_cast<uint16_t>(c * NT + tid);
+      }
+  }
   __syncthreads();
-  if (warp == kLpWarps - 1) {
-    LpState x;
-    x.m = -INFINITY;
-    x.R = x.W = 0.f;
-    if (lane < kLpWarps) x = s_state[lane];
-    x = lp_warp_join(x, k);
-    const int before = __reduce_add_sync(0xffffffffu, lane < kLpWarps ? s_before[lane] : 0);
+  if (warp == 0) {
+    float R = 0.f, Wx = 0.f;
+    int equal = 0;
+    if (m > -INFINITY) {
+      auto add = [&](float x) {
+        if (x == m) ++equal;
+        else lp_add(x, m, k, R, Wx);
+      };
+      if (ends && lane == 0 && arg < head) add(V::one(base + arg));
+      if (ends && lane == 0 && tail + arg < p.vocab) add(V::one(base + tail + arg));
+      for (int v = v_beg + arg + lane * NT; v < v_end; v += 32 * NT) {
+        const uint4 raw = __ldg(vec + v);
+#pragma unroll
+        for (int e = 0; e < V::N; ++e) add(V::get(raw, e));
+      }
+    }
+    if (lane < kWarps) {
+      R += s_S[lane];
+      Wx += s_W[lane];
+    }
+    R = warp_sum(R);
+    Wx = warp_sum(Wx);
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    const int before = __reduce_add_sync(0xffffffffu, lane < kWarps ? s_before[lane] : 0);
     if (lane == 0) {
-      s_part.m = x.m;
-      s_part.R = x.R;
-      s_part.W = x.W;
+      s_part.m = m;
+      s_part.R = R + (equal > 1 ? static_cast<float>(equal - 1) : 0.f);
+      s_part.W = Wx;
       s_part.before = before;
     }
   }
   if (n > 0) {
-    // the n-th best of the groups' bests
-    if (tid < kLpGroups) {
-      const uint64_t mineg = s_group[tid];
-      int above = 0;
-#pragma unroll 16
-      for (int i = 0; i < kLpGroups; ++i) above += (s_group[i] > mineg || (s_group[i] == mineg && i < tid)) ? 1 : 0;
-      if (above == n - 1) s_bound = mineg;
-    }
-    __syncthreads();
-    uint64_t bound = max(s_bound, static_cast<uint64_t>(1));
-    if (my_best >= bound) s_hot[atomicAdd(&s_n_hot, 1)] = tid;
-    __syncthreads();
     const int n_hot = s_n_hot;
     while (true) {
-      for (int i = warp; i < n_hot; i += kLpWarps) {
-        const int h = s_hot[i];
-        auto put = [&](float x, int id) {
-          const uint64_t key = lp_key(x, id);
-          if (x == x && key >= bound) {
-            const int at = atomicAdd(&s_n_cand, 1);
-            if (at < kLpCand) s_cand[at] = key;
-          }
-        };
-        if (ends && lane == 0 && h < head) put(V::one(base + h), h);
-        if (ends && lane == 0 && tail + h < p.vocab) put(V::one(base + tail + h), tail + h);
-        for (int v = v_beg + h + lane * kLpThreads; v < v_end; v += 32 * kLpThreads) {
-          const uint4 raw = __ldg(vec + v);
-#pragma unroll
-          for (int e = 0; e < V::N; ++e) put(V::get(raw, e), head + v * V::N + e);
+      auto put = [&](float x, int id) {
+        const uint64_t key = lp_key(x, id);
+        if (x == x && key >= bound) {
+          const int at = atomicAdd(&s_n_cand, 1);
+          if (at < kLpCand) s_cand[at] = key;
         }
+      };
+      auto put_vec = [&](int v) {
+        const uint4 raw = __ldg(vec + v);
+#pragma unroll
+        for (int e = 0; e < V::N; ++e) put(V::get(raw, e), head + v * V::N + e);
+      };
+      if (ends && tid < head) put(V::one(base + tid), tid);
+      if (ends && tail + tid < p.vocab) put(V::one(base + tail + tid), tail + tid);
+      if (n_hot <= kLpHot) {
+        // V::B lanes a cell: the loads of its batches
+        for (int i = tid / V::B; i < n_hot; i += NT / V::B) {
+          const int h = s_hot[i];
+          for (int v = v_beg + h % NT + (h / NT * V::B + tid % V::B) * NT; v < v_end; v += kLpCells * V::B * NT) put_vec(v);
+        }
+      } else {
+        for (int v = v_beg + tid; v < v_end; v += NT) put_vec(v);
       }
       __syncthreads();
       const int found = s_n_cand;
       const int kept = min(found, kLpCand);
       // rank by counting; keys are distinct
-      for (int i = tid; i < kept; i += kLpThreads) {
+      for (int i = tid; i < kept; i += NT) {
         const uint64_t key = s_cand[i];
         int above = 0;
         for (int j = 0; j < kept; ++j) above += s_cand[j] > key ? 1 : 0;
@@ -452,7 +520,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
   if (ctas == 1) {
     if (tid < n) put_top(tid, s_top[tid]);
   } else {
-    const int total = n * static_cast<int>(ctas);  // at most kLpGroups * kLpMaxCluster = kLpThreads keys
+    const int total = n * static_cast<int>(ctas);  // at most kLpGroups * kLpMaxCluster = kLpThreadsFew keys
     const uint64_t key = tid < total ? lp_peer_u64(&s_top[tid % n], tid / n) : 0;
     __syncwarp();
     lp_cluster_sync();
@@ -466,13 +534,11 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
   }
 }
 
-cudaError_t launch_token_logprobs(const LogprobParams& p, bool bf16, cudaStream_t stream, bool pdl) {
-  // CTAs a row: as many as keep the launch within two CTAs an SM
-  int ctas = 1;
-  while (ctas < kLpMaxCluster && p.rows * ctas * 2 <= 2 * p.sms) ctas *= 2;
+template <typename T, int NT>
+static cudaError_t launch_token_logprobs_t(const LogprobParams& p, int ctas, cudaStream_t stream, bool pdl) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.rows * ctas);
-  cfg.blockDim = dim3(kLpThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * ctas);
+  cfg.blockDim = dim3(NT);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -483,8 +549,19 @@ cudaError_t launch_token_logprobs(const LogprobParams& p, bool bf16, cudaStream_
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return bf16 ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<__nv_bfloat16>, p)
-              : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<float>, p);
+  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NT>, p);
+}
+
+cudaError_t launch_token_logprobs(LogprobParams p, bool bf16, cudaStream_t stream, bool pdl) {
+  // CTAs a row: as many as keep the launch within two CTAs an SM
+  int ctas = 1;
+  while (ctas < kLpMaxCluster && static_cast<int64_t>(p.rows) * ctas <= p.sms) ctas *= 2;
+  if (ctas > 1)
+    return bf16 ? launch_token_logprobs_t<__nv_bfloat16, kLpThreadsFew>(p, ctas, stream, pdl)
+                : launch_token_logprobs_t<float, kLpThreadsFew>(p, ctas, stream, pdl);
+  p.ahead = 4 * p.sms;
+  return bf16 ? launch_token_logprobs_t<__nv_bfloat16, kLpThreadsMany>(p, 1, stream, pdl)
+              : launch_token_logprobs_t<float, kLpThreadsMany>(p, 1, stream, pdl);
 }
 
 }  // namespace gr

@@ -197,6 +197,7 @@ struct LogprobParams {
   float* top_logprob;
   int32_t* top_ids;
   int sms;
+  int ahead;  // rows in flight: a row's CTA prefetches the row this many further on
   int32_t* status;
 };
 
@@ -269,7 +270,7 @@ void kv8_attention_blocks(int rows, int* blocks, int* per_block);
 constexpr int kKv8TicketPairs = 16384;  // (request, K/V head, row block) triples of one call
 constexpr int kKv8MaxSplits = 128;
 constexpr int kKv8MaxChunk = 8192;      // cache tokens of a split
-cudaError_t launch_token_logprobs(const LogprobParams& p, bool bf16, cudaStream_t stream, bool pdl);
+cudaError_t launch_token_logprobs(LogprobParams p, bool bf16, cudaStream_t stream, bool pdl);
 constexpr int kLogprobMaxTop = 64;
 cudaError_t launch_pack_gate_up(const __nv_bfloat16* src, __nv_bfloat16* dst, int I, int H, cudaStream_t s);
 
