@@ -128,8 +128,6 @@ _SIGS = {
     "gr_penalty_cumulate": (_I, [_I, _P, _I, _P, _I, ctypes.POINTER(Sampling), _P]),
     "gr_bd_attention_ordered": (_I, [_P, _P, _P, _L, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _Z, _P,
                                      _P]),
-}
-_SIGS.update({
     "gr_qk_norm_rope_write": (_I, [_P, _L, _I, _I, ctypes.POINTER(KvCache), _P, _P, ctypes.c_double, _P, _P, _P, _P, _I, _I,
                                    _P, _P, _P, _P]),
     "gr_kv_read": (_I, [ctypes.POINTER(KvCache), _P, _L, _P, _P, _P, _P]),
@@ -137,7 +135,7 @@ _SIGS.update({
     "gr_kv8_attention_plan": (_I, [_I, _I, _I, _I, _I, _P]),
     "gr_kv8_attention": (_I, [_P, ctypes.POINTER(KvCache), _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _Z, _P, _P]),
     "gr_token_logprobs": (_I, [_P, _I, _L, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P]),
-})
+}
 GR_ERR_SCRATCH_LIMIT = 8
 NOALLOC_SCRATCH_BYTES = 8 << 20
 
@@ -145,6 +143,8 @@ NOALLOC_SCRATCH_BYTES = 8 << 20
 def load(path: Optional[str] = None):
     """Load the library (once).  Raises if it is missing: there is no CPU or library fallback."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -335,22 +335,33 @@ KV_BF16, KV_E4M3, KV_INT8 = range(3)
 _KV_FORMATS = {torch.bfloat16: KV_BF16, torch.float8_e4m3fn: KV_E4M3, torch.int8: KV_INT8}
 
 
-def _same_device(first: torch.Tensor, **others: Optional[torch.Tensor]) -> None:
-    for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise RuntimeError(f"{name} is on {t.device}, the call's other tensors on {first.device}")
+def _bad(t: torch.Tensor, dtype: torch.dtype, device: int, n: int, name: str, exact: bool) -> None:
+    """What is wrong with an argument that ``_arg`` did not take."""
+    _need(t, dtype, name)
+    if t.get_device() != device:
+        raise RuntimeError(f"{name} is on cuda:{t.get_device()}, the call's other tensors on cuda:{device}")
+    raise RuntimeError(f"{name} holds {t.numel()} elements, the call needs {'' if exact else 'at least '}{n}")
 
 
-def _numel(t: torch.Tensor, n: int, name: str) -> None:
-    if t.numel() != n:
-        raise RuntimeError(f"{name} holds {t.numel()} elements, the call needs {n}")
+def _arg(t: torch.Tensor, dtype: torch.dtype, device: int, n: int, name: str) -> int:
+    """Pointer of a contiguous tensor of n elements on the call's device."""
+    if t.dtype is not dtype or t.get_device() != device or t.numel() != n or not t.is_contiguous():
+        _bad(t, dtype, device, n, name, True)
+    return t.data_ptr()
 
 
-def _status_ok(status: Optional[torch.Tensor]) -> None:
-    if status is not None:
-        _need(status, torch.int32, "status")
-        if status.numel() < 1:
-            raise RuntimeError("status is empty")
+def _arg_least(t: torch.Tensor, dtype: torch.dtype, device: int, n: int, name: str) -> int:
+    if t.dtype is not dtype or t.get_device() != device or t.numel() < n or not t.is_contiguous():
+        _bad(t, dtype, device, n, name, False)
+    return t.data_ptr()
+
+
+def _call(device: int, stream, fn, *args) -> int:
+    """fn(*args, stream) with ``device`` current, on the given stream or the device's current one."""
+    if device == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream)
+    with torch.cuda.device(device):
+        return fn(*args, _stream(stream))
 
 
 def kv_cache(k: torch.Tensor, v: torch.Tensor, k_exp: Optional[torch.Tensor] = None,
@@ -373,10 +384,14 @@ def kv_cache(k: torch.Tensor, v: torch.Tensor, k_exp: Optional[torch.Tensor] = N
             _need(t, torch.int8, name)
             if t.shape != k.shape[:3]:
                 raise RuntimeError(f"{name} must be {tuple(k.shape[:3])}, got {tuple(t.shape)}")
-    _same_device(k, v=v, k_exp=k_exp, v_exp=v_exp)
+    for t, name in ((v, "v"), (k_exp, "k_exp"), (v_exp, "v_exp")):
+        if t is not None and t.device != k.device:
+            raise RuntimeError(f"{name} is on {t.device}, k on {k.device}")
     c.n_pages, c.n_kv_heads, c.page_size = k.shape[0], k.shape[1], 16
     c.k, c.v, c.k_exp, c.v_exp = _ptr(k), _ptr(v), _ptr(k_exp), _ptr(v_exp)
     c.tensors = (k, v, k_exp, v_exp)
+    c.device = k.get_device()
+    c.ref = ctypes.byref(c)
     return c
 
 
@@ -386,49 +401,40 @@ def qk_norm_rope_write(qkv: torch.Tensor, n_q_heads: int, cache: KvCache, row_sl
                        status=None, stream=None) -> None:
     """Projected rows qkv [m, >= (n_q_heads + 2 kv_heads) * 128] bf16 (a row stride is allowed): per-head norms of q and k
     (optional), the rotation, q to q_out, k and v to the cache at row_slot (gr_qk_norm_rope_write)."""
-    if not qkv.is_cuda or qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+    if qkv.dtype is not torch.bfloat16 or qkv.dim() != 2 or not qkv.is_cuda or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
         raise RuntimeError("qkv must be a CUDA bf16 [m, width] tensor with unit column stride")
-    m, heads = qkv.shape[0], n_q_heads + 2 * cache.n_kv_heads
-    if m < 1 or n_q_heads < 1 or qkv.shape[1] < heads * 128:
+    dev = cache.device
+    m, width = qkv.shape
+    heads = n_q_heads + 2 * cache.n_kv_heads
+    if m < 1 or n_q_heads < 1 or width < heads * 128:
         raise RuntimeError(f"qkv {tuple(qkv.shape)} does not hold {heads} heads of 128")
-    _need(row_slot, torch.int64, "row_slot")
-    _need(q_out, torch.bfloat16, "q_out")
-    _numel(row_slot, m, "row_slot")
-    _numel(q_out, m * n_q_heads * 128, "q_out")
-    for t, n, dt, name in ((row_pos, m, torch.int32, "row_pos"), (row_pos3, 3 * m, torch.int32, "row_pos3"),
-                           (inv_freq, rotary_dim // 2, torch.float32, "inv_freq"), (q_norm, 128, torch.bfloat16, "q_norm"),
-                           (k_norm, 128, torch.bfloat16, "k_norm")):
-        if t is not None:
-            _need(t, dt, name)
-            _numel(t, n, name)
-    _status_ok(status)
-    _same_device(qkv, cache=cache.tensors[0], row_slot=row_slot, q_out=q_out, row_pos=row_pos, row_pos3=row_pos3,
-                 inv_freq=inv_freq, q_norm=q_norm, k_norm=k_norm, status=status)
-    sec = None if mrope_section is None else (ctypes.c_int32 * 3)(*mrope_section)
-    with torch.cuda.device(qkv.device):
-        rc = load().gr_qk_norm_rope_write(qkv.data_ptr(), qkv.stride(0) if m > 1 else max(qkv.stride(0), qkv.shape[1]), m,
-                                          n_q_heads, ctypes.byref(cache), _ptr(q_norm), _ptr(k_norm), eps,
-                                          _ptr(row_pos), _ptr(row_pos3), sec, _ptr(inv_freq), rotary_dim,
-                                          1 if rope_half else 0, row_slot.data_ptr(), q_out.data_ptr(), _ptr(status),
-                                          _stream(stream))
-    _check(rc, "gr_qk_norm_rope_write")
+    if qkv.get_device() != dev:
+        raise RuntimeError(f"qkv is on {qkv.device}, the cache on cuda:{dev}")
+    rc = _call(dev, stream, load().gr_qk_norm_rope_write, qkv.data_ptr(), qkv.stride(0) if m > 1 else width, m, n_q_heads,
+               cache.ref,
+               None if q_norm is None else _arg(q_norm, torch.bfloat16, dev, 128, "q_norm"),
+               None if k_norm is None else _arg(k_norm, torch.bfloat16, dev, 128, "k_norm"), eps,
+               None if row_pos is None else _arg(row_pos, torch.int32, dev, m, "row_pos"),
+               None if row_pos3 is None else _arg(row_pos3, torch.int32, dev, 3 * m, "row_pos3"),
+               None if mrope_section is None else (ctypes.c_int32 * 3)(*mrope_section),
+               None if inv_freq is None else _arg(inv_freq, torch.float32, dev, rotary_dim // 2, "inv_freq"), rotary_dim,
+               1 if rope_half else 0, _arg(row_slot, torch.int64, dev, m, "row_slot"),
+               _arg(q_out, torch.bfloat16, dev, m * n_q_heads * 128, "q_out"),
+               None if status is None else _arg_least(status, torch.int32, dev, 1, "status"))
+    if rc:
+        _check(rc, "gr_qk_norm_rope_write")
 
 
 def kv_read(cache: KvCache, slots: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, *, status=None,
             stream=None) -> None:
     """Cache rows at ``slots`` (int64 [n]) back in bf16: k_out / v_out [n, kv_heads * 128] (gr_kv_read)."""
-    _need(slots, torch.int64, "slots")
-    _need(k_out, torch.bfloat16, "k_out")
-    _need(v_out, torch.bfloat16, "v_out")
-    n = slots.numel()
-    _numel(k_out, n * cache.n_kv_heads * 128, "k_out")
-    _numel(v_out, n * cache.n_kv_heads * 128, "v_out")
-    _status_ok(status)
-    _same_device(slots, cache=cache.tensors[0], k_out=k_out, v_out=v_out, status=status)
-    with torch.cuda.device(slots.device):
-        rc = load().gr_kv_read(ctypes.byref(cache), slots.data_ptr(), n, k_out.data_ptr(), v_out.data_ptr(), _ptr(status),
-                               _stream(stream))
-    _check(rc, "gr_kv_read")
+    dev, n = cache.device, slots.numel()
+    out = n * cache.n_kv_heads * 128
+    rc = _call(dev, stream, load().gr_kv_read, cache.ref, _arg(slots, torch.int64, dev, n, "slots"), n,
+               _arg(k_out, torch.bfloat16, dev, out, "k_out"), _arg(v_out, torch.bfloat16, dev, out, "v_out"),
+               None if status is None else _arg_least(status, torch.int32, dev, 1, "status"))
+    if rc:
+        _check(rc, "gr_kv_read")
 
 
 def kv8_attention_workspace_bytes(bs: int, K: int, n_q_heads: int, n_kv_heads: int, max_splits: int) -> int:
@@ -446,26 +452,22 @@ def kv8_attention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, seq
                   draft: int, base_add: int, n_q_heads: int, chunk: int, max_splits: int, out: torch.Tensor,
                   workspace: Optional[torch.Tensor], *, status=None, stream=None) -> None:
     """``bd_attention`` over an 8-bit cache; K = 1 is the attention of one new token (gr_kv8_attention)."""
-    _need(q, torch.bfloat16, "q")
-    _need(out, torch.bfloat16, "out")
-    _need(page_table, torch.int32, "page_table")
-    _need(seq_lens, torch.int64, "seq_lens")
-    if q.numel() < bs * K * n_q_heads * 128 or out.numel() < bs * K * n_q_heads * 128:
-        raise RuntimeError(f"q / out hold fewer than bs * K = {bs * K} rows of {n_q_heads} heads")
-    if page_table.dim() != 2 or page_table.shape[0] < bs or seq_lens.numel() < bs:
-        raise RuntimeError(f"page_table {tuple(page_table.shape)} / seq_lens {tuple(seq_lens.shape)} hold fewer than {bs} requests")
-    _status_ok(status)
-    if workspace is not None:
-        _need(workspace, workspace.dtype, "workspace")
-    _same_device(q, cache=cache.tensors[0], page_table=page_table, seq_lens=seq_lens, out=out, workspace=workspace,
-                 status=status)
-    with torch.cuda.device(q.device):
-        rc = load().gr_kv8_attention(q.data_ptr(), ctypes.byref(cache), page_table.data_ptr(), page_table.shape[1],
-                                     seq_lens.data_ptr(), bs, K, int(draft), base_add, n_q_heads, chunk, max_splits,
-                                     out.data_ptr(), _ptr(workspace),
-                                     0 if workspace is None else workspace.numel() * workspace.element_size(),
-                                     _ptr(status), _stream(stream))
-    _check(rc, "gr_kv8_attention")
+    dev, n = cache.device, bs * K * n_q_heads * 128
+    if page_table.dim() != 2 or page_table.shape[0] < bs:
+        raise RuntimeError(f"page_table {tuple(page_table.shape)} holds fewer than {bs} requests")
+    pages = page_table.shape[1]
+    if workspace is None:
+        ws, ws_bytes = None, 0
+    else:
+        ws_bytes = workspace.numel() * workspace.element_size()
+        ws = _arg_least(workspace, workspace.dtype, dev, 0, "workspace")
+    rc = _call(dev, stream, load().gr_kv8_attention, _arg_least(q, torch.bfloat16, dev, n, "q"), cache.ref,
+               _arg_least(page_table, torch.int32, dev, bs * pages, "page_table"), pages,
+               _arg_least(seq_lens, torch.int64, dev, bs, "seq_lens"), bs, K, int(draft), base_add, n_q_heads, chunk,
+               max_splits, _arg_least(out, torch.bfloat16, dev, n, "out"), ws, ws_bytes,
+               None if status is None else _arg_least(status, torch.int32, dev, 1, "status"))
+    if rc:
+        _check(rc, "gr_kv8_attention")
 
 
 # ---------------------------------------------------------------------- log probabilities
@@ -475,35 +477,25 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, logprob: torch.Tenso
                    stream=None) -> None:
     """Log probability, rank and entropy of ids [rows] under softmax(logits / temperature), and the best alternatives into
     top_logprob / top_ids [rows, n].  logits: fp32 or bf16 [rows, vocab]; a row stride is allowed (gr_token_logprobs)."""
-    if not logits.is_cuda or logits.dtype not in (torch.float32, torch.bfloat16) or logits.dim() != 2 or (
+    bf16 = logits.dtype is torch.bfloat16
+    if not (bf16 or logits.dtype is torch.float32) or logits.dim() != 2 or not logits.is_cuda or (
             logits.shape[1] > 1 and logits.stride(1) != 1):
         raise RuntimeError("logits must be a CUDA fp32 or bf16 [rows, vocab] tensor with unit column stride")
     rows, vocab = logits.shape
-    _need(ids, torch.int64, "ids")
-    _need(logprob, torch.float32, "logprob")
-    _need(entropy, torch.float32, "entropy")
-    _need(rank, torch.int32, "rank")
-    for t, name in ((ids, "ids"), (logprob, "logprob"), (entropy, "entropy"), (rank, "rank")):
-        _numel(t, rows, name)
-    if temperature is not None:
-        _need(temperature, torch.float32, "temperature")
-        _numel(temperature, rows, "temperature")
-    n_top = 0
+    dev, n_top, top, tid = logits.get_device(), 0, None, None
     if (top_logprob is None) != (top_ids is None):
         raise RuntimeError("top_logprob and top_ids come together")
     if top_ids is not None:
-        _need(top_logprob, torch.float32, "top_logprob")
-        _need(top_ids, torch.int32, "top_ids")
         if top_ids.dim() != 2 or top_ids.shape[0] != rows or top_logprob.shape != top_ids.shape:
             raise RuntimeError(f"top_logprob / top_ids must be [{rows}, n]")
         n_top = top_ids.shape[1]
-    _status_ok(status)
-    _same_device(logits, ids=ids, logprob=logprob, entropy=entropy, rank=rank, top_logprob=top_logprob, top_ids=top_ids,
-                 temperature=temperature, status=status)
-    with torch.cuda.device(logits.device):
-        rc = load().gr_token_logprobs(logits.data_ptr(), int(logits.dtype == torch.bfloat16),
-                                      logits.stride(0) if rows > 1 else max(logits.stride(0), vocab), rows, vocab,
-                                      ids.data_ptr(), _ptr(temperature), n_top, logprob.data_ptr(), entropy.data_ptr(),
-                                      rank.data_ptr(), _ptr(top_logprob), _ptr(top_ids), _ptr(status),
-                                      _stream(stream))
-    _check(rc, "gr_token_logprobs")
+        top = _arg(top_logprob, torch.float32, dev, rows * n_top, "top_logprob")
+        tid = _arg(top_ids, torch.int32, dev, rows * n_top, "top_ids")
+    rc = _call(dev, stream, load().gr_token_logprobs, logits.data_ptr(), bf16, logits.stride(0) if rows > 1 else vocab, rows,
+               vocab, _arg(ids, torch.int64, dev, rows, "ids"),
+               None if temperature is None else _arg(temperature, torch.float32, dev, rows, "temperature"), n_top,
+               _arg(logprob, torch.float32, dev, rows, "logprob"), _arg(entropy, torch.float32, dev, rows, "entropy"),
+               _arg(rank, torch.int32, dev, rows, "rank"), top, tid,
+               None if status is None else _arg_least(status, torch.int32, dev, 1, "status"))
+    if rc:
+        _check(rc, "gr_token_logprobs")

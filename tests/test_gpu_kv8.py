@@ -555,5 +555,7 @@ def test_wrappers_refuse():
     pt = torch.zeros((1, 4), dtype=torch.int32, device=DEV)
     with pytest.raises(RuntimeError, match="fewer than"):
         L.kv8_attention(q, h, pt, slots, 2, 1, 0, 0, 2, 32, 1, q, None)
+    with pytest.raises(RuntimeError, match="at least"):
+        L.kv8_attention(q, h, pt.expand(2, 4).contiguous(), slots, 2, 1, 0, 0, 2, 32, 1, q, None)
     with pytest.raises(RuntimeError, match="invalid argument"):
         L.kv8_attention(q, h, pt, slots, 1, 1, 0, 0, 2, 32, 2, q, None)
