@@ -836,10 +836,10 @@ int gr_qk_norm_rope_write(const void* qkv, int64_t ld_qkv, int m, int n_q_heads,
   if (rc) return rc;
   if (!qkv || m <= 0 || n_q_heads <= 0 || !row_slot || !q_out || !(eps >= 0.0)) return GR_ERR_ARG;
   if (n_q_heads > 1024 || cache->n_kv_heads > 1024) return GR_ERR_UNSUPPORTED;
-  if (ld_qkv < static_cast<int64_t>(n_q_heads + 2 * cache->n_kv_heads) * 128 || ld_qkv % 4 || !aligned(qkv, 8) ||
-      !aligned(q_out, 8) || !aligned(q_norm, 8) || !aligned(k_norm, 8))
+  if (ld_qkv < static_cast<int64_t>(n_q_heads + 2 * cache->n_kv_heads) * 128 || ld_qkv % 8 || !aligned(qkv, 16) ||
+      !aligned(q_out, 16) || !aligned(q_norm, 16) || !aligned(k_norm, 16))
     return GR_ERR_ARG;
-  if (rotary_dim < 0 || rotary_dim > 128 || rotary_dim % 8) return GR_ERR_ARG;
+  if (rotary_dim < 0 || rotary_dim > 128 || rotary_dim % (rope_half ? 16 : 8)) return GR_ERR_ARG;
   if (rotary_dim > 0 && (!inv_freq || (!row_pos && !row_pos3))) return GR_ERR_ARG;
   if (row_pos && row_pos3) return GR_ERR_ARG;
   if (row_pos3 && (!mrope_section || mrope_section[0] < 0 || mrope_section[1] < 0 || mrope_section[2] < 0 ||

@@ -2,8 +2,9 @@
 //
 // qk_norm_rope_write: one pass over projected rows [q heads | k heads | v heads] x 128.  q and k heads get their RMS norm
 // (optional) and the rotation, q goes to q_out in bf16, k and v rows go to the cache at the row's slot.  A warp owns a
-// row, or a share of its heads when there are few rows: its lanes compute the row's cos / sin once, in registers, and
-// a head is 32 lanes x 4 elements, so norms and row maxima are warp reductions.
+// row, or a share of its heads when there are few rows.  Its lanes compute the row's cos / sin once, into shared memory; a
+// head is 16 lanes x 8 elements (16-byte loads and stores), so a warp works on two heads of a kind at a time and norms
+// and row maxima are four shuffles for both.
 // q is computed in fp32 and rounded once to bf16.  An 8-bit k row is computed in fp64 (position angle, norm, rotation) and
 // rounded once to its grid: an fp32 result would land on the wrong side of a rounding border about once in 10^6
 // elements, and the cached codes would then depend on the kernel's operation order.
@@ -15,158 +16,218 @@ namespace gr {
 constexpr int kWriteThreads = 128;
 constexpr int kReadThreads = 256;
 
-__device__ __forceinline__ double shfl_d(double v, int src) {
-  return __hiloint2double(__shfl_sync(0xffffffffu, __double2hiint(v), src),
-                          __shfl_sync(0xffffffffu, __double2loint(v), src));
+__device__ __forceinline__ void unpack8(const uint4& raw, float (&x)[8]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
 }
-__device__ __forceinline__ void load4(const __nv_bfloat16* src, float (&x)[4]) {
-  const uint2 raw = *reinterpret_cast<const uint2*>(src);
-  x[0] = __uint_as_float(raw.x << 16);
-  x[1] = __uint_as_float(raw.x & 0xffff0000u);
-  x[2] = __uint_as_float(raw.y << 16);
-  x[3] = __uint_as_float(raw.y & 0xffff0000u);
+__device__ __forceinline__ void store8(__nv_bfloat16* dst, const float (&y)[8]) {
+  *reinterpret_cast<uint4*>(dst) =
+      make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
 }
-__device__ __forceinline__ void store4(__nv_bfloat16* dst, const float (&y)[4]) {
-  uint2 pk;
-  pk.x = pack_bf16(y[0], y[1]);
-  pk.y = pack_bf16(y[2], y[3]);
-  *reinterpret_cast<uint2*>(dst) = pk;
+// Sum / maximum over the 16 lanes of a head.
+template <typename T>
+__device__ __forceinline__ T head_sum(T v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ int head_max(int v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
 
-// Norm and rotation of one head in T (float or double): y = rope(x * rsqrt(mean x^2 + eps) * w).  c / s: this lane's
-// four cosines and signed sines; partner elements are x[i ^ 1] (interleaved) or the same i of lane `src` (half-split).
-template <typename T, bool HALF>
-__device__ __forceinline__ void norm_rotate(const float (&x)[4], const float* w, double eps, bool rot, int src,
-                                            const T (&c)[4], const T (&s)[4], T (&y)[4]) {
+// Where pair i of the row's (cos, sin) lies: lanes that read together read side by side.
+template <bool HALF>
+__device__ __forceinline__ int pair_slot(int i) {
+  return HALF ? (i & 7) * 8 + (i >> 3) : (i & 3) * 16 + (i >> 2);
+}
+// This lane's k-th pair: of its elements 2k, 2k + 1, or (half-split) of its element k and its partner.
+template <bool HALF>
+__device__ __forceinline__ int lane_slot(int k, int l16, int hop) {
+  return HALF ? k * 8 + (l16 < hop ? l16 : (l16 - hop) & 7) : k * 16 + l16;
+}
+// Norm and rotation of a head in T (float or double): y = rope(x * w / sqrt(mean x^2 + eps)); cs(k): this lane's k-th pair.
+template <typename T, bool HALF, typename F>
+__device__ __forceinline__ void norm_rotate(const float (&x)[8], bool norm, const uint4& w, double eps, int rotary_dim,
+                                            int l16, T (&y)[8], F cs) {
+  if (norm) {
+    float wf[8];
+    unpack8(w, wf);
+    T ss = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = x[i];
-  if (w) {
-    T ss = y[0] * y[0] + y[1] * y[1] + y[2] * y[2] + y[3] * y[3];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    for (int i = 0; i < 8; ++i) ss += static_cast<T>(x[i]) * static_cast<T>(x[i]);
+    ss = head_sum(ss);
     const T r = static_cast<T>(rsqrt(ss * static_cast<T>(1.0 / 128) + static_cast<T>(eps)));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] *= r * static_cast<T>(w[i]);
+    for (int i = 0; i < 8; ++i) y[i] = static_cast<T>(x[i] * wf[i]) * r;  // a product of two bf16 is exact in fp32
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i];
   }
-  T z[4];
+  if (rotary_dim == 0) return;
+  const bool rot = l16 * 8 < rotary_dim;
+  if (HALF) {
+    const int hop = rotary_dim >> 4;  // lanes between an element and its partner
+    const bool low = l16 < hop;
+    const int src = (threadIdx.x & 16) | (!rot ? l16 : (low ? l16 + hop : l16 - hop));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) z[i] = HALF ? __shfl_sync(0xffffffffu, y[i], src) : y[i ^ 1];
-  if (rot) {
+    for (int i = 0; i < 8; ++i) {
+      const T z = __shfl_sync(0xffffffffu, y[i], src);
+      const auto c = cs(i);
+      if (rot) y[i] = y[i] * c.x + z * (low ? -c.y : c.y);
+    }
+  } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = y[i] * c[i] + z[i] * s[i];
+    for (int i = 0; i < 4; ++i) {
+      const T a = y[2 * i], b = y[2 * i + 1];
+      const auto c = cs(i);
+      if (rot) {
+        y[2 * i] = a * c.x - b * c.y;
+        y[2 * i + 1] = b * c.x + a * c.y;
+      }
+    }
   }
 }
 
-// One 8-bit row: the warp's 128 values to codes and exponent at byte offset `at` (codes) and index `ai` (exponents).
-template <int FMT>
-__device__ __forceinline__ void put_row(const double (&y)[4], int lane, uint8_t* codes, int8_t* exps) {
-  // largest |y| by its bits, the sign shifted out: NaNs rank highest (an fp64 abs may give a NaN a sign)
-  unsigned long long b = 0;
+// One 8-bit row: the head's 128 values to codes and exponent.
+template <int FMT, typename T>
+__device__ __forceinline__ void put_row(const T (&y)[8], int l16, bool store, uint8_t* codes, int8_t* exps) {
+  // the largest |y| by its bits (NaNs rank highest)
+  int raw;
+  if constexpr (sizeof(T) == 8) {
+    // the high words, one up where the low word is not zero: the exponent's border has zeros below the high word
+    uint32_t b = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) b = max(b, static_cast<unsigned long long>(__double_as_longlong(y[i])) << 1);
-  const int raw = __reduce_max_sync(0xffffffffu, kv_exp_of<FMT>(static_cast<long long>(b >> 1)));
+    for (int i = 0; i < 8; ++i)
+      b = max(b, (static_cast<uint32_t>(__double2hiint(y[i])) & 0x7fffffffu) + (__double2loint(y[i]) != 0 ? 1u : 0u));
+    raw = kv_exp_of<FMT>(static_cast<long long>(static_cast<unsigned long long>(b) << 32));
+  } else {
+    uint32_t b = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b = max(b, __float_as_uint(y[i]) & 0x7fffffffu);
+    raw = kv_exp_of<FMT>(b);
+  }
+  raw = head_max(raw);
   const int e = max(kKvExpMin, min(kKvExpMax, raw));
-  const double f = exp2i64(-e);
-  double q[4];
+  T f;
+  if constexpr (sizeof(T) == 8) f = exp2i64(-e);
+  else f = exp2i(-e);
+  T lo[4], hi[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = fmin(fmax(y[i] * f, -448.0), 448.0);
+  for (int i = 0; i < 4; ++i) {
+    lo[i] = y[i] * f;
+    hi[i] = y[4 + i] * f;
+  }
+  if (raw > kKvExpMax) {  // past the exponents' range: saturate (a bad row's codes are dropped below)
+    constexpr T top = FMT == GR_KV_E4M3 ? 448 : 127;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lo[i] = lo[i] > top ? top : (lo[i] < -top ? -top : lo[i]);
+      hi[i] = hi[i] > top ? top : (hi[i] < -top ? -top : hi[i]);
+    }
+  }
   const bool bad = raw >= (1 << 20);
-  *reinterpret_cast<uint32_t*>(codes + lane * 4) = bad ? 0u : kv_pack<FMT>(q);
-  if (lane == 0) *exps = static_cast<int8_t>(bad ? kKvExpBad : e);
-}
-template <int FMT>
-__device__ __forceinline__ void put_row(const float (&y)[4], int lane, uint8_t* codes, int8_t* exps) {
-  uint32_t b = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) b = max(b, __float_as_uint(y[i]) & 0x7fffffffu);
-  const int raw = __reduce_max_sync(0xffffffffu, kv_exp_of<FMT>(b));
-  const int e = max(kKvExpMin, min(kKvExpMax, raw));
-  const float f = exp2i(-e);
-  float q[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = fminf(fmaxf(y[i] * f, -448.f), 448.f);
-  const bool bad = raw >= (1 << 20);
-  *reinterpret_cast<uint32_t*>(codes + lane * 4) = bad ? 0u : kv_pack<FMT>(q);
-  if (lane == 0) *exps = static_cast<int8_t>(bad ? kKvExpBad : e);
+  const uint2 c = bad ? make_uint2(0u, 0u) : make_uint2(kv_pack<FMT>(lo), kv_pack<FMT>(hi));
+  if (store) {
+    *reinterpret_cast<uint2*>(codes + l16 * 8) = c;
+    if (l16 == 0) *exps = static_cast<int8_t>(bad ? kKvExpBad : e);
+  }
 }
 
 template <int FMT, bool HALF>
 __global__ void __launch_bounds__(kWriteThreads) qk_norm_rope_write_kernel(const KvWriteParams p) {
+  __shared__ double2 s_cs64[FMT != GR_KV_BF16 ? kWriteThreads / 32 : 1][64];
+  __shared__ float2 s_cs32[kWriteThreads / 32][64];
   if (threadIdx.x == 0) pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, l16 = lane & 15, sub = lane >> 4;
   const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kWriteThreads + threadIdx.x) >> 5;
   const int64_t row = unit / p.groups;
   if (row >= p.m) return;
   const int g = static_cast<int>(unit - row * p.groups);
-  const int n_heads = p.n_q_heads + 2 * p.n_kv_heads;
-  // this row's angles: lane l computes pairs l and l + 32, then every lane fetches the pairs of its four elements
-  const int pairs = p.rotary_dim >> 1;
-  double cd[4], sd[4];
-  float cf[4], sf[4];
-  {
-    double c2[2] = {1.0, 1.0}, s2[2] = {0.0, 0.0};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int i = lane + 32 * h;
-      if (i < pairs) {
-        int pos;
-        if (p.row_pos3) pos = p.row_pos3[row * 3 + (i < p.mrope_s0 ? 0 : (i < p.mrope_s0 + p.mrope_s1 ? 1 : 2))];
-        else pos = p.row_pos[row];
-        sincos(static_cast<double>(pos) * static_cast<double>(p.inv_freq[i]), &s2[h], &c2[h]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane * 4 + i;
-      const int pair = HALF ? (d < pairs ? d : d - pairs) : (d >> 1);
-      const double ca = shfl_d(c2[0], pair & 31), cb = shfl_d(c2[1], pair & 31);
-      const double sa = shfl_d(s2[0], pair & 31), sb = shfl_d(s2[1], pair & 31);
-      const bool neg = HALF ? d < pairs : !(i & 1);
-      cd[i] = (pair & 32) ? cb : ca;
-      sd[i] = (pair & 32) ? sb : sa;
-      if (neg) sd[i] = -sd[i];
-      cf[i] = static_cast<float>(cd[i]);
-      sf[i] = static_cast<float>(sd[i]);
-    }
-  }
-  const bool rot = lane * 4 < p.rotary_dim;
-  const int hop = p.rotary_dim >> 3;  // half-split: partner elements are rotary_dim / 2 apart
-  const int src = !HALF || !rot ? lane : (lane < hop ? lane + hop : lane - hop);
-  float wq[4], wk[4];
-  if (p.q_norm) load4(p.q_norm + lane * 4, wq);
-  if (p.k_norm) load4(p.k_norm + lane * 4, wk);
+  // pairs of heads: q, then k, then v; this warp takes g, g + groups, ...
+  const int n_qp = (p.n_q_heads + 1) >> 1, n_kp = (p.n_kv_heads + 1) >> 1;
+  const bool even = !((p.n_q_heads | p.n_kv_heads) & 1);
   int64_t slot = p.row_slot[row];
   if (slot >= p.n_slots) {
-    if (lane == 0) report(p.status, GR_ERR_BAD_PAGE);
+    if (lane == 0 && g == 0) report(p.status, GR_ERR_BAD_PAGE);
     slot = -1;
   }
-  const int64_t page = slot >> 4;
-  const int off = static_cast<int>(slot & 15);
-  const __nv_bfloat16* in = p.qkv + row * p.ld_qkv + lane * 4;
-  for (int h = g; h < n_heads; h += p.groups) {
-    if (h >= p.n_q_heads && slot < 0) break;
-    float x[4];
-    load4(in + h * 128, x);
-    if (h < p.n_q_heads) {
-      float y[4];
-      norm_rotate<float, HALF>(x, p.q_norm ? wq : nullptr, p.eps, rot, src, cf, sf, y);
-      store4(p.q_out + (row * p.n_q_heads + h) * 128 + lane * 4, y);
+  const int n_pairs = slot < 0 ? n_qp : n_qp + 2 * n_kp;
+  const __nv_bfloat16* in = p.qkv + row * p.ld_qkv + l16 * 8;
+  // this lane's head of pair i, from the row's start (an odd count's last pair has one head: its other half repeats it)
+  auto head_of = [&](int i) {
+    if (i < n_qp) return min(2 * i + sub, p.n_q_heads - 1);
+    i -= n_qp;
+    if (i < n_kp) return p.n_q_heads + min(2 * i + sub, p.n_kv_heads - 1);
+    return p.n_q_heads + p.n_kv_heads + min(2 * (i - n_kp) + sub, p.n_kv_heads - 1);
+  };
+  auto load = [&](int i) { return __ldg(reinterpret_cast<const uint4*>(in + (even ? 2 * i + sub : head_of(i)) * 128)); };
+  uint4 next = make_uint4(0, 0, 0, 0), next2 = next;
+  if (g < n_pairs) next = load(g);
+  if (g + p.groups < n_pairs) next2 = load(g + p.groups);
+
+  double2* cs64 = s_cs64[FMT != GR_KV_BF16 ? threadIdx.x >> 5 : 0];
+  float2* cs32 = s_cs32[threadIdx.x >> 5];
+  for (int i = lane; i < (p.rotary_dim >> 1); i += 32) {
+    int pos;
+    if (p.row_pos3) pos = p.row_pos3[row * 3 + (i < p.mrope_s0 ? 0 : (i < p.mrope_s0 + p.mrope_s1 ? 1 : 2))];
+    else pos = p.row_pos[row];
+    // sincospi reduces exactly; the multiplication by 1 / pi is off by 2^-53 of the angle
+    double c, s;
+    sincospi(static_cast<double>(pos) * static_cast<double>(p.inv_freq[i]) * 0.31830988618379067154, &s, &c);
+    if (FMT != GR_KV_BF16) cs64[pair_slot<HALF>(i)] = make_double2(c, s);
+    cs32[pair_slot<HALF>(i)] = make_float2(static_cast<float>(c), static_cast<float>(s));
+  }
+  uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;
+  if (p.q_norm) wq = __ldg(reinterpret_cast<const uint4*>(p.q_norm) + l16);
+  if (p.k_norm) wk = __ldg(reinterpret_cast<const uint4*>(p.k_norm) + l16);
+  __syncwarp();
+  // q's pairs stay in registers, the fp64 ones are read when a k head comes
+  const int hop = p.rotary_dim >> 4;
+  float2 csf[HALF ? 8 : 4];
+#pragma unroll
+  for (int k = 0; k < (HALF ? 8 : 4); ++k) csf[k] = cs32[lane_slot<HALF>(k, l16, hop)];
+  auto cs_f = [&](int k) { return csf[k]; };
+  auto cs_d = [&](int k) { return cs64[lane_slot<HALF>(k, l16, hop)]; };
+
+  const int64_t cache_row = (slot >> 4) * p.n_kv_heads * 16 + (slot & 15);
+  for (int i = g; i < n_pairs; i += p.groups) {
+    float x[8];
+    unpack8(next, x);
+    next = next2;
+    if (i + 2 * p.groups < n_pairs) next2 = load(i + 2 * p.groups);
+    if (i < n_qp) {
+      const int h = 2 * i + sub;
+      float y[8];
+      norm_rotate<float, HALF>(x, p.q_norm != nullptr, wq, p.eps, p.rotary_dim, l16, y, cs_f);
+      if (h < p.n_q_heads) store8(p.q_out + (row * p.n_q_heads + h) * 128 + l16 * 8, y);
       continue;
     }
-    const bool is_k = h < p.n_q_heads + p.n_kv_heads;
-    const int kvh = h - p.n_q_heads - (is_k ? 0 : p.n_kv_heads);
-    const int64_t r = (page * p.n_kv_heads + kvh) * 16 + off;  // the cache row
+    const bool is_k = i < n_qp + n_kp;
+    const int kvh = 2 * (i - n_qp - (is_k ? 0 : n_kp)) + sub;
+    const bool store = kvh < p.n_kv_heads;
+    const int64_t r = cache_row + kvh * 16;
     if (FMT == GR_KV_BF16) {
-      float y[4];
-      if (is_k) norm_rotate<float, HALF>(x, p.k_norm ? wk : nullptr, p.eps, rot, src, cf, sf, y);
-      store4(static_cast<__nv_bfloat16*>(is_k ? p.k : p.v) + r * 128 + lane * 4, is_k ? y : x);
+      float y[8];
+      if (is_k) {
+        norm_rotate<float, HALF>(x, p.k_norm != nullptr, wk, p.eps, p.rotary_dim, l16, y, cs_f);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = x[e];
+      }
+      if (store) store8(static_cast<__nv_bfloat16*>(is_k ? p.k : p.v) + r * 128 + l16 * 8, y);
     } else if (is_k) {
-      double y[4];
-      norm_rotate<double, HALF>(x, p.k_norm ? wk : nullptr, p.eps, rot, src, cd, sd, y);
-      put_row<FMT>(y, lane, static_cast<uint8_t*>(p.k) + r * 128, p.k_exp + r);
+      double y[8];
+      norm_rotate<double, HALF>(x, p.k_norm != nullptr, wk, p.eps, p.rotary_dim, l16, y, cs_d);
+      put_row<FMT>(y, l16, store, static_cast<uint8_t*>(p.k) + r * 128, p.k_exp + r);
     } else {
-      put_row<FMT>(x, lane, static_cast<uint8_t*>(p.v) + r * 128, p.v_exp + r);
+      put_row<FMT>(x, l16, store, static_cast<uint8_t*>(p.v) + r * 128, p.v_exp + r);
     }
   }
 }
@@ -218,11 +279,11 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const KvReadParam
 }
 
 cudaError_t launch_qk_norm_rope_write(KvWriteParams p, int format, bool half, cudaStream_t s, bool pdl) {
-  const int n_heads = p.n_q_heads + 2 * p.n_kv_heads;
+  const int n_pairs = (p.n_q_heads + 1) / 2 + 2 * ((p.n_kv_heads + 1) / 2);
   // a warp per row once that fills the GPU; fewer rows share their heads between warps
   const int64_t want = static_cast<int64_t>(p.sms) * 16;
   int64_t groups = (want + p.m - 1) / p.m;
-  p.groups = static_cast<int>(groups < 1 ? 1 : (groups > n_heads ? n_heads : groups));
+  p.groups = static_cast<int>(groups < 1 ? 1 : (groups > n_pairs ? n_pairs : groups));
   const int64_t units = static_cast<int64_t>(p.m) * p.groups;
   const dim3 grid(static_cast<unsigned>((units + kWriteThreads / 32 - 1) / (kWriteThreads / 32)));
   auto go = [&](auto kern) { return launch_dependent(kern, grid, kWriteThreads, 0, s, pdl, p); };

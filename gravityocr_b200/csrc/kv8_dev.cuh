@@ -46,7 +46,12 @@ __device__ __forceinline__ float kv_scale(int e) {
   return e == kKvExpBad ? __int_as_float(0x7fc00000) : exp2i(e);
 }
 
-// Four values, already scaled by 2^-e and within +-top, to four codes (low byte first).
+// Low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// Four values, already scaled by 2^-e and within +-top, to four codes (low byte first).  Adding 1.5 * 2^23 (2^52 in fp64)
+// rounds to an integer, ties to even, whose low bits are the sum's.
 template <int FMT>
 __device__ __forceinline__ uint32_t kv_pack(const float (&y)[4]) {
   if (FMT == GR_KV_E4M3) {
@@ -54,15 +59,11 @@ __device__ __forceinline__ uint32_t kv_pack(const float (&y)[4]) {
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
     return lo | (hi << 16);
   }
-  uint32_t r = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int q = max(-127, min(127, __float2int_rn(y[i])));
-    r |= static_cast<uint32_t>(q & 0xff) << (8 * i);
-  }
-  return r;
+  constexpr float big = 12582912.f;
+  return low_bytes(__float_as_uint(y[0] + big), __float_as_uint(y[1] + big), __float_as_uint(y[2] + big),
+                   __float_as_uint(y[3] + big));
 }
-// The same from fp64 values, rounded once: adding 1.5 * 2^52 * step rounds to a multiple of step, ties to even.
+// The same from fp64 values, rounded once.
 template <int FMT>
 __device__ __forceinline__ uint32_t kv_pack(const double (&y)[4]) {
   if (FMT == GR_KV_E4M3) {
@@ -74,15 +75,11 @@ __device__ __forceinline__ uint32_t kv_pack(const double (&y)[4]) {
       const double c = __hiloint2double(((k - 3 + 52 + 1023) << 20) | 0x80000, 0);
       f[i] = static_cast<float>(__dsub_rn(__dadd_rn(y[i], c), c));  // exact: a multiple of the step below 2^9
     }
-    return kv_pack<FMT>(f);  // exact: the values are on the grid (above 448 they saturate)
+    return kv_pack<FMT>(f);  // exact: the values are on the grid
   }
-  uint32_t r = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int q = max(-127, min(127, __double2int_rn(y[i])));
-    r |= static_cast<uint32_t>(q & 0xff) << (8 * i);
-  }
-  return r;
+  constexpr double big = 6755399441055744.0;
+  return low_bytes(__double2loint(__dadd_rn(y[0], big)), __double2loint(__dadd_rn(y[1], big)),
+                   __double2loint(__dadd_rn(y[2], big)), __double2loint(__dadd_rn(y[3], big)));
 }
 
 // Two codes in the low 16 bits -> two halves, exact.

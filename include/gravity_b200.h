@@ -292,10 +292,10 @@ typedef struct gr_kv_cache {
   int8_t* v_exp;
 } gr_kv_cache;
 
-/* From m projected rows qkv [m, ld_qkv] bf16 (q heads | k heads | v heads, 128 each; ld_qkv % 4 == 0, 8-byte aligned) in
- * one pass: q and k heads take their RMS norm (q_norm / k_norm bf16 [128], or NULL for none), x * w / sqrt(mean x^2 + eps);
- * then the rotation of their first rotary_dim elements (a multiple of 8, 0..128; rope_half 0: pairs (2i, 2i + 1); 1: pairs
- * (i, i + rotary_dim / 2)) by the angle position * inv_freq[i], formed in 64 bits; q goes to q_out bf16 [m, n_q_heads *
+/* From m projected rows qkv [m, ld_qkv] bf16 (q heads | k heads | v heads, 128 each; ld_qkv % 8 == 0; qkv, q_out and the
+ * norm weights 16-byte aligned) in one pass: q and k heads take their RMS norm (q_norm / k_norm bf16 [128], or NULL for none), x * w / sqrt(mean x^2 + eps);
+ * then the rotation of their first rotary_dim elements (0..128, a multiple of 8, of 16 with rope_half; rope_half 0:
+ * pairs (2i, 2i + 1); 1: pairs (i, i + rotary_dim / 2)) by the angle position * inv_freq[i], formed in 64 bits; q goes to q_out bf16 [m, n_q_heads *
  * 128], k and v rows to the cache at row_slot (page * 16 + offset).  Positions are row_pos [m], or row_pos3 [m][3] with
  * mrope_section (three pair counts, as gr_epilogue); both NULL only with rotary_dim 0.  A negative slot writes q only; a
  * slot past the cache sets GR_ERR_BAD_PAGE and writes q only.  No two rows may share a slot.  Inputs and outputs may not

@@ -82,7 +82,7 @@ WRITES = [
     (1, "int8", False, 64, True, False, 16, 8), (1, "e4m3", True, 128, False, False, 16, 8),
     (3, "bf16", False, 32, True, True, 4, 4), (17, "e4m3", False, 64, False, True, 16, 8),
     (130, "int8", True, 96, True, False, 5, 1), (257, "int8", False, 0, True, False, 2, 2),
-    (257, "e4m3", True, 8, True, True, 7, 7), (1000, "bf16", True, 128, False, False, 16, 2),
+    (257, "e4m3", True, 16, True, True, 7, 7), (33, "int8", False, 8, True, True, 3, 1), (1000, "bf16", True, 128, False, False, 16, 2),
     (2500, "int8", False, 128, True, True, 12, 4), (2500, "e4m3", False, 64, True, False, 16, 8),
 ]
 

@@ -44,10 +44,10 @@ def _write(cache=None, **kw):
                                           a["slot"], a["q"], None, None)
 
 
-@pytest.mark.parametrize("kw", [dict(qkv=None), dict(qkv=P + 4), dict(ld=32 * 128 - 4), dict(ld=32 * 128 + 2), dict(m=0),
+@pytest.mark.parametrize("kw", [dict(qkv=None), dict(qkv=P + 8), dict(ld=32 * 128 - 8), dict(ld=32 * 128 + 4), dict(m=0),
                                 dict(nq=0), dict(eps=-1.0), dict(eps=float("nan")), dict(pos=None), dict(inv=None),
-                                dict(rd=-8), dict(rd=136), dict(rd=60), dict(slot=None), dict(q=None), dict(q=P + 4),
-                                dict(qn=P + 2), dict(kn=P + 2), dict(pos3=P), dict(pos=None, pos3=P),
+                                dict(rd=-8), dict(rd=136), dict(rd=60), dict(rd=56, half=1), dict(slot=None), dict(q=None), dict(q=P + 8),
+                                dict(qn=P + 8), dict(kn=P + 8), dict(pos3=P), dict(pos=None, pos3=P),
                                 dict(pos=None, pos3=P, sec=(8, 12, 11)), dict(pos=None, pos3=P, sec=(-1, 21, 12))])
 def test_write_refuses(kw):
     assert _write(**kw) == ARG
