@@ -79,7 +79,7 @@ __device__ __forceinline__ void norm_rotate(const float (&x)[8], bool norm, cons
     for (int i = 0; i < 8; ++i) {
       const T z = __shfl_sync(0xffffffffu, y[i], src);
       const auto c = cs(i);
-      if (rot) y[i] = y[i] * c.x + z * (low ? -c.y : c.y);
+      if (rot) y[i] = y[i] * c.x + z * c.y;  // c.y has the sign of the element's half
     }
   } else {
 #pragma unroll
@@ -140,7 +140,7 @@ __device__ __forceinline__ void put_row(const T (&y)[8], int l16, bool store, ui
 }
 
 template <int FMT, bool HALF>
-__global__ void __launch_bounds__(kWriteThreads) qk_norm_rope_write_kernel(const KvWriteParams p) {
+__global__ void __launch_bounds__(kWriteThreads, 6) qk_norm_rope_write_kernel(const KvWriteParams p) {
   __shared__ double2 s_cs64[FMT != GR_KV_BF16 ? kWriteThreads / 32 : 1][64];
   __shared__ float2 s_cs32[kWriteThreads / 32][64];
   if (threadIdx.x == 0) pdl_trigger();
@@ -192,9 +192,16 @@ __global__ void __launch_bounds__(kWriteThreads) qk_norm_rope_write_kernel(const
   const int hop = p.rotary_dim >> 4;
   float2 csf[HALF ? 8 : 4];
 #pragma unroll
-  for (int k = 0; k < (HALF ? 8 : 4); ++k) csf[k] = cs32[lane_slot<HALF>(k, l16, hop)];
+  for (int k = 0; k < (HALF ? 8 : 4); ++k) {
+    csf[k] = cs32[lane_slot<HALF>(k, l16, hop)];
+    if (HALF && l16 < hop) csf[k].y = -csf[k].y;
+  }
   auto cs_f = [&](int k) { return csf[k]; };
-  auto cs_d = [&](int k) { return cs64[lane_slot<HALF>(k, l16, hop)]; };
+  auto cs_d = [&](int k) {
+    double2 c = cs64[lane_slot<HALF>(k, l16, hop)];
+    if (HALF && l16 < hop) c.y = -c.y;
+    return c;
+  };
 
   const int64_t cache_row = (slot >> 4) * p.n_kv_heads * 16 + (slot & 15);
   for (int i = g; i < n_pairs; i += p.groups) {
