@@ -7,6 +7,9 @@ Data layout in HBM (bf16 unless noted):
     ``embed`` [V, H], ``norm`` [H], ``lm_head`` [V, H].
   * K/V cache: two tensors [layers, pages, kv_heads, page_size=16, head_dim] -- one (page, head) block of a layer is
     4 KiB contiguous, the TMA box of the attention kernel; requests own fixed page tables [bs, pages_per_req] int32.
+    With an 8-bit ``kv_dtype`` (float8_e4m3fn or int8) the two tensors hold codes and two more, int8
+    [layers, pages, kv_heads, page_size], the rows' exponents: half the memory; the projected rows then go through
+    ``qk_norm_rope_write`` and the attention is ``kv8_attention``.
   * per-forward activations for M = bs*K rows: residual ``h`` fp32 x2 (ping-pong), ``x`` bf16 (normed GEMM input),
     ``q`` / ``attn`` bf16 [M, q_dim], ``y`` fp32 [M, H] (o_proj / down_proj output), ``act`` bf16 [M, I].
   * round state (device, int64 like the reference's ``seq_lens`` / seed pool): ``seq_lens`` (K/V length; x0 not yet
@@ -66,15 +69,21 @@ class DeviceWeights:
 
 
 class PagePool:
-    """Fixed-size page pool of the paged K/V cache; pages are handed out per request and returned on release."""
+    """Fixed-size page pool of the paged K/V cache (bf16, or 8-bit codes with exponents); pages are handed out per request
+    and returned on release."""
 
-    def __init__(self, cfg: ModelConfig, n_pages: int, page_size: int, device: torch.device):
+    def __init__(self, cfg: ModelConfig, n_pages: int, page_size: int, device: torch.device,
+                 dtype: torch.dtype = torch.bfloat16):
         self.cfg = cfg
         self.page_size = page_size
         self.n_pages = n_pages
         shape = (cfg.n_layers, n_pages, cfg.n_kv_heads, page_size, cfg.head_dim)
-        self.k = torch.zeros(shape, dtype=torch.bfloat16, device=device)
-        self.v = torch.zeros(shape, dtype=torch.bfloat16, device=device)
+        self.k = torch.zeros(shape, dtype=dtype, device=device)
+        self.v = torch.zeros(shape, dtype=dtype, device=device)
+        self.k_exp = self.v_exp = None
+        if dtype != torch.bfloat16:
+            self.k_exp = torch.zeros(shape[:-1], dtype=torch.int8, device=device)
+            self.v_exp = torch.zeros(shape[:-1], dtype=torch.int8, device=device)
         self.free: List[int] = list(range(n_pages - 1, -1, -1))
 
     def alloc(self, n: int) -> List[int]:
@@ -86,8 +95,9 @@ class PagePool:
         self.free.extend(int(p) for p in pages)
 
     @staticmethod
-    def bytes_needed(cfg: ModelConfig, n_pages: int, page_size: int) -> int:
-        return 2 * cfg.n_layers * n_pages * cfg.n_kv_heads * page_size * cfg.head_dim * 2
+    def bytes_needed(cfg: ModelConfig, n_pages: int, page_size: int, dtype: torch.dtype = torch.bfloat16) -> int:
+        row = cfg.head_dim * 2 if dtype == torch.bfloat16 else cfg.head_dim + 1
+        return 2 * cfg.n_layers * n_pages * cfg.n_kv_heads * page_size * row
 
 
 # Split chunk (cache tokens per CTA) by (request, kv head) pairs: measured on a B200 with the config-3 prefix mix
@@ -163,22 +173,31 @@ class Engine:
     """One model replica on one GPU: the forward, the round and graph capture."""
 
     def __init__(self, cfg: ModelConfig, weights: Dict[str, torch.Tensor], *, max_rows: int, n_pages: int,
-                 page_size: int = 16, device: Optional[torch.device] = None, pdl: bool = True):
+                 page_size: int = 16, device: Optional[torch.device] = None, pdl: bool = True,
+                 kv_dtype: torch.dtype = torch.bfloat16):
+        """kv_dtype: bfloat16, or float8_e4m3fn / int8 for an 8-bit K/V cache (see the module's data layout)."""
         L.load()
         if page_size != 16:
             raise ValueError("the attention kernel's TMA box is one 16-token page")
+        if kv_dtype not in (torch.bfloat16, torch.float8_e4m3fn, torch.int8):
+            raise ValueError(f"no K/V cache in {kv_dtype}")
+        self.kv8 = kv_dtype != torch.bfloat16
         self.cfg = cfg
         self.device = device or torch.device("cuda", torch.cuda.current_device())
         self.page_size = page_size
         L.set_pdl(pdl)
         self.w = DeviceWeights(cfg, weights, self.device)
-        self.pool = PagePool(cfg, n_pages, page_size, self.device)
+        self.pool = PagePool(cfg, n_pages, page_size, self.device, kv_dtype)
+        pool = self.pool
+        self.kv = [L.kv_cache(pool.k[l], pool.v[l], pool.k_exp[l], pool.v_exp[l])
+                   for l in range(cfg.n_layers)] if self.kv8 else []
         self.max_rows = max_rows
         dev, H = self.device, cfg.hidden
         self.h = [torch.zeros((max_rows, H), dtype=torch.float32, device=dev) for _ in range(2)]
         self.x = torch.zeros((max_rows, H), dtype=torch.bfloat16, device=dev)
         self.q = torch.zeros((max_rows, cfg.q_dim), dtype=torch.bfloat16, device=dev)
         self.attn = torch.zeros((max_rows, cfg.q_dim), dtype=torch.bfloat16, device=dev)
+        self.qkv = torch.zeros((max_rows if self.kv8 else 0, cfg.qkv_dim), dtype=torch.bfloat16, device=dev)
         self.y = torch.zeros((0,), dtype=torch.float32, device=dev)   # split-K partials of o_proj / down_proj
         self._grow_y(max_rows)
         self.act = torch.zeros((max_rows, cfg.intermediate), dtype=torch.bfloat16, device=dev)
@@ -195,7 +214,7 @@ class Engine:
     def gemm_shapes(self) -> List[Tuple[int, int, int]]:
         """(n_out, k_in, epilogue mode) of every projection a forward or a sampled round runs."""
         c = self.cfg
-        return [(c.qkv_dim, c.hidden, L.EPI_QKV_ROPE), (c.hidden, c.q_dim, L.EPI_PARTIAL_F32),
+        return [(c.qkv_dim, c.hidden, L.EPI_STORE_BF16 if self.kv8 else L.EPI_QKV_ROPE), (c.hidden, c.q_dim, L.EPI_PARTIAL_F32),
                 (2 * c.intermediate, c.hidden, L.EPI_SWIGLU), (c.hidden, c.intermediate, L.EPI_PARTIAL_F32),
                 (c.vocab, c.hidden, L.EPI_ARGMAX), (c.vocab, c.hidden, L.EPI_STORE_F32)]
 
@@ -223,10 +242,17 @@ class Engine:
         self._grow_y(m)
 
     def _attn_workspace(self, bs: int, K: int, splits: int) -> torch.Tensor:
-        need = L.attention_workspace_bytes(bs, K, self.cfg.n_q_heads, self.cfg.n_kv_heads, splits)
+        size = L.kv8_attention_workspace_bytes if self.kv8 else L.attention_workspace_bytes
+        need = size(bs, K, self.cfg.n_q_heads, self.cfg.n_kv_heads, splits)
         if self.attn_ws is None or self.attn_ws.numel() < need:
             self.attn_ws = torch.zeros((max(need, 256),), dtype=torch.uint8, device=self.device)
         return self.attn_ws
+
+    def attention_plan(self, bs: int, K: int, max_len: int, avg_len: int) -> Tuple[int, int]:
+        """(chunk, splits) of the attention over up to max_len committed tokens and the K window rows."""
+        if self.kv8:
+            return L.kv8_attention_split(bs, K, max_len + K + 1, self.cfg.n_q_heads, self.cfg.n_kv_heads)
+        return attention_split(bs, K, max_len, avg_len, self.cfg.n_kv_heads, self.sms)
 
     # ------------------------------------------------------------------ forward
     def forward(self, rows_mode: int, bs: int, K: int, seq_lens: torch.Tensor, page_table: torch.Tensor, *,
@@ -269,26 +295,30 @@ class Engine:
         cur = 0
         for l, d in enumerate(w.layers):
             nxt = w.layers[l + 1] if l + 1 < len(w.layers) else None
-            e = L.Epilogue()
-            e.mode = L.EPI_QKV_ROPE
-            e.q_out = self.q.data_ptr()
-            e.k_cache = self.pool.k[l].data_ptr()
-            e.v_cache = self.pool.v[l].data_ptr()
-            e.row_pos = self.row_pos.data_ptr()
-            e.row_slot = self.row_slot.data_ptr()
-            e.inv_freq = w.inv_freq.data_ptr()
-            e.rotary_dim = cfg.rotary_dim
-            if rope_pos3 is not None:
-                e.row_pos3 = rope_pos3.data_ptr()
-                for i in range(3):
-                    e.mrope_section[i] = cfg.mrope_section[i]
-            e.n_q_heads = cfg.n_q_heads
-            e.n_kv_heads = cfg.n_kv_heads
-            e.page_size = self.page_size
-            ops.linear(d["qkv"], self.x, M, e, self.lin_ws, prefetch=d["o"], status=st)
-            ops.bd_attention(self.q, self.pool.k[l], self.pool.v[l], page_table, seq_lens, bs, K, draft, base_add,
-                           cfg.n_q_heads, cfg.n_kv_heads, self.page_size, attn_chunk, attn_splits, self.attn, ws_attn,
-                           status=st, order=order)
+            if self.kv8:
+                self._qkv_attention_8bit(l, d, bs, K, seq_lens, page_table, attn_chunk, attn_splits, st, ws_attn, draft,
+                                         base_add, rope_pos3)
+            else:
+                e = L.Epilogue()
+                e.mode = L.EPI_QKV_ROPE
+                e.q_out = self.q.data_ptr()
+                e.k_cache = self.pool.k[l].data_ptr()
+                e.v_cache = self.pool.v[l].data_ptr()
+                e.row_pos = self.row_pos.data_ptr()
+                e.row_slot = self.row_slot.data_ptr()
+                e.inv_freq = w.inv_freq.data_ptr()
+                e.rotary_dim = cfg.rotary_dim
+                if rope_pos3 is not None:
+                    e.row_pos3 = rope_pos3.data_ptr()
+                    for i in range(3):
+                        e.mrope_section[i] = cfg.mrope_section[i]
+                e.n_q_heads = cfg.n_q_heads
+                e.n_kv_heads = cfg.n_kv_heads
+                e.page_size = self.page_size
+                ops.linear(d["qkv"], self.x, M, e, self.lin_ws, prefetch=d["o"], status=st)
+                ops.bd_attention(self.q, self.pool.k[l], self.pool.v[l], page_table, seq_lens, bs, K, draft, base_add,
+                               cfg.n_q_heads, cfg.n_kv_heads, self.page_size, attn_chunk, attn_splits, self.attn, ws_attn,
+                               status=st, order=order)
             e = L.Epilogue()
             e.mode = L.EPI_PARTIAL_F32
             e.out = self.y.data_ptr()
@@ -322,6 +352,23 @@ class Engine:
         e.out_gap = 0 if out_gap is None else out_gap.data_ptr()
         ops.linear(w.lm_head, self.x, M, e, self.lin_ws, status=st)
 
+    def _qkv_attention_8bit(self, l, d, bs, K, seq_lens, page_table, attn_chunk, attn_splits, st, ws_attn, draft, base_add,
+                            rope_pos3) -> None:
+        """Layer l's projection, rotation with the quantised cache write, and attention over the 8-bit cache."""
+        cfg, M = self.cfg, bs * K
+        e = L.Epilogue()
+        e.mode = L.EPI_STORE_BF16
+        e.out = self.qkv.data_ptr()
+        e.ld_out = cfg.qkv_dim
+        L.linear(d["qkv"], self.x, M, e, self.lin_ws, prefetch=d["o"], status=st)
+        mm = rope_pos3 is not None
+        L.qk_norm_rope_write(self.qkv[:M], cfg.n_q_heads, self.kv[l], self.row_slot[:M], self.q[:M], self.w.inv_freq,
+                             cfg.rotary_dim, row_pos=None if mm else self.row_pos[:M],
+                             row_pos3=rope_pos3[:M] if mm else None, mrope_section=cfg.mrope_section if mm else None,
+                             status=st)
+        L.kv8_attention(self.q, self.kv[l], page_table, seq_lens, bs, K, draft, base_add, cfg.n_q_heads, attn_chunk,
+                        attn_splits, self.attn, ws_attn, status=st)
+
     def final_hidden(self) -> torch.Tensor:
         """Normed input of lm_head of the last forward (bf16 [max_rows, H]); for logits checks in tests."""
         return self.x
@@ -335,7 +382,7 @@ class Engine:
         dev = self.device
         pool_size = pool_size or bs
         ml = max_len or pages_per_req * self.page_size
-        chunk, splits = attention_split(bs, K, ml, avg_len or ml, self.cfg.n_kv_heads, self.sms)
+        chunk, splits = self.attention_plan(bs, K, ml, avg_len or ml)
         i32 = dict(dtype=torch.int32, device=dev)
         i64 = dict(dtype=torch.int64, device=dev)
         f32 = dict(dtype=torch.float32, device=dev)
@@ -408,7 +455,7 @@ class Engine:
                         pos3[i, : s1 - s0] = prefix_pos3[b][:, s0:s1].T.to(torch.int32)
                 pos3 = pos3.view(nb * chunk, 3).to(dev)
             ml = (c + 1) * chunk
-            ach, asp = attention_split(nb, chunk, ml, ml, self.cfg.n_kv_heads, self.sms)
+            ach, asp = self.attention_plan(nb, chunk, ml, ml)
             if attn_chunk:
                 ach, asp = attn_chunk, int(math.ceil(ml / attn_chunk))
             self.forward(L.ROWS_EXPLICIT, nb, chunk, seq, pt, out_idx=out_idx, ids64=ids, row_embeds=rows_e,
@@ -482,8 +529,8 @@ class Engine:
 
     def kernels_per_forward(self, rows: int = 0) -> int:
         """Kernel launches of one forward of `rows` rows: embed + per layer (4 projections, attention, 2 residual
-        norms) + lm_head (projection + per-token argmax reduction)."""
-        return 3 + 7 * self.cfg.n_layers
+        norms; with an 8-bit cache the write) + lm_head (projection + per-token argmax reduction)."""
+        return 3 + (8 if self.kv8 else 7) * self.cfg.n_layers
 
     def capture(self, rb: RoundBuffers, override: bool = False, warmup: int = 0) -> torch.cuda.CUDAGraph:
         """Capture one round (both forwards and the commit) into a CUDA graph; replays read the device-resident
