@@ -138,10 +138,6 @@ __device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
-// 1.5 * 2^23 + x as a float, |x| < 2^22: an integer becomes a float by an addition.  (The conversion unit, 8 cycles a warp,
-// already has the weights' exponentials and the joining of O.)
-constexpr float kIntBias = 12582912.f;
-__device__ __forceinline__ float int_biased(uint32_t x) { return __uint_as_float(x + 0x4B400000u); }
 __device__ __forceinline__ float warp_max(float v) {
   float r;
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));  // NaNs are ignored
@@ -220,18 +216,11 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
     tma_prefetch_desc(&tmk);
     tma_prefetch_desc(&tmv);
   }
-  // TMEM is taken before the dependent launch is released: a CTA of a later kernel (which may wait for this grid) can
-  // then never hold the columns this CTA is waiting for
-  if (warp == kMmaWarp) tmem_alloc(tmem_slot, Sh::tmem_cols);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  if (tid == 0) pdl_trigger();
   pdl_wait();
 
-  const int split = blockIdx.x, b = blockIdx.z;
-  const int kvh = blockIdx.y / p.row_blocks, blk = blockIdx.y - kvh * p.row_blocks;
+  // x = K/V head and row block, y = request, z = split: the splits that only the longest requests have launch last
+  const int split = blockIdx.z, b = blockIdx.y;
+  const int kvh = blockIdx.x / p.row_blocks, blk = blockIdx.x - kvh * p.row_blocks;
   const int G = p.n_q_heads / p.n_kv_heads;
   const int R_all = G * p.K;
   const int r0 = blk * p.rows_per_block;
@@ -243,10 +232,18 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
   const int base = static_cast<int>(min(max(base64, static_cast<int64_t>(-p.K)), cap));
   const int L = static_cast<int>(min(max(end64, static_cast<int64_t>(0)), cap));  // the last row's limit
   const int n_active = min(p.max_splits, max(1, (L + p.chunk - 1) / p.chunk));
-  const bool active = split < n_active;  // uniform over the CTA
+  if (split >= n_active) return;
+  // TMEM is taken before the dependent launch is released: a CTA of a later kernel (which may wait for this grid) can
+  // then never hold the columns this CTA is waiting for
+  if (warp == kMmaWarp) tmem_alloc(tmem_slot, Sh::tmem_cols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (tid == 0) pdl_trigger();
   const int kv_beg = split * p.chunk;
   const int kv_end = min(L, kv_beg + p.chunk);
-  const int n_tiles = active && kv_end > kv_beg ? (kv_end - kv_beg + kQTile - 1) / kQTile : 0;
+  const int n_tiles = kv_end > kv_beg ? (kv_end - kv_beg + kQTile - 1) / kQTile : 0;
   const int64_t slot0 = (static_cast<int64_t>(b) * p.n_kv_heads + kvh) * p.max_splits;
 
   // ---- first code row of each of the chunk's pages; page ids are checked here
@@ -260,7 +257,7 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
     }
     pages[k] = (id * p.n_kv_heads + kvh) * 16;
   }
-  if (active && warp < kMmaWarp) {
+  if (warp < kMmaWarp) {
     // ---- query rows to shared memory, in parts: a warp per row, each step for all of a warp's rows (their latencies overlap)
     float* coef = reinterpret_cast<float*>(smem + Sh::coef);
     int* lim = reinterpret_cast<int*>(smem + Sh::lim);
@@ -399,7 +396,7 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
       __syncwarp();
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (active) {
+  } else {
     // ---- one thread per token (weights), then per dimension (output), for the rows of its group
     const int t128 = tid & 127, grp = H == 1 ? 0 : warp >> 2, rb = grp * RH;
     const float* coef = reinterpret_cast<const float*>(smem + Sh::coef) + rb;
@@ -440,8 +437,7 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
           if (FMT == GR_KV_E4M3) {
             x = fmaf(__uint_as_float(s[RH + r]), 1.f / 16, __uint_as_float(s[r]));
           } else {
-            // hi * 256 + lo by additions: 1.5 * 2^23 + x is a float's bits, and the biases (multiples of 256) leave exactly
-            x = fmaf(int_biased(s[r]), 256.f, -kIntBias * 257.f) + int_biased(s[RH + r]);
+            x = static_cast<float>(static_cast<int>(s[r]) * 256 + static_cast<int>(s[RH + r]));
           }
           w[r] = x;
         }
@@ -610,7 +606,7 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
     tc_fence_after();
     tmem_dealloc(tmem, Sh::tmem_cols);
   }
-  if (!active || n_active == 1) return;
+  if (n_active == 1) return;
 
   // ---- the last split to arrive joins them, in split order
   __threadfence();
@@ -745,7 +741,7 @@ static cudaError_t launch_kv8_attention_t(const CUtensorMap& tmk, const CUtensor
   });
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.max_splits, p.n_kv_heads * p.row_blocks, p.bs);
+  cfg.gridDim = dim3(p.n_kv_heads * p.row_blocks, p.bs, p.max_splits);
   cfg.blockDim = dim3(Sh::threads);
   cfg.dynamicSmemBytes = Sh::bytes;
   cfg.stream = stream;

@@ -908,14 +908,17 @@ int gr_kv8_attention_plan(int bs, int K, int max_len, int n_q_heads, int n_kv_he
   if (!out || bs <= 0 || K <= 0 || max_len <= 0 || max_len > kKv8MaxChunk * kKv8MaxSplits || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads)
     return GR_ERR_ARG;
   // the (request, head, row block) triples times the splits of the longest request make about one wave of two CTAs an SM
-  // (131,071 tokens of one request: 37 splits 50 us, 55 splits 54 us); many requests of mixed lengths go in even pieces of
-  // at most 1,536 tokens (64 requests of 288-4,128 tokens: 52 us, against 54 at 1,024 and 56 uncut)
+  // (131,071 tokens of one request: 37 splits 52 us, 55 splits 55 us); many requests of mixed lengths go in even pieces.
+  // A CTA of more than 16 rows pays about five tiles' time for its queries and its part of the join, so its pieces are
+  // longer (64 requests of 288-4,128 tokens, one row: 56 us at 1,536 tokens, 61 at 1,024; 17 rows: 116 us at 3,200, 135
+  // at 1,536).
   int blocks, per_block;
   kv8_attention_blocks(n_q_heads / n_kv_heads * K, &blocks, &per_block);
   const int64_t units = static_cast<int64_t>(bs) * n_kv_heads * blocks;
   const int64_t per = std::max<int64_t>(1, 2LL * num_sms() / units);
+  const int64_t piece = per_block > 16 ? 3200 : 1536;
   int64_t chunk = (static_cast<int64_t>(max_len) + per - 1) / per;
-  if (chunk > 1536 && units >= num_sms()) chunk = 1536;
+  if (chunk > piece && units >= num_sms()) chunk = piece;
   const int64_t least = (static_cast<int64_t>(max_len) + kKv8MaxSplits - 1) / kKv8MaxSplits;
   if (chunk < least) chunk = least;
   if (chunk < 128) chunk = 128;
