@@ -14,7 +14,8 @@
 namespace gr {
 
 constexpr int kWriteThreads = 128;
-constexpr int kReadThreads = 256;
+constexpr int kReadThreads = 128;
+constexpr int kReadItems = 4;
 
 __device__ __forceinline__ void unpack8(const uint4& raw, float (&x)[8]) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -140,7 +141,7 @@ __device__ __forceinline__ void put_row(const T (&y)[8], int l16, bool store, ui
 }
 
 template <int FMT, bool HALF>
-__global__ void __launch_bounds__(kWriteThreads, 6) qk_norm_rope_write_kernel(const KvWriteParams p) {
+__global__ void __launch_bounds__(kWriteThreads, 7) qk_norm_rope_write_kernel(const KvWriteParams p) {
   __shared__ double2 s_cs64[FMT != GR_KV_BF16 ? kWriteThreads / 32 : 1][64];
   __shared__ float2 s_cs32[kWriteThreads / 32][64];
   if (threadIdx.x == 0) pdl_trigger();
@@ -168,9 +169,8 @@ __global__ void __launch_bounds__(kWriteThreads, 6) qk_norm_rope_write_kernel(co
     return p.n_q_heads + p.n_kv_heads + min(2 * (i - n_kp) + sub, p.n_kv_heads - 1);
   };
   auto load = [&](int i) { return __ldg(reinterpret_cast<const uint4*>(in + (even ? 2 * i + sub : head_of(i)) * 128)); };
-  uint4 next = make_uint4(0, 0, 0, 0), next2 = next;
+  uint4 next = make_uint4(0, 0, 0, 0);
   if (g < n_pairs) next = load(g);
-  if (g + p.groups < n_pairs) next2 = load(g + p.groups);
 
   double2* cs64 = s_cs64[FMT != GR_KV_BF16 ? threadIdx.x >> 5 : 0];
   float2* cs32 = s_cs32[threadIdx.x >> 5];
@@ -207,8 +207,7 @@ __global__ void __launch_bounds__(kWriteThreads, 6) qk_norm_rope_write_kernel(co
   for (int i = g; i < n_pairs; i += p.groups) {
     float x[8];
     unpack8(next, x);
-    next = next2;
-    if (i + 2 * p.groups < n_pairs) next2 = load(i + 2 * p.groups);
+    if (i + p.groups < n_pairs) next = load(i + p.groups);
     if (i < n_qp) {
       const int h = 2 * i + sub;
       float y[8];
@@ -239,50 +238,63 @@ __global__ void __launch_bounds__(kWriteThreads, 6) qk_norm_rope_write_kernel(co
   }
 }
 
-// Sixteen elements per item: item = ((row * 2 + K or V) * heads + head) * 8 + eighth of the head.
+// A warp reads one row's K or V; a lane takes 8 elements (a warp's stores cover whole lines) of kReadItems pairs of heads at a
+// time, every load before the first store.
 template <int FMT>
 __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const KvReadParams p) {
   if (threadIdx.x == 0) pdl_trigger();
   pdl_wait();
-  const int per_row = 16 * p.n_kv_heads;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * kReadThreads + threadIdx.x;
-  const int64_t row = item / per_row;
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kReadThreads / 32) + (threadIdx.x >> 5);
+  const int64_t row = unit >> 1;
   if (row >= p.n) return;
-  const int rest = static_cast<int>(item - row * per_row);
-  const int which = rest / (8 * p.n_kv_heads);
-  const int hc = rest - which * 8 * p.n_kv_heads;  // head * 8 + eighth
-  const int64_t slot = p.slots[row];
-  if (slot < 0) return;
-  if (slot >= p.n_slots) {
-    report(p.status, GR_ERR_BAD_PAGE);
-    return;
-  }
-  const int64_t r = ((slot >> 4) * p.n_kv_heads + (hc >> 3)) * 16 + (slot & 15);
-  uint4* dst = reinterpret_cast<uint4*>((which ? p.v_out : p.k_out) + row * p.n_kv_heads * 128 + hc * 16);
-  if (FMT == GR_KV_BF16) {
-    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(which ? p.v : p.k) + r * 128 +
-                                                      (hc & 7) * 16);
-    const uint4 a = __ldg(src), b = __ldg(src + 1);
-    dst[0] = a;
-    dst[1] = b;
-    return;
-  }
-  const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(which ? p.v : p.k) + r * 128 +
-                                                    (hc & 7) * 16);
-  const float f = kv_scale((which ? p.v_exp : p.k_exp)[r]);
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  uint32_t o[8];
+  const bool v = unit & 1;
+  const int64_t slot = __ldg(p.slots + row);
+  if (slot >= p.n_slots && lane == 0) report(p.status, GR_ERR_BAD_PAGE);
+  if (slot < 0 || slot >= p.n_slots) return;
+  const int64_t row0 = (slot >> 4) * p.n_kv_heads * 16 + (slot & 15);  // cache row of head 0
+  const uint8_t* codes = static_cast<const uint8_t*>(v ? p.v : p.k);
+  const int8_t* exps = v ? p.v_exp : p.k_exp;
+  __nv_bfloat16* out = (v ? p.v_out : p.k_out) + row * p.n_kv_heads * 128 + (lane & 15) * 8;
+  for (int h0 = lane >> 4; h0 < p.n_kv_heads; h0 += 2 * kReadItems) {
+    uint4 raw[kReadItems];
+    int e[kReadItems];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t a, b;
-    kv_unpack<FMT>(w[i], a, b);
-    const float2 fa = __half22float2(*reinterpret_cast<__half2*>(&a));
-    const float2 fb = __half22float2(*reinterpret_cast<__half2*>(&b));
-    o[2 * i] = pack_bf16(fa.x * f, fa.y * f);
-    o[2 * i + 1] = pack_bf16(fb.x * f, fb.y * f);
+    for (int u = 0; u < kReadItems; ++u) {
+      const int h = h0 + 2 * u;
+      if (h >= p.n_kv_heads) break;
+      const int64_t at = (row0 + h * 16) * 128 + (lane & 15) * 8;
+      if (FMT == GR_KV_BF16) {
+        raw[u] = __ldg(reinterpret_cast<const uint4*>(codes + at * 2));
+      } else {
+        const uint2 c = __ldg(reinterpret_cast<const uint2*>(codes + at));
+        raw[u].x = c.x;
+        raw[u].y = c.y;
+        e[u] = __ldg(exps + row0 + h * 16);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kReadItems; ++u) {
+      const int h = h0 + 2 * u;
+      if (h >= p.n_kv_heads) break;
+      if (FMT != GR_KV_BF16) {
+        const float f = kv_scale(e[u]);
+        const uint32_t w[2] = {raw[u].x, raw[u].y};
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t a, b;
+          kv_unpack<FMT>(w[i], a, b);
+          const float2 fa = __half22float2(*reinterpret_cast<__half2*>(&a));
+          const float2 fb = __half22float2(*reinterpret_cast<__half2*>(&b));
+          o[2 * i] = pack_bf16(fa.x * f, fa.y * f);
+          o[2 * i + 1] = pack_bf16(fb.x * f, fb.y * f);
+        }
+        raw[u] = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+      *reinterpret_cast<uint4*>(out + h * 128) = raw[u];
+    }
   }
-  dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
 cudaError_t launch_qk_norm_rope_write(KvWriteParams p, int format, bool half, cudaStream_t s, bool pdl) {
@@ -305,8 +317,7 @@ cudaError_t launch_qk_norm_rope_write(KvWriteParams p, int format, bool half, cu
 }
 
 cudaError_t launch_kv_read(const KvReadParams& p, int format, cudaStream_t s, bool pdl) {
-  const int64_t items = p.n * 16 * p.n_kv_heads;
-  const dim3 grid(static_cast<unsigned>((items + kReadThreads - 1) / kReadThreads));
+  const dim3 grid(static_cast<unsigned>((2 * p.n + kReadThreads / 32 - 1) / (kReadThreads / 32)));
   switch (format) {
     case GR_KV_E4M3: return launch_dependent(kv_read_kernel<GR_KV_E4M3>, grid, kReadThreads, 0, s, pdl, p);
     case GR_KV_INT8: return launch_dependent(kv_read_kernel<GR_KV_INT8>, grid, kReadThreads, 0, s, pdl, p);
