@@ -17,12 +17,13 @@
 // reading every such thread's logits again cost 20% more DRAM traffic.)
 // Bound: reading the row.  Few rows are shared between the CTAs of a cluster, whose states, counts and best lists the first
 // one joins through distributed shared memory.
+#include <type_traits>
+
 #include "params.cuh"
 
 namespace gr {
 
-constexpr int kLpThreadsFew = 512;        // where the CTAs of a cluster share a row
-constexpr int kLpThreadsMany = 256;       // a CTA a row: four an SM, so one's selection overlaps the others' reading
+constexpr int kLpMaxThreads = 512;
 constexpr int kLpGroups = 64;             // groups of threads whose bests bound the n-th best; n <= kLpGroups
 constexpr int kLpCand = 1024;             // candidates kept at once
 constexpr uint32_t kLpAhead = 48 << 10;   // bytes of a later row fetched to L2 while this one is finished
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const Log
     }
   }
   if (ends && tail + tid < p.vocab) lp_one(t, V::one(base + tail + tid), tail + tid, k, mine, my_id);
-  if (NT == kLpThreadsMany && tid == 0 && row + p.ahead < p.rows) {
+  if (NT < kLpMaxThreads && tid == 0 && row + p.ahead < p.rows) {
     // CTAs that started together reach their selection together: meanwhile the row that will follow on this SM comes to L2
     const T* after = base + p.ahead * p.ld;
     const uintptr_t from = (reinterpret_cast<uintptr_t>(after) + 15) & ~uintptr_t(15);
@@ -390,8 +391,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const Log
   }
   if (n > 0 && v_beg + tid < v_end && (static_cast<uint64_t>(my_best) << 32 | 0xffffffffu) >= bound) {
     const int cells = min(kLpCells, (v_end - v_beg - tid + V::B * NT - 1) / (V::B * NT));
-    for (int c = 0; c < cells; ++c)
-      if ((static_cast<uint64_t>(lp_order(s_cell[c][tid])) << 32 | 0xffffffffu) >= bound) {
+#pragma unroll
+    for (int c = 0; c < kLpCells; ++c)
+      if (c < cells && (static_cast<uint64_t>(lp_order(s_cell[c][tid])) << 32 | 0xffffffffu) >= bound) {
         const int at = atomicAdd(&s_n_hot, 1);
         if (at < kLpHot) s_hot[at] = static_cast<uint16_t>(c * NT + tid);
       }
@@ -520,7 +522,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const Log
   if (ctas == 1) {
     if (tid < n) put_top(tid, s_top[tid]);
   } else {
-    const int total = n * static_cast<int>(ctas);  // at most kLpGroups * kLpMaxCluster = kLpThreadsFew keys
+    const int total = n * static_cast<int>(ctas);  // at most kLpGroups * kLpMaxCluster keys, where ctas > 1 comes with as many threads
     const uint64_t key = tid < total ? lp_peer_u64(&s_top[tid % n], tid / n) : 0;
     __syncwarp();
     lp_cluster_sync();
@@ -552,16 +554,21 @@ static cudaError_t launch_token_logprobs_t(const LogprobParams& p, int ctas, cud
   return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NT>, p);
 }
 
+// 1,024 threads an SM, in CTAs of 512, 256 or 128, a CTA a row: as many rows in flight as there are, since a row's
+// selection (about 6 us) leaves the memory to the other rows' reading.  1,088 rows of 59,392 fp32 logits: 52 us in CTAs of
+// 128 (one wave), 57 in CTAs of 256 (two); 600 rows: 46 / 44; 150 rows: 23 / 17.  Fewer rows than SMs are shared by clusters.
 cudaError_t launch_token_logprobs(LogprobParams p, bool bf16, cudaStream_t stream, bool pdl) {
-  // CTAs a row: as many as keep the launch within two CTAs an SM
+  auto go = [&](auto nt, int ctas) {
+    constexpr int NT = decltype(nt)::value;
+    p.ahead = 1024 / NT * p.sms;
+    return bf16 ? launch_token_logprobs_t<__nv_bfloat16, NT>(p, ctas, stream, pdl)
+                : launch_token_logprobs_t<float, NT>(p, ctas, stream, pdl);
+  };
+  if (p.rows > 4 * p.sms) return go(std::integral_constant<int, 128>(), 1);
+  if (p.rows > 2 * p.sms) return go(std::integral_constant<int, 256>(), 1);
   int ctas = 1;
   while (ctas < kLpMaxCluster && static_cast<int64_t>(p.rows) * ctas <= p.sms) ctas *= 2;
-  if (ctas > 1)
-    return bf16 ? launch_token_logprobs_t<__nv_bfloat16, kLpThreadsFew>(p, ctas, stream, pdl)
-                : launch_token_logprobs_t<float, kLpThreadsFew>(p, ctas, stream, pdl);
-  p.ahead = 4 * p.sms;
-  return bf16 ? launch_token_logprobs_t<__nv_bfloat16, kLpThreadsMany>(p, 1, stream, pdl)
-              : launch_token_logprobs_t<float, kLpThreadsMany>(p, 1, stream, pdl);
+  return go(std::integral_constant<int, kLpMaxThreads>(), ctas);
 }
 
 }  // namespace gr
