@@ -391,7 +391,6 @@ def kv_cache(k: torch.Tensor, v: torch.Tensor, k_exp: Optional[torch.Tensor] = N
     c.k, c.v, c.k_exp, c.v_exp = _ptr(k), _ptr(v), _ptr(k_exp), _ptr(v_exp)
     c.tensors = (k, v, k_exp, v_exp)
     c.device = k.get_device()
-    c.ref = ctypes.byref(c)
     return c
 
 
@@ -411,7 +410,7 @@ def qk_norm_rope_write(qkv: torch.Tensor, n_q_heads: int, cache: KvCache, row_sl
     if qkv.get_device() != dev:
         raise RuntimeError(f"qkv is on {qkv.device}, the cache on cuda:{dev}")
     rc = _call(dev, stream, load().gr_qk_norm_rope_write, qkv.data_ptr(), qkv.stride(0) if m > 1 else width, m, n_q_heads,
-               cache.ref,
+               ctypes.byref(cache),
                None if q_norm is None else _arg(q_norm, torch.bfloat16, dev, 128, "q_norm"),
                None if k_norm is None else _arg(k_norm, torch.bfloat16, dev, 128, "k_norm"), eps,
                None if row_pos is None else _arg(row_pos, torch.int32, dev, m, "row_pos"),
@@ -430,7 +429,7 @@ def kv_read(cache: KvCache, slots: torch.Tensor, k_out: torch.Tensor, v_out: tor
     """Cache rows at ``slots`` (int64 [n]) back in bf16: k_out / v_out [n, kv_heads * 128] (gr_kv_read)."""
     dev, n = cache.device, slots.numel()
     out = n * cache.n_kv_heads * 128
-    rc = _call(dev, stream, load().gr_kv_read, cache.ref, _arg(slots, torch.int64, dev, n, "slots"), n,
+    rc = _call(dev, stream, load().gr_kv_read, ctypes.byref(cache), _arg(slots, torch.int64, dev, n, "slots"), n,
                _arg(k_out, torch.bfloat16, dev, out, "k_out"), _arg(v_out, torch.bfloat16, dev, out, "v_out"),
                None if status is None else _arg_least(status, torch.int32, dev, 1, "status"))
     if rc:
@@ -461,7 +460,8 @@ def kv8_attention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, seq
     else:
         ws_bytes = workspace.numel() * workspace.element_size()
         ws = _arg_least(workspace, workspace.dtype, dev, 0, "workspace")
-    rc = _call(dev, stream, load().gr_kv8_attention, _arg_least(q, torch.bfloat16, dev, n, "q"), cache.ref,
+    rc = _call(dev, stream, load().gr_kv8_attention, _arg_least(q, torch.bfloat16, dev, n, "q"),
+               ctypes.byref(cache),
                _arg_least(page_table, torch.int32, dev, bs * pages, "page_table"), pages,
                _arg_least(seq_lens, torch.int64, dev, bs, "seq_lens"), bs, K, int(draft), base_add, n_q_heads, chunk,
                max_splits, _arg_least(out, torch.bfloat16, dev, n, "out"), ws, ws_bytes,

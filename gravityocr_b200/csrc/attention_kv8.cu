@@ -143,6 +143,11 @@ __device__ __forceinline__ float warp_max(float v) {
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));  // NaNs are ignored
   return r;
 }
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ void named_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -228,7 +233,10 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
   const int64_t base64 = p.seq_lens[b] + p.base_add;
   const int64_t cap = static_cast<int64_t>(p.pt_stride) * 16;
   const int64_t end64 = base64 + p.K;
-  if (end64 > cap && tid == 0 && split == 0) report(p.status, GR_ERR_BAD_PAGE);
+  if (tid == 0 && split == 0) {
+    if (end64 > cap) report(p.status, GR_ERR_BAD_PAGE);
+    else if (end64 > static_cast<int64_t>(p.chunk) * p.max_splits) report(p.status, GR_ERR_ARG);
+  }
   const int base = static_cast<int>(min(max(base64, static_cast<int64_t>(-p.K)), cap));
   const int L = static_cast<int>(min(max(end64, static_cast<int64_t>(0)), cap));  // the last row's limit
   const int n_active = min(p.max_splits, max(1, (L + p.chunk - 1) / p.chunk));
@@ -496,6 +504,10 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
         const float4 bt = *reinterpret_cast<const float4*>(betas + rb + r);
         float x[4] = {ex2_approx(w[r] + rf.x), ex2_approx(w[r + 1] + rf.y), ex2_approx(w[r + 2] + rf.z),
                       ex2_approx(w[r + 3] + rf.w)};
+        if (FMT == GR_KV_INT8) {  // the largest weight's exponent is rounded: past 32639 the digits would wrap
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[k] = min_nan(x[k], 32639.f);
+        }
         // a hidden token's exponent may be that of a bad row, or of no row: its weight is 0, and 2^-ev is finite
         l[r] = fmaf(x[0] * unv, bt.x, l[r]);
         l[r + 1] = fmaf(x[1] * unv, bt.y, l[r + 1]);

@@ -313,7 +313,7 @@ int gr_kv_read(const gr_kv_cache* cache, const int64_t* slots, int64_t n, void* 
 /* gr_bd_attention over an 8-bit cache (GR_KV_BF16 is GR_ERR_UNSUPPORTED: gr_bd_attention reads that): the same rows, masks
  * (draft 0, 1, 2) and page tables.  K = 1 is one decode token.  A row that sees nothing (seq_lens[b] + base_add + j < 0: a
  * padding request has seq_lens -K - base_add) gives zeros.  Lengths past the page table, and page ids past the cache, set
- * GR_ERR_BAD_PAGE.  chunk: a multiple of 32, at most 8192; max_splits <= 128;
+ * GR_ERR_BAD_PAGE; lengths past chunk * max_splits set GR_ERR_ARG (the rest is not seen).  chunk: a multiple of 32, at most 8192; max_splits <= 128;
  * chunk * max_splits >= the longest length + K.
  * workspace: gr_kv8_attention_workspace_bytes, zero-filled once (needed for max_splits > 1), one call at a time. */
 size_t gr_kv8_attention_workspace_bytes(int bs, int K, int n_q_heads, int n_kv_heads, int max_splits);

@@ -416,6 +416,38 @@ def test_attention_rows_that_see_nothing():
     assert (_attend(_attn_case("e4m3", [-1], 1, 16, 8), chunk=32) == 0).all()
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("K", [1, 17])
+def test_attention_huge_scores(fmt, K):
+    """Scores of tens of thousands (base 2), where a score's fp32 step is a good part of a percent of a weight: the largest
+    weight of a tile must not wrap, and each row still attends to its largest scores alone."""
+    c = _attn_case(fmt, [700, 130], K, 16, 8, spread=0.0)
+    c["q"] = (c["q"].float() * 4000).bfloat16()
+    out = _attend(c).double().cpu().view(2, K, 16, 128)
+    for b in range(2):
+        q = c["q"][b * K: (b + 1) * K].double().view(K, 16, 128)
+        k, v = c["k"][c["slots"][b]], c["v"][c["slots"][b]]
+        s = torch.einsum("jhd,thd->jht", q, k.repeat_interleave(2, 1)) / math.sqrt(128) * 1.4427
+        lim = torch.tensor(R.row_limits(0, c["lens"][b], K))
+        s[(torch.arange(k.shape[0])[None] >= lim[:, None])[:, None].expand(s.shape)] = -math.inf
+        top = torch.topk(s, 2, -1)
+        sure = top.values[..., 0] - top.values[..., 1] > 64    # all the weight on one token, whatever the rounding
+        assert sure.float().mean() > 0.5  # of the inputs, not of the kernel: most rows have a clear winner
+        want = v.repeat_interleave(2, 1).transpose(0, 1)[torch.arange(16)[None], top.indices[..., 0]]
+        err = (out[b] - want).abs()[sure]
+        assert (err <= BF16 * want.abs()[sure] + 2.0 ** -14 * want.abs().amax(-1, keepdim=True).expand(want.shape)[sure]).all()
+
+
+def test_attention_reports_a_plan_that_is_too_short():
+    c = _attn_case("int8", [100, 20], 1, 16, 8)
+    st = _status()
+    _attend(c, chunk=64, splits=1, status=st)
+    assert int(st) == 1
+    st.zero_()
+    _attend(c, chunk=64, splits=2, status=st)
+    assert int(st) == 0
+
+
 def test_attention_reports_bad_pages():
     c = _attn_case("int8", [100, 30], 1, 16, 8)
     st = _status()
@@ -533,6 +565,34 @@ def test_decode_steps_write_then_attend(fmt):
                 _check_attention(dict(c, q=q[b: b + 1].cpu(), k=k, v=v, slots=[torch.arange(k.shape[0])],
                                       lens=[k.shape[0] - 1]), out[b: b + 1])
     assert int(st) == 0
+
+
+def test_a_dropped_handle_frees_the_cache():
+    import gc
+    gc.collect()
+    gc.disable()
+    try:
+        before = torch.cuda.memory_allocated()
+        L.kv_cache(*_cache(64, 8, "int8"))
+        assert torch.cuda.memory_allocated() == before
+    finally:
+        gc.enable()
+
+
+def test_calls_on_two_streams_at_once():
+    """Two requests' attention with a workspace each, on two streams, many times over: the same rows as one after the other."""
+    a, b = _attn_case("int8", [3000], 1, 16, 8), _attn_case("e4m3", [2500], 1, 16, 8, seed=4)
+    want = [_attend(c, chunk=256) for c in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, c in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(_attend(c, chunk=256))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(x, w) for x in g)
 
 
 def test_wrappers_refuse():
