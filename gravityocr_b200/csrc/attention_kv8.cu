@@ -140,7 +140,8 @@ __device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[N]) {
 }
 __device__ __forceinline__ float warp_max(float v) {
   float r;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));  // NaNs are ignored
+  // NaNs are ignored; volatile: every lane has to take part, wherever the result is used
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
 __device__ __forceinline__ float min_nan(float a, float b) {

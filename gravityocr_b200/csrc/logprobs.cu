@@ -59,7 +59,8 @@ __device__ __forceinline__ LpState lp_join(const LpState& a, const LpState& b, f
 }
 __device__ __forceinline__ float lp_warp_max(float v) {
   float r;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));  // NaNs are ignored
+  // NaNs are ignored; volatile: every lane has to take part, wherever the result is used
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
