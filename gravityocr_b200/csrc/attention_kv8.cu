@@ -20,18 +20,24 @@
 //   w = s * coef_r * 2^ek + ev (base 2),  p = 2^(w - M_r),  O = sum p code_v,  l = sum p 2^-ev,  out = O / l.
 // |ev| <= 40 keeps l: a token whose p underflows has a score 46 binades below the best.
 //
-//
 // P is measured from its own tile's maximum T_r, not the running one: its parts then resolve the tile's weights whatever the
 // rest of the sequence holds (a first token that takes most of the attention would otherwise push every later weight
 // below int8's two digits), and O and l take a tile in fp32 with the factor 2^(T_r - M_r).  M_r is the first tile's maximum,
 // raised only where a tile's is 2^64 above it: fp32 holds the rest, and the sums are hardly ever rescaled.
 //
-// CTA: (split, K/V head and block of at most 40 rows, request).  One thread per token (then per dimension) and row group: up
-// to 16 rows four warps take all of them, above that eight warps take half the rows each.  One warp issues the MMAs, one the
-// TMA copies (8 pages a 128-token tile, 2 KB of K and 2 KB of V each; ~85 cycles an issue, which on the MMA warp would sit
-// between a tile's two products).  Per tile: S -> weights -> P to shared memory -> O -> registers.  K and V have rings of
-// their own, so a tile's K half is refilled as soon as its scores exist, and the two or three CTAs of an SM cover each
-// other's latencies.
+// CTA: (split, K/V head and block of at most 40 rows, request).  A thread per token (then per dimension) and row group: one
+// group of four warps, or two that share the rows (launch_kv8_attention_f).  One warp issues the MMAs, one the TMA copies (8
+// pages a 128-token tile, 2 KB of K and 2 KB of V each; ~85 cycles an issue, which on the MMA warp would sit between a
+// tile's two products).  Per tile: S -> weights -> P to shared memory -> O -> registers.  K and V have rings of their own,
+// so a tile's K half is refilled as soon as its scores exist, and the two or three CTAs of an SM cover each other's
+// latencies.
+//
+// Measured (8 K/V heads of 2 query heads).  One row: 131,071 tokens of one request 50 us, 283 MB, 5.6 TB/s, where a plain
+// sum of as many bytes takes 49.5; 64 requests of 288-4,128 tokens 53 us (291 MB): bound by the memory.  17 rows of these 64:
+// 99 us int8, 115 e4m3, bound by the softmax threads: their instructions fill half of the issue slots, and a tile's chain
+// (scores, maxima, weights, P, O) the time between.
+#include <type_traits>
+
 #include "kv8_dev.cuh"
 
 namespace gr {
@@ -43,25 +49,24 @@ constexpr int kQExpStages = 4;                              // tiles' exponents
 constexpr int kQMaxRows = 40;                               // rows of a CTA
 constexpr size_t kQTicketBytes = kKv8TicketPairs * sizeof(int);
 
-// RT rows in H groups of RH.  Columns: S has part k of row r at group * 2 * RH + k * RH + r (within its group), P
-// likewise with every group padded to 16 columns.
-template <int FMT, int RT, int H>
+// H groups of RH rows, each padded to RP (a multiple of four; the padding has columns, but no arithmetic).  Columns: S has
+// part k of a group's row r at group * 2 * RP + k * RP + r, P likewise with every group padded to 16 columns.
+template <int FMT, int RH, int H>
 struct KvAttnShape {
-  static constexpr int RH = RT / H;
+  static constexpr int RP = (RH + 3) / 4 * 4, RT = RP * H;
   static constexpr int p_parts = FMT == GR_KV_E4M3 ? 3 : 2;
-  static constexpr int p_cols = (p_parts * RH + 15) / 16 * 16;
+  static constexpr int p_cols = (p_parts * RP + 15) / 16 * 16;
   static constexpr int n1 = (2 * RT + 15) / 16 * 16;
   static constexpr int n2 = p_cols * H;
   static constexpr int tmem_cols = n1 + n2 <= 32 ? 32 : (n1 + n2 <= 64 ? 64 : (n1 + n2 <= 128 ? 128 : 256));
   static constexpr int threads = 128 * H + 64;
-  static constexpr int ctas = RT > 16 ? 2 : 3;              // per SM
   // shared memory, from a 1024-aligned start
   static constexpr int k = 0;
   static constexpr int v = k + kQStages * kQHalf;
   static constexpr int q = v + kQStages * kQHalf;           // [n1][128], 128-byte swizzle
   static constexpr int p = q + n1 * 128;                    // [n2 / 16][128 tokens][16]
   static constexpr int exps = p + n2 * 128;                 // [kQExpStages][K, V][128]
-  static constexpr int xm = exps + kQExpStages * 2 * kQTile;                   // [4][RT] warp maxima of a tile; at the end, the sums l
+  static constexpr int xm = exps + kQExpStages * 2 * kQTile;  // [4][RT] warp maxima of a tile; at the end, the sums l
   static constexpr int coef = xm + RT * 16;                 // [RT] score scale
   static constexpr int ref = coef + RT * 4;                 // [RT] off - T_r
   static constexpr int alpha = ref + RT * 4;                // [RT] factor of the sums so far
@@ -70,7 +75,8 @@ struct KvAttnShape {
   static constexpr int pages = lim + RT * 4;                // [kKv8MaxChunk / 16] first code row of each page
   static constexpr int bars = (pages + kKv8MaxChunk / 4 + 15) / 16 * 16;
   static constexpr int bytes = 1024 + bars + (2 * kQStages + kQExpStages + 5) * 8 + 16;
-  static_assert(RH % 4 == 0 && n1 <= 256 && n1 + n2 <= 256, "rows are handled by fours");
+  static constexpr bool ordered = RH > 8;                   // may take requests by length
+  static_assert(n1 + n2 <= 256, "two CTAs share an SM's 512 columns");
 };
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
@@ -138,6 +144,14 @@ __device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
+// f(first row, rows) over a group's RP (padded) rows: at once up to 12, else in two parts, so that a tile's TMEM columns and
+// the thread's sums fit the registers together.
+template <int RP, typename F>
+__device__ __forceinline__ void rows_by_parts(F f) {
+  constexpr int first = RP <= 12 ? RP : (RP / 2 + 3) / 4 * 4;
+  f(std::integral_constant<int, 0>(), std::integral_constant<int, first>());
+  if constexpr (first < RP) f(std::integral_constant<int, first>(), std::integral_constant<int, RP - first>());
+}
 __device__ __forceinline__ float warp_max(float v) {
   float r;
   // NaNs are ignored; volatile: every lane has to take part, wherever the result is used
@@ -167,7 +181,7 @@ __device__ __forceinline__ uint64_t smem_desc_mn16(uint32_t addr, uint32_t block
   return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(128 >> 4) << 16) |
          (static_cast<uint64_t>(block_bytes >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
 }
-// Four scaled q values to q_parts words of four codes.
+// Four scaled q values to two words of four codes, one a part.
 template <int FMT>
 __device__ __forceinline__ void split_q(const float (&x)[4], uint32_t* part) {
   if (FMT == GR_KV_E4M3) {  // |x| < 256
@@ -192,11 +206,15 @@ __device__ __forceinline__ void split_q(const float (&x)[4], uint32_t* part) {
   }
 }
 
-template <int FMT, int RT, int H>
-__global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_kernel(
+struct Kv8Place {
+  int b, kvh, blk, r0, R, n_active;
+};
+
+template <int FMT, int RH, int H>
+__global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_kernel(
     const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const KvAttnParams p) {
-  using Sh = KvAttnShape<FMT, RT, H>;
-  constexpr int RH = Sh::RH;
+  using Sh = KvAttnShape<FMT, RH, H>;
+  constexpr int RP = Sh::RP, RT = Sh::RT;
   constexpr int kMmaWarp = 4 * H, kCopyWarp = kMmaWarp + 1, kSoft = 128 * H;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -225,10 +243,36 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
   pdl_wait();
 
   // x = K/V head and row block, y = request, z = split: the splits that only the longest requests have launch last
-  const int split = blockIdx.z, b = blockIdx.y;
+  const int split = blockIdx.z;
+  int b = blockIdx.y;
+  volatile int* request = flag + 1;
+  if (Sh::ordered && p.longest_first) {
+    // the split's requests by length: the blockIdx.y-th longest (equal ones by index), by counting
+    int* keys = reinterpret_cast<int*>(smem + Sh::pages);
+    int key = -1;
+    if (tid < p.bs) {
+      const int64_t n = max(static_cast<int64_t>(0), min(p.seq_lens[tid] + p.base_add + p.K,
+                                                         static_cast<int64_t>(kKv8MaxChunk) * kKv8MaxSplits));
+      key = static_cast<int>(n) * kKv8MaxSort + kKv8MaxSort - 1 - tid;
+    }
+    if (tid < kKv8MaxSort) keys[tid] = key;
+    // idle splits leave: fewer requests than blockIdx.y reach past the split's start
+    const int least = split == 0 ? 0 : (split * p.chunk + 1) * kKv8MaxSort;
+    if (b >= __syncthreads_count(key >= least)) return;
+    if (tid < p.bs) {
+      int before = 0;
+#pragma unroll 4
+      for (int i = 0; i < (p.bs + 3) >> 2; ++i) {
+        const int4 x = reinterpret_cast<const int4*>(keys)[i];
+        before += (x.x > key) + (x.y > key) + (x.z > key) + (x.w > key);
+      }
+      if (before == b) *request = tid;
+    }
+    __syncthreads();
+    b = *request;
+  }
   const int kvh = blockIdx.x / p.row_blocks, blk = blockIdx.x - kvh * p.row_blocks;
-  const int G = p.n_q_heads / p.n_kv_heads;
-  const int R_all = G * p.K;
+  const int G = p.group, R_all = p.group * p.K;
   const int r0 = blk * p.rows_per_block;
   const int R = min(p.rows_per_block, R_all - r0);  // this CTA's rows r0 .. r0 + R - 1
   const int64_t base64 = p.seq_lens[b] + p.base_add;
@@ -242,6 +286,20 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
   const int L = static_cast<int>(min(max(end64, static_cast<int64_t>(0)), cap));  // the last row's limit
   const int n_active = min(p.max_splits, max(1, (L + p.chunk - 1) / p.chunk));
   if (split >= n_active) return;
+  // what the code behind the tile loop needs is found again there, not held in registers through the loop
+  if (tid == 0) request[1] = n_active;
+  auto where = [&] {
+    Kv8Place w;
+    uint32_t x;
+    asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(x));
+    w.b = Sh::ordered && p.longest_first ? request[0] : static_cast<int>(blockIdx.y);
+    w.kvh = static_cast<int>(x) / p.row_blocks;
+    w.blk = static_cast<int>(x) - w.kvh * p.row_blocks;
+    w.r0 = w.blk * p.rows_per_block;
+    w.R = min(p.rows_per_block, p.group * p.K - w.r0);
+    w.n_active = request[1];
+    return w;
+  };
   // TMEM is taken before the dependent launch is released: a CTA of a later kernel (which may wait for this grid) can
   // then never hold the columns this CTA is waiting for
   if (warp == kMmaWarp) tmem_alloc(tmem_slot, Sh::tmem_cols);
@@ -253,7 +311,6 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
   const int kv_beg = split * p.chunk;
   const int kv_end = min(L, kv_beg + p.chunk);
   const int n_tiles = kv_end > kv_beg ? (kv_end - kv_beg + kQTile - 1) / kQTile : 0;
-  const int64_t slot0 = (static_cast<int64_t>(b) * p.n_kv_heads + kvh) * p.max_splits;
 
   // ---- first code row of each of the chunk's pages; page ids are checked here
   int* pages = reinterpret_cast<int*>(smem + Sh::pages);
@@ -277,11 +334,13 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
 #pragma unroll
     for (int u = 0; u < per_warp; ++u) {
       const int r = warp + u * kMmaWarp;
-      const int g = (r0 + min(r, R - 1)) / p.K, j = (r0 + min(r, R - 1)) - g * p.K;
+      const int row = r / RP * RH + r % RP;  // of the CTA's
+      const bool live = r % RP < RH && row < R;
+      const int g = (r0 + min(row, R - 1)) / p.K, j = (r0 + min(row, R - 1)) - g * p.K;
       raw[u] = __ldg(reinterpret_cast<const uint2*>(
           p.q + ((static_cast<int64_t>(b) * p.K + j) * p.n_q_heads + kvh * G + g) * 128) + lane);
-      limit[u] = r < R ? min(kv_end, p.draft ? ((j == 0 && p.draft == 1) ? base + 1 : base + p.K) : base + j + 1) : 0;
-      if (r >= R) raw[u] = make_uint2(0u, 0u);
+      limit[u] = live ? min(kv_end, p.draft ? ((j == 0 && p.draft == 1) ? base + 1 : base + p.K) : base + j + 1) : 0;
+      if (!live) raw[u] = make_uint2(0u, 0u);
     }
 #pragma unroll
     for (int u = 0; u < per_warp; ++u) {
@@ -321,7 +380,7 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
       if (RT % kMmaWarp == 0 || r < RT) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int col = (r / RH) * 2 * RH + k * RH + r % RH;
+          const int col = r / RP * 2 * RP + k * RP + r % RP;
           *reinterpret_cast<uint32_t*>(smem + Sh::q + sw128(col, lane >> 2) + (lane & 3) * 4) = part[k];
         }
         if (lane == 0) {
@@ -407,7 +466,7 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     // ---- one thread per token (weights), then per dimension (output), for the rows of its group
-    const int t128 = tid & 127, grp = H == 1 ? 0 : warp >> 2, rb = grp * RH;
+    const int t128 = tid & 127, grp = H == 1 ? 0 : warp >> 2, rb = grp * RP;
     const float* coef = reinterpret_cast<const float*>(smem + Sh::coef) + rb;
     const int* lim = reinterpret_cast<const int*>(smem + Sh::lim) + rb;
     float* refs = reinterpret_cast<float*>(smem + Sh::ref);
@@ -415,7 +474,7 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
     float* betas = reinterpret_cast<float*>(smem + Sh::beta);
     float* xm = reinterpret_cast<float*>(smem + Sh::xm);
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t t_s = t_lane + grp * 2 * RH, t_o = t_lane + Sh::n1 + grp * Sh::p_cols;
+    const uint32_t t_s = t_lane + grp * 2 * RP, t_o = t_lane + Sh::n1 + grp * Sh::p_cols;
     uint8_t* ps = smem + Sh::p + grp * Sh::p_cols * kQTile;
     constexpr float off = FMT == GR_KV_E4M3 ? 8.f : 14.994309f;  // weights up to 2^8, or 32639 (two digits' largest)
     const int min_lim = min(kv_end, p.draft == 2 ? base + p.K : base + 1);
@@ -436,29 +495,26 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
       const float ev = ve == kKvExpBad ? __int_as_float(0x7fc00000) : static_cast<float>(ve);
       const float unv = ve == kKvExpBad ? 1.f : exp2i(-ve);
       float w[RH];
-      {
-        uint32_t s[2 * RH];
-        tmem_ld_cols<2 * RH>(t_s, s);
+      rows_by_parts<RP>([&](auto beg, auto num) {
+        constexpr int r0 = decltype(beg)::value, n = decltype(num)::value;
+        uint32_t s[2 * n];
+        tmem_ld_cols<n>(t_s + r0, s);
+        tmem_ld_cols<n>(t_s + RP + r0, s + n);
         tmem_ld_done(s);
 #pragma unroll
-        for (int r = 0; r < RH; ++r) {
-          float x;
-          if (FMT == GR_KV_E4M3) {
-            x = fmaf(__uint_as_float(s[RH + r]), 1.f / 16, __uint_as_float(s[r]));
-          } else {
-            x = static_cast<float>(static_cast<int>(s[r]) * 256 + static_cast<int>(s[RH + r]));
-          }
-          w[r] = x;
-        }
+        for (int r = 0; r < n; r += 4) {
+          const float4 c = *reinterpret_cast<const float4*>(coef + r0 + r);
+          float x[4];
 #pragma unroll
-        for (int r = 0; r < RH; r += 4) {
-          const float4 c = *reinterpret_cast<const float4*>(coef + r);
-          w[r] = fmaf(w[r], c.x * fk, ev);
-          w[r + 1] = fmaf(w[r + 1], c.y * fk, ev);
-          w[r + 2] = fmaf(w[r + 2], c.z * fk, ev);
-          w[r + 3] = fmaf(w[r + 3], c.w * fk, ev);
+          for (int e = 0; e < 4; ++e)
+            x[e] = FMT == GR_KV_E4M3 ? fmaf(__uint_as_float(s[n + r + e]), 1.f / 16, __uint_as_float(s[r + e]))
+                                     : static_cast<float>(static_cast<int>(s[r + e]) * 256 + static_cast<int>(s[n + r + e]));
+          const float cf[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (r0 + r + e < RH) w[r0 + r + e] = fmaf(x[e], cf[e] * fk, ev);
         }
-      }
+      });
       if (partial) {
 #pragma unroll
         for (int r = 0; r < RH; ++r)
@@ -474,8 +530,10 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
       // row maxima over the tile's 128 tokens: by warp, then one thread per row
 #pragma unroll
       for (int r = 0; r < RH; r += 4) {
-        const float4 x = make_float4(warp_max(w[r]), warp_max(w[r + 1]), warp_max(w[r + 2]), warp_max(w[r + 3]));
-        if (lane == 0) *reinterpret_cast<float4*>(xm + (warp & 3) * RT + rb + r) = x;
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = r + e < RH ? warp_max(w[r + e]) : 0.f;
+        if (lane == 0) *reinterpret_cast<float4*>(xm + (warp & 3) * RT + rb + r) = make_float4(x[0], x[1], x[2], x[3]);
       }
       named_sync(1, kSoft);
       bool raised = false;
@@ -488,6 +546,7 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
         betas[tid] = mt == -INFINITY ? 1.f : ex2_approx(mt - m_row);
         refs[tid] = off - (mt == -INFINITY ? 0.f : mt);
       }
+      __syncwarp();
       if (named_any(1, kSoft, raised)) {
 #pragma unroll
         for (int r = 0; r < RH; ++r) {
@@ -503,23 +562,22 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
       for (int r = 0; r < RH; r += 4) {
         const float4 rf = *reinterpret_cast<const float4*>(refs + rb + r);
         const float4 bt = *reinterpret_cast<const float4*>(betas + rb + r);
-        float x[4] = {ex2_approx(w[r] + rf.x), ex2_approx(w[r + 1] + rf.y), ex2_approx(w[r + 2] + rf.z),
-                      ex2_approx(w[r + 3] + rf.w)};
-        if (FMT == GR_KV_INT8) {  // the largest weight's exponent is rounded: past 32639 the digits would wrap
+        const float rfs[4] = {rf.x, rf.y, rf.z, rf.w}, bts[4] = {bt.x, bt.y, bt.z, bt.w};
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[k] = min_nan(x[k], 32639.f);
+        for (int e = 0; e < 4; ++e) {
+          if (r + e >= RH) break;
+          x[e] = ex2_approx(w[r + e] + rfs[e]);
+          if (FMT == GR_KV_INT8) x[e] = min_nan(x[e], 32639.f);  // the exponent is rounded: past 32639 the digits would wrap
+          // a hidden token's exponent may be that of a bad row, or of no row: its weight is 0, and 2^-ev is finite
+          l[r + e] = fmaf(x[e] * unv, bts[e], l[r + e]);
         }
-        // a hidden token's exponent may be that of a bad row, or of no row: its weight is 0, and 2^-ev is finite
-        l[r] = fmaf(x[0] * unv, bt.x, l[r]);
-        l[r + 1] = fmaf(x[1] * unv, bt.y, l[r + 1]);
-        l[r + 2] = fmaf(x[2] * unv, bt.z, l[r + 2]);
-        l[r + 3] = fmaf(x[3] * unv, bt.w, l[r + 3]);
         if (FMT == GR_KV_E4M3) {
 #pragma unroll
           for (int k = 0; k < 3; ++k) {
             const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
             const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
-            pw[(k * RH + r) / 4] = __byte_perm(lo, hi, 0x5410);
+            pw[(k * RP + r) / 4] = __byte_perm(lo, hi, 0x5410);
             if (k < 2) {
               const uint32_t h01 = e4m3x2_to_half2(lo), h23 = e4m3x2_to_half2(hi);
               const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h01));
@@ -537,7 +595,7 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
           for (int k = 0; k < 4; ++k) t[k] = __float_as_uint(x[k] + 8421504.f);
           const uint32_t a = __byte_perm(t[0], t[1], 0x5140), c = __byte_perm(t[2], t[3], 0x5140);  // lo lo hi hi
           pw[r / 4] = __byte_perm(a, c, 0x7632) ^ 0x80808080u;
-          pw[(RH + r) / 4] = __byte_perm(a, c, 0x5410) ^ 0x80808080u;
+          pw[(RP + r) / 4] = __byte_perm(a, c, 0x5410) ^ 0x80808080u;
         }
       }
 #pragma unroll
@@ -550,28 +608,33 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
       if (lane == 0) mbar_arrive(p_full);
       ok = ok && mbar_wait(o_full + (i & 1), (i >> 1) & 1, p.status, GR_ERR_TIMEOUT);
       tc_fence_after();
-      {
-        uint32_t x[Sh::p_parts * RH];
-        tmem_ld_cols<Sh::p_parts * RH>(t_o, x);
+      rows_by_parts<RP>([&](auto beg, auto num) {
+        constexpr int r0 = decltype(beg)::value, n = decltype(num)::value;
+        uint32_t x[Sh::p_parts * n];
+#pragma unroll
+        for (int k = 0; k < Sh::p_parts; ++k) tmem_ld_cols<n>(t_o + k * RP + r0, x + k * n);
         tmem_ld_done(x);
 #pragma unroll
-        for (int r1 = 0; r1 < RH; r1 += 4) {
-          const float4 bt = *reinterpret_cast<const float4*>(betas + rb + r1);
+        for (int r1 = 0; r1 < n; r1 += 4) {
+          const float4 bt = *reinterpret_cast<const float4*>(betas + rb + r0 + r1);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int r = r1 + e;
+            if (r0 + r >= RH) break;
             float y;
             if (FMT == GR_KV_E4M3)
-              y = fmaf(fmaf(__uint_as_float(x[2 * RH + r]), 1.f / 16, __uint_as_float(x[RH + r])), 1.f / 16,
+              y = fmaf(fmaf(__uint_as_float(x[2 * n + r]), 1.f / 16, __uint_as_float(x[n + r])), 1.f / 16,
                        __uint_as_float(x[r]));
             else
-              y = static_cast<float>(static_cast<int>(x[r]) * 256 + static_cast<int>(x[RH + r]));
-            o[r] = fmaf(y, e == 0 ? bt.x : (e == 1 ? bt.y : (e == 2 ? bt.z : bt.w)), o[r]);
+              y = static_cast<float>(static_cast<int>(x[r]) * 256 + static_cast<int>(x[n + r]));
+            o[r0 + r] = fmaf(y, e == 0 ? bt.x : (e == 1 ? bt.y : (e == 2 ? bt.z : bt.w)), o[r0 + r]);
           }
         }
-      }
+      });
     }
     // ---- l over the 128 tokens, then this split's result
+    const auto [b, kvh, blk, r0, R, n_active] = where();
+    const int64_t slot0 = (static_cast<int64_t>(b) * p.n_kv_heads + kvh) * p.max_splits;
     float* part = reinterpret_cast<float*>(smem + Sh::k);  // [RT][128]; the last tile's scores are done with the ring
 #pragma unroll
     for (int r = 0; r < RH; ++r) part[(rb + r) * kQTile + t128] = l[r];
@@ -594,23 +657,24 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
         if (lane == 0 && warp + u * kMmaWarp < RT) xm[warp + u * kMmaWarp] = sum[u];
     }
     named_sync(1, kSoft);
-    if (n_active > 1 && tid < R)
-      __stcg(reinterpret_cast<float2*>(p.ws_ml) + (slot0 + split) * R_all + r0 + tid, make_float2(m_row, xm[tid]));
+    const int own = tid / RP * RH + tid % RP;  // a row thread's row
+    if (n_active > 1 && tid < RT && tid % RP < RH && own < R)
+      __stcg(reinterpret_cast<float2*>(p.ws_ml) + (slot0 + split) * R_all + r0 + own, make_float2(m_row, xm[tid]));
     if (n_active == 1) {
 #pragma unroll
       for (int r = 0; r < RH; ++r) {
-        if (rb + r >= R) break;
+        if (grp * RH + r >= R) break;
         const float sum = xm[rb + r];
-        const int g = (r0 + rb + r) / p.K, j = (r0 + rb + r) - g * p.K;
+        const int g = (r0 + grp * RH + r) / p.K, j = (r0 + grp * RH + r) - g * p.K;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         p.out[((static_cast<int64_t>(b) * p.K + j) * p.n_q_heads + kvh * G + g) * 128 + t128] =
             __float2bfloat16(o[r] * inv);
       }
     } else {
-      float* dst = p.ws_o + ((slot0 + split) * R_all + r0 + rb) * 128 + t128;
+      float* dst = p.ws_o + ((slot0 + split) * R_all + r0 + grp * RH) * 128 + t128;
 #pragma unroll
       for (int r = 0; r < RH; ++r)
-        if (rb + r < R) __stcg(dst + r * 128, o[r]);
+        if (grp * RH + r < R) __stcg(dst + r * 128, o[r]);
     }
     tc_fence_before();
   }
@@ -619,14 +683,16 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
     tc_fence_after();
     tmem_dealloc(tmem, Sh::tmem_cols);
   }
-  if (n_active == 1) return;
 
   // ---- the last split to arrive joins them, in split order
+  const Kv8Place at = where();
+  if (at.n_active == 1) return;
+  const int64_t slot0 = (static_cast<int64_t>(at.b) * p.n_kv_heads + at.kvh) * p.max_splits;
   __threadfence();
   __syncthreads();
   if (tid == 0) {
-    int* tk = p.ws_ticket + (static_cast<int64_t>(b) * p.n_kv_heads + kvh) * p.row_blocks + blk;
-    const bool last = atomicAdd(tk, 1) == n_active - 1;
+    int* tk = p.ws_ticket + (static_cast<int64_t>(at.b) * p.n_kv_heads + at.kvh) * p.row_blocks + at.blk;
+    const bool last = atomicAdd(tk, 1) == at.n_active - 1;
     if (last) *tk = 0;
     *flag = last;
   }
@@ -652,7 +718,7 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int k = 0; k < per_lane; ++k)
-      if (lane + 32 * k < n_active) wgt[r * kKv8MaxSplits + lane + 32 * k] = x[k].x * inv;
+      if (lane + 32 * k < at.n_active) wgt[r * kKv8MaxSplits + lane + 32 * k] = x[k].x * inv;
   };
 #pragma unroll
   for (int u0 = 0; u0 < per_warp; u0 += 2) {  // two rows' loads at a time
@@ -663,25 +729,25 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
 #pragma unroll
       for (int k = 0; k < per_lane; ++k) {
         const int s2 = lane + 32 * k;
-        x[u][k] = r < R && s2 < n_active ? __ldcg(ml + (slot0 + s2) * R_all + r0 + r) : make_float2(-INFINITY, 0.f);
+        x[u][k] = r < at.R && s2 < at.n_active ? __ldcg(ml + (slot0 + s2) * R_all + at.r0 + r) : make_float2(-INFINITY, 0.f);
       }
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-      if (warp + (u0 + u) * kMmaWarp < R) weights(warp + (u0 + u) * kMmaWarp, x[u]);
+      if (warp + (u0 + u) * kMmaWarp < at.R) weights(warp + (u0 + u) * kMmaWarp, x[u]);
   }
   named_sync(1, kSoft);
   auto store4 = [&](int it, float4 a) {
-    const int r = r0 + (it >> 5);
+    const int r = at.r0 + (it >> 5);
     const int g = r / p.K, j = r - g * p.K;
     uint2 pk;
     pk.x = pack_bf16(a.x, a.y);
     pk.y = pack_bf16(a.z, a.w);
-    *reinterpret_cast<uint2*>(p.out + ((static_cast<int64_t>(b) * p.K + j) * p.n_q_heads + kvh * G + g) * 128 +
+    *reinterpret_cast<uint2*>(p.out + ((static_cast<int64_t>(at.b) * p.K + j) * p.n_q_heads + at.kvh * G + g) * 128 +
                               (it & 31) * 4) = pk;
   };
   auto add = [&](float4& a, int it, int s2) {
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_o + ((slot0 + s2) * R_all + r0 + (it >> 5)) * 128) +
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_o + ((slot0 + s2) * R_all + at.r0 + (it >> 5)) * 128) +
                             (it & 31));
     const float w = wgt[(it >> 5) * kKv8MaxSplits + s2];
     a.x += w * v.x;
@@ -689,20 +755,20 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
     a.z += w * v.z;
     a.w += w * v.w;
   };
-  if (R * 32 * 2 <= kSoft) {
+  if (at.R * 32 * 2 <= kSoft) {
     // one or two rows: the splits are shared between the threads, too
-    const int parts = kSoft / (R * 32), it = tid % (R * 32), part = tid / (R * 32);
+    const int parts = kSoft / (at.R * 32), it = tid % (at.R * 32), part = tid / (at.R * 32);
     float4* pool = reinterpret_cast<float4*>(smem + Sh::v);
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     if (part < parts) {
 #pragma unroll 8
-      for (int s2 = part; s2 < n_active; s2 += parts) add(a, it, s2);
+      for (int s2 = part; s2 < at.n_active; s2 += parts) add(a, it, s2);
     }
     pool[tid] = a;
     named_sync(1, kSoft);
     if (part == 0) {
       for (int k = 1; k < parts; ++k) {
-        const float4 v = pool[k * R * 32 + it];
+        const float4 v = pool[k * at.R * 32 + it];
         a.x += v.x;
         a.y += v.y;
         a.z += v.z;
@@ -712,19 +778,19 @@ __global__ void __launch_bounds__(128 * H + 64, RT > 16 ? 2 : 3) kv8_attention_k
     }
     return;
   }
-  for (int it0 = tid; it0 < R * 32; it0 += 4 * kSoft) {  // four (row, 4 dims) items' loads at a time
+  for (int it0 = tid; it0 < at.R * 32; it0 += 4 * kSoft) {  // four (row, 4 dims) items' loads at a time
     float4 a[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) a[u] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
-    for (int s2 = 0; s2 < n_active; ++s2) {
+    for (int s2 = 0; s2 < at.n_active; ++s2) {
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (it0 + u * kSoft < R * 32) add(a[u], it0 + u * kSoft, s2);
+        if (it0 + u * kSoft < at.R * 32) add(a[u], it0 + u * kSoft, s2);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (it0 + u * kSoft < R * 32) store4(it0 + u * kSoft, a[u]);
+      if (it0 + u * kSoft < at.R * 32) store4(it0 + u * kSoft, a[u]);
   }
 }
 
@@ -741,11 +807,11 @@ void kv8_attention_blocks(int rows, int* blocks, int* per_block) {
   *per_block = (rows + *blocks - 1) / *blocks;
 }
 
-template <int FMT, int RT, int H>
+template <int FMT, int RH, int H>
 static cudaError_t launch_kv8_attention_t(const CUtensorMap& tmk, const CUtensorMap& tmv, const KvAttnParams& p,
                                           cudaStream_t stream, bool pdl) {
-  auto kern = kv8_attention_kernel<FMT, RT, H>;
-  using Sh = KvAttnShape<FMT, RT, H>;
+  auto kern = kv8_attention_kernel<FMT, RH, H>;
+  using Sh = KvAttnShape<FMT, RH, H>;
   static PerDeviceOnce configured;
   cudaError_t e = once_per_device(configured, [&] {
     cudaError_t r = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::bytes);
@@ -768,15 +834,27 @@ static cudaError_t launch_kv8_attention_t(const CUtensorMap& tmk, const CUtensor
 template <int FMT>
 static cudaError_t launch_kv8_attention_f(const CUtensorMap& tmk, const CUtensorMap& tmv, const KvAttnParams& p,
                                           cudaStream_t stream, bool pdl) {
-  if (p.rows_per_block <= 4) return launch_kv8_attention_t<FMT, 4, 1>(tmk, tmv, p, stream, pdl);
-  if (p.rows_per_block <= 8) return launch_kv8_attention_t<FMT, 8, 1>(tmk, tmv, p, stream, pdl);
-  if (p.rows_per_block <= 16) return launch_kv8_attention_t<FMT, 16, 1>(tmk, tmv, p, stream, pdl);
-  return launch_kv8_attention_t<FMT, kQMaxRows, 2>(tmk, tmv, p, stream, pdl);
+  // Two groups halve a thread's share of a tile's chain, but an SM then holds two CTAs, not three.  Up to 8 rows they are
+  // for few CTAs (one request of 16,000 tokens, 8 rows: 18 us, one group 20; of 131,071, 2 rows: 50, 52) and one group for
+  // many (64 requests of 288-4,128, 8 rows: 59 us, two groups 64; 2 rows: 53).  From 9 rows on two are better everywhere (16
+  // rows: 74 us, one group 77).  A group has the rows of the next size up, 2 x 12, 17 or 20 (24 rows: 74 us, as 2 x 20 100;
+  // 34 rows: 95, 105).
+  if (p.rows_per_block <= 4)
+    return p.few ? launch_kv8_attention_t<FMT, 2, 2>(tmk, tmv, p, stream, pdl)
+                 : launch_kv8_attention_t<FMT, 4, 1>(tmk, tmv, p, stream, pdl);
+  if (p.rows_per_block <= 8)
+    return p.few ? launch_kv8_attention_t<FMT, 4, 2>(tmk, tmv, p, stream, pdl)
+                 : launch_kv8_attention_t<FMT, 8, 1>(tmk, tmv, p, stream, pdl);
+  if (p.rows_per_block <= 16) return launch_kv8_attention_t<FMT, 8, 2>(tmk, tmv, p, stream, pdl);
+  if (p.rows_per_block <= 24) return launch_kv8_attention_t<FMT, 12, 2>(tmk, tmv, p, stream, pdl);
+  if (p.rows_per_block <= 34) return launch_kv8_attention_t<FMT, 17, 2>(tmk, tmv, p, stream, pdl);
+  return launch_kv8_attention_t<FMT, kQMaxRows / 2, 2>(tmk, tmv, p, stream, pdl);
 }
 
 cudaError_t launch_kv8_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, KvAttnParams p, int format,
                                  cudaStream_t stream, bool pdl) {
-  kv8_attention_blocks(p.n_q_heads / p.n_kv_heads * p.K, &p.row_blocks, &p.rows_per_block);
+  p.group = p.n_q_heads / p.n_kv_heads;
+  kv8_attention_blocks(p.group * p.K, &p.row_blocks, &p.rows_per_block);
   return format == GR_KV_E4M3 ? launch_kv8_attention_f<GR_KV_E4M3>(tmk, tmv, p, stream, pdl)
                               : launch_kv8_attention_f<GR_KV_INT8>(tmk, tmv, p, stream, pdl);
 }

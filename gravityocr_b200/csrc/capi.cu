@@ -900,30 +900,35 @@ int gr_kv_read(const gr_kv_cache* cache, const int64_t* slots, int64_t n, void* 
 }
 
 size_t gr_kv8_attention_workspace_bytes(int bs, int K, int n_q_heads, int n_kv_heads, int max_splits) {
-  if (bs <= 0 || K <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads || max_splits <= 0) return 0;
+  if (bs <= 0 || K <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads || max_splits <= 0 ||
+      static_cast<int64_t>(n_q_heads / n_kv_heads) * K > kKv8MaxRows || max_splits > kKv8MaxSplits ||
+      static_cast<int64_t>(bs) * n_kv_heads > kKv8TicketPairs)
+    return 0;
   return kv8_attention_ws_bytes(bs, n_q_heads / n_kv_heads * K, n_kv_heads, max_splits, nullptr, nullptr);
 }
 
 int gr_kv8_attention_plan(int bs, int K, int max_len, int n_q_heads, int n_kv_heads, int32_t* out) {
-  if (!out || bs <= 0 || K <= 0 || max_len <= 0 || max_len > kKv8MaxChunk * kKv8MaxSplits || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads)
+  if (!out || bs <= 0 || K <= 0 || max_len <= 0 || max_len > kKv8MaxChunk * kKv8MaxSplits || n_kv_heads <= 0 ||
+      n_q_heads <= 0 || n_q_heads % n_kv_heads)
     return GR_ERR_ARG;
-  // the (request, head, row block) triples times the splits of the longest request make about one wave of two CTAs an SM
-  // (131,071 tokens of one request: 37 splits 52 us, 55 splits 55 us); many requests of mixed lengths go in even pieces.
-  // A CTA of more than 16 rows pays about five tiles' time for its queries and its part of the join, so its pieces are
-  // longer (64 requests of 288-4,128 tokens, one row: 56 us at 1,536 tokens, 61 at 1,024; 17 rows: 116 us at 3,200, 135
-  // at 1,536).
+  const int64_t rows = static_cast<int64_t>(n_q_heads / n_kv_heads) * K;
+  if (rows > kKv8MaxRows || static_cast<int64_t>(bs) * n_kv_heads > kKv8TicketPairs) return GR_ERR_UNSUPPORTED;
+  // The (request, head, row block) triples times the splits of the longest request make about one wave of two CTAs an SM
+  // (131,071 tokens of one request: 37 splits 52 us, 55 splits 55 us).  Where the triples alone fill the SMs, lengths are
+  // taken to be mixed: pieces of at most 3,200 tokens, shorter where that leaves SMs without a second CTA (64 requests of
+  // 288-4,128 tokens, one row: 54 us at 3,200, 58 at 1,536, 54 unsplit; 17 rows: 95, 120, 99; 20 requests, one row: 29 us
+  // at 3,200, 24 at 2,048; 64 of 100-16,000, one row: 167 us at 3,200, 181 at 8,192).
+  // Pieces of c tokens cost c / 128 tiles in turn and a join of length / c parts by one CTA, which takes half a tile's time a
+  // part: no less than c = 8 sqrt(length).  One request of 3,000 tokens, 17 rows: 20 us at 384, 29 at 128; of 16,000: 32
+  // at 1,024, 44 at 448; one row: 10 and 11, 14 and 16.  Whole tiles: 192 takes as long as 256, and joins more.
   int blocks, per_block;
-  kv8_attention_blocks(n_q_heads / n_kv_heads * K, &blocks, &per_block);
-  const int64_t units = static_cast<int64_t>(bs) * n_kv_heads * blocks;
-  const int64_t per = std::max<int64_t>(1, 2LL * num_sms() / units);
-  const int64_t piece = per_block > 16 ? 3200 : 1536;
-  int64_t chunk = (static_cast<int64_t>(max_len) + per - 1) / per;
-  if (chunk > piece && units >= num_sms()) chunk = piece;
-  const int64_t least = (static_cast<int64_t>(max_len) + kKv8MaxSplits - 1) / kKv8MaxSplits;
-  if (chunk < least) chunk = least;
-  if (chunk < 128) chunk = 128;
-  chunk = (chunk + 31) / 32 * 32;
-  if (chunk > kKv8MaxChunk) chunk = kKv8MaxChunk;
+  kv8_attention_blocks(static_cast<int>(rows), &blocks, &per_block);
+  const int64_t units = static_cast<int64_t>(bs) * n_kv_heads * blocks, wave = 2LL * num_sms();
+  int64_t chunk = units < num_sms() ? (max_len + wave / units - 1) / (wave / units)
+                                    : std::min<int64_t>({3200, max_len, (max_len * units + wave - 1) / wave});
+  const int64_t tiles = static_cast<int64_t>(8.0 * std::sqrt(static_cast<double>(max_len)) / 128 + 0.5);
+  chunk = std::max({chunk, tiles * 128, (static_cast<int64_t>(max_len) + kKv8MaxSplits - 1) / kKv8MaxSplits});
+  chunk = std::min<int64_t>((chunk + 127) / 128 * 128, kKv8MaxChunk);
   out[0] = static_cast<int32_t>(chunk);
   out[1] = static_cast<int32_t>((max_len + chunk - 1) / chunk);
   return GR_OK;
@@ -936,11 +941,11 @@ int gr_kv8_attention(const void* q, const gr_kv_cache* cache, const int32_t* pag
   if (rc) return rc;
   if (cache->format == GR_KV_BF16) return GR_ERR_UNSUPPORTED;
   if (!q || !page_table || !seq_lens || !out || bs <= 0 || K <= 0 || pt_stride <= 0 || n_q_heads <= 0 ||
-      n_q_heads % cache->n_kv_heads || draft < 0 || draft > 2 || chunk <= 0 || chunk % 32 || chunk > kKv8MaxChunk || max_splits <= 0 ||
-      max_splits > kKv8MaxSplits || !aligned(q, 16) || !aligned(out, 16))
+      n_q_heads % cache->n_kv_heads || draft < 0 || draft > 2 || chunk <= 0 || chunk % 32 || chunk > kKv8MaxChunk ||
+      max_splits <= 0 || max_splits > kKv8MaxSplits || !aligned(q, 16) || !aligned(out, 16))
     return GR_ERR_ARG;
   const int64_t rows = static_cast<int64_t>(n_q_heads / cache->n_kv_heads) * K;
-  if (rows > 128) return GR_ERR_UNSUPPORTED;
+  if (rows > kKv8MaxRows) return GR_ERR_UNSUPPORTED;
   int blocks, per_block;
   kv8_attention_blocks(static_cast<int>(rows), &blocks, &per_block);
   if (static_cast<int64_t>(bs) * cache->n_kv_heads * blocks > kKv8TicketPairs || pt_stride > (INT32_MAX - 8192) / 16)
@@ -979,6 +984,12 @@ int gr_kv8_attention(const void* q, const gr_kv_cache* cache, const int32_t* pag
   p.n_kv_heads = cache->n_kv_heads;
   p.chunk = chunk;
   p.max_splits = max_splits;
+  // More CTAs than run at once (two an SM): requests in order of length, longest first, so that no long one starts last.
+  // 64 requests of 288-4,128 tokens, 17 rows: 95 us, 108-115 by index; 1.5 us more where all are of 1,000 tokens (57).  Up
+  // to 16 rows CTAs wait for memory rather than for the last one's end: one row 52 us against 54, and 96 against 89 at 128
+  // requests.
+  p.few = static_cast<int64_t>(bs) * cache->n_kv_heads * blocks * max_splits <= 2 * num_sms();
+  p.longest_first = per_block > 16 && bs > 1 && bs <= kKv8MaxSort && !p.few;
   p.scale_log2 = (1.0f / sqrtf(128.0f)) * 1.4426950408889634f;
   p.status = status;
   return launch_kv8_attention(tmk, tmv, p, cache->format, static_cast<cudaStream_t>(stream), g_pdl) == cudaSuccess

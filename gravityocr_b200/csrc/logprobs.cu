@@ -82,7 +82,6 @@ __device__ __forceinline__ float lp_key_logit(uint64_t k) {
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
 
-// 16-byte loads of logits: their maximum (NaNs ignored), and how many are >= t.
 // Two fp32 numbers in a register pair (add, mul and fma take both at once).
 __device__ __forceinline__ uint64_t f2_pack(float a, float b) {
   uint64_t r;
@@ -108,6 +107,7 @@ __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
+// A 16-byte load of logits: its elements, their maximum (NaNs ignored), and how many are >= t.
 template <typename T>
 struct LpVec;
 template <>
@@ -191,7 +191,8 @@ __device__ __forceinline__ void lp_one(LpThread& t, float x, int id, float k, fl
 // A batch of loads NT apart, id0 the id of the first one's first element; the first `valid` hold logits, the rest
 // -inf, which adds nothing to the sums and must not be counted.  Returns the batch's maximum.
 template <typename T, int NT>
-__device__ __forceinline__ float lp_batch(LpThread& t, const uint4 (&raw)[LpVec<T>::B], int id0, int valid, float k, float mine, float mine_next, int my_id) {
+__device__ __forceinline__ float lp_batch(LpThread& t, const uint4 (&raw)[LpVec<T>::B], int id0, int valid, float k,
+                                          float mine, float mine_next, int my_id) {
   using V = LpVec<T>;
   float bm = V::max_of(raw[0]);
 #pragma unroll
@@ -523,7 +524,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const Log
   if (ctas == 1) {
     if (tid < n) put_top(tid, s_top[tid]);
   } else {
-    const int total = n * static_cast<int>(ctas);  // at most kLpGroups * kLpMaxCluster keys, where ctas > 1 comes with as many threads
+    // at most kLpGroups * kLpMaxCluster keys: clusters come with as many threads
+    const int total = n * static_cast<int>(ctas);
     const uint64_t key = tid < total ? lp_peer_u64(&s_top[tid % n], tid / n) : 0;
     __syncwarp();
     lp_cluster_sync();

@@ -177,7 +177,10 @@ struct KvAttnParams {
   const int64_t* seq_lens;
   int bs, K, draft, base_add, n_q_heads, n_kv_heads;
   int chunk, max_splits;
+  int group;                       // query heads of a K/V head
   int row_blocks, rows_per_block;  // a CTA's share of a K/V head's query rows
+  int few;                         // no more CTAs than run at once
+  int longest_first;               // requests are taken by length, not by index (bs <= kKv8MaxSort, more than 16 rows)
   float scale_log2;
   float* ws_o;
   float* ws_ml;
@@ -269,6 +272,8 @@ cudaError_t launch_kv8_attention(const CUtensorMap& tmk, const CUtensorMap& tmv,
 void kv8_attention_blocks(int rows, int* blocks, int* per_block);
 constexpr int kKv8TicketPairs = 16384;  // (request, K/V head, row block) triples of one call
 constexpr int kKv8MaxSplits = 128;
+constexpr int kKv8MaxRows = 128;        // query heads of a K/V head times window rows
+constexpr int kKv8MaxSort = 256;       // requests that the attention orders by length
 constexpr int kKv8MaxChunk = 8192;      // cache tokens of a split
 cudaError_t launch_token_logprobs(LogprobParams p, bool bf16, cudaStream_t stream, bool pdl);
 constexpr int kLogprobMaxTop = 64;

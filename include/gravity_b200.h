@@ -293,13 +293,13 @@ typedef struct gr_kv_cache {
 } gr_kv_cache;
 
 /* From m projected rows qkv [m, ld_qkv] bf16 (q heads | k heads | v heads, 128 each; ld_qkv % 8 == 0; qkv, q_out and the
- * norm weights 16-byte aligned) in one pass: q and k heads take their RMS norm (q_norm / k_norm bf16 [128], or NULL for none), x * w / sqrt(mean x^2 + eps);
- * then the rotation of their first rotary_dim elements (0..128, a multiple of 8, of 16 with rope_half; rope_half 0:
- * pairs (2i, 2i + 1); 1: pairs (i, i + rotary_dim / 2)) by the angle position * inv_freq[i], formed in 64 bits; q goes to q_out bf16 [m, n_q_heads *
- * 128], k and v rows to the cache at row_slot (page * 16 + offset).  Positions are row_pos [m], or row_pos3 [m][3] with
- * mrope_section (three pair counts, as gr_epilogue); both NULL only with rotary_dim 0.  A negative slot writes q only; a
- * slot past the cache sets GR_ERR_BAD_PAGE and writes q only.  No two rows may share a slot.  Inputs and outputs may not
- * overlap. */
+ * norm weights 16-byte aligned) in one pass: q and k heads take their RMS norm (q_norm / k_norm bf16 [128], or NULL for
+ * none), x * w / sqrt(mean x^2 + eps); then the rotation of their first rotary_dim elements (0..128, a multiple of 8, of 16
+ * with rope_half; rope_half 0: pairs (2i, 2i + 1); 1: pairs (i, i + rotary_dim / 2)) by the angle position * inv_freq[i],
+ * formed in 64 bits; q goes to q_out bf16 [m, n_q_heads * 128], k and v rows to the cache at row_slot (page * 16 + offset).
+ * Positions are row_pos [m], or row_pos3 [m][3] with mrope_section (three pair counts, as gr_epilogue); both NULL only with
+ * rotary_dim 0.  A negative slot writes q only; a slot past the cache sets GR_ERR_BAD_PAGE and writes q only.  No two rows
+ * may share a slot.  Inputs and outputs may not overlap. */
 int gr_qk_norm_rope_write(const void* qkv, int64_t ld_qkv, int m, int n_q_heads, const gr_kv_cache* cache,
                           const void* q_norm, const void* k_norm, double eps, const int32_t* row_pos,
                           const int32_t* row_pos3, const int32_t* mrope_section, const float* inv_freq, int rotary_dim,
@@ -313,9 +313,10 @@ int gr_kv_read(const gr_kv_cache* cache, const int64_t* slots, int64_t n, void* 
 /* gr_bd_attention over an 8-bit cache (GR_KV_BF16 is GR_ERR_UNSUPPORTED: gr_bd_attention reads that): the same rows, masks
  * (draft 0, 1, 2) and page tables.  K = 1 is one decode token.  A row that sees nothing (seq_lens[b] + base_add + j < 0: a
  * padding request has seq_lens -K - base_add) gives zeros.  Lengths past the page table, and page ids past the cache, set
- * GR_ERR_BAD_PAGE; lengths past chunk * max_splits set GR_ERR_ARG (the rest is not seen).  chunk: a multiple of 32, at most 8192; max_splits <= 128;
- * chunk * max_splits >= the longest length + K.
- * workspace: gr_kv8_attention_workspace_bytes, zero-filled once (needed for max_splits > 1), one call at a time. */
+ * GR_ERR_BAD_PAGE; lengths past chunk * max_splits set GR_ERR_ARG (the rest is not seen).  Query heads per K/V head times K
+ * at most 128.  chunk: a multiple of 32, at most 8192; max_splits <= 128; chunk * max_splits >= the longest length + K.
+ * workspace: gr_kv8_attention_workspace_bytes (0: a shape that is not supported), zero-filled once (needed for max_splits >
+ * 1), one call at a time. */
 size_t gr_kv8_attention_workspace_bytes(int bs, int K, int n_q_heads, int n_kv_heads, int max_splits);
 int gr_kv8_attention(const void* q, const gr_kv_cache* cache, const int32_t* page_table, int pt_stride,
                      const int64_t* seq_lens, int bs, int K, int draft, int base_add, int n_q_heads, int chunk,

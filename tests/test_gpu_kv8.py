@@ -333,6 +333,51 @@ def test_attention_splits(fmt, K, chunk, splits):
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("K,nkv,group", [(1, 8, 2), (1, 8, 1), (3, 8, 2), (4, 8, 2), (1, 8, 5), (6, 8, 2), (3, 8, 3), (8, 8, 2),
+                                         (9, 8, 2), (12, 8, 2), (25, 8, 1), (17, 8, 2), (7, 8, 5), (20, 8, 2), (41, 8, 1)])
+def test_attention_row_counts(fmt, K, nkv, group):
+    """Every split of the rows between thread groups, for more CTAs than run at once and for few."""
+    lens = [(37 * b) % 150 for b in range(76)]
+    c = _attn_case(fmt, lens, K, group * nkv, nkv)
+    out = _attend(c)
+    cut = dict(c, pt=c["pt"][:9].contiguous(), q=c["q"][: 9 * K], lens=lens[:9], bs=9)
+    few = _attend(cut)
+    _check_attention(cut, few)
+    _check_attention(cut, out[: 9 * K])
+    c["slots"], c["lens"] = c["slots"][-9:], c["lens"][-9:]
+    _check_attention(dict(c, q=c["q"][-9 * K:], bs=9), out[-9 * K:])
+
+
+@pytest.mark.parametrize("bs", [20, 255, 256, 257])
+@pytest.mark.parametrize("fmt,K", [("int8", 17), ("e4m3", 20)])
+def test_attention_of_many_requests_is_each_ones_own(fmt, K, bs):
+    """Whatever order the requests run in (mixed, equal, empty and padding ones, more or fewer than are sorted), each gets the
+    rows that it gets alone, and the tickets come back to zero."""
+    g = torch.Generator().manual_seed(bs)
+    lens = torch.randint(0, 700, (bs,), generator=g).tolist()
+    lens[1], lens[2], lens[3], lens[bs - 1] = 0, -K, lens[5], 699
+    c = _attn_case(fmt, lens, K, 16, 8)
+    ws = torch.zeros((L.kv8_attention_workspace_bytes(bs, K, 16, 8, 3),), dtype=torch.uint8, device=DEV)
+    st = _status()
+    out = _attend(c, chunk=256, splits=3, ws=ws, status=st)
+    assert int(st) == 0 and int(ws[:65536].sum()) == 0
+    for b in sorted({0, 1, 2, 3, 5, bs - 1, *torch.randint(0, bs, (12,), generator=g).tolist()}):
+        one = dict(c, pt=c["pt"][b: b + 1].contiguous(), q=c["q"][b * K: (b + 1) * K], lens=[lens[b]], bs=1)
+        assert torch.equal(out[b * K: (b + 1) * K], _attend(one, chunk=256, splits=3)), b
+    if bs == 20:
+        _check_attention(c, out)
+        # beyond a short plan, and beyond the page table: reported, the other requests as before
+        for cut, code in ((2, 1), (3, 6)):
+            short = dict(c, pt=c["pt"] if cut == 2 else c["pt"][:, :30].contiguous())
+            st.zero_()
+            got = _attend(short, chunk=256, splits=cut, ws=ws, status=st)
+            assert int(st) == code and int(ws[:65536].sum()) == 0
+            for b in range(bs):
+                if lens[b] + K <= 480:
+                    assert torch.equal(got[b * K: (b + 1) * K], out[b * K: (b + 1) * K])
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 def test_attention_peaked_and_flat_scores(fmt):
     for q_scale in (0.0, 8.0):
         c = _attn_case(fmt, [1500, 40], 1, 16, 8, q_scale=q_scale)

@@ -130,6 +130,16 @@ def test_plan_refuses():
     assert L.kv8_attention_workspace_bytes(1, 1, 15, 8, 1) == 0
 
 
+def test_plan_of_too_many_rows():
+    """Row counts past the kernel's 128, and past 32 bits."""
+    lib, out = L.load(), (ctypes.c_int32 * 2)()
+    for K, nq, nkv in [(65, 16, 8), (2 ** 31 - 1, 16, 8), (2 ** 31 - 1, 2 ** 31 - 1, 1), (1, 129, 1)]:
+        assert lib.gr_kv8_attention_plan(1, K, 4096, nq, nkv, out) == UNSUPPORTED
+        assert L.kv8_attention_workspace_bytes(1, K, nq, nkv, 4) == 0
+    assert lib.gr_kv8_attention_plan(2 ** 31 - 1, 1, 2 ** 20, 2 ** 31 - 1, 2 ** 31 - 1, out) == UNSUPPORTED
+    assert L.kv8_attention_workspace_bytes(2 ** 31 - 1, 1, 8, 8, 4) == L.kv8_attention_workspace_bytes(1, 1, 8, 8, 129) == 0
+
+
 def test_wrappers_want_cuda_tensors():
     k = torch.zeros((2, 1, 16, 128), dtype=torch.int8)
     e = torch.zeros((2, 1, 16), dtype=torch.int8)
