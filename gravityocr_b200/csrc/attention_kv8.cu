@@ -36,6 +36,7 @@
 // sum of as many bytes takes 49.5; 64 requests of 288-4,128 tokens 53 us (291 MB): bound by the memory.  17 rows of these 64:
 // 99 us int8, 115 e4m3, bound by the softmax threads: their instructions fill half of the issue slots, and a tile's chain
 // (scores, maxima, weights, P, O) the time between.
+#include <algorithm>
 #include <type_traits>
 
 #include "kv8_dev.cuh"
@@ -801,10 +802,14 @@ size_t kv8_attention_ws_bytes(int bs, int rows, int n_kv_heads, int max_splits, 
   return kQTicketBytes + n * 520;
 }
 
-// Rows of a CTA: at most kQMaxRows, the row blocks of a head as even as possible.
-void kv8_attention_blocks(int rows, int* blocks, int* per_block) {
-  *blocks = (rows + kQMaxRows - 1) / kQMaxRows;
+// Row blocks of a head: at least as many as keep kQMaxRows, at most `room` (CTAs that are to spare) down to 8 rows, as even as
+// possible.  A block reads the cache again, from L2: for few CTAs that costs less than a long softmax and one CTA's join
+// (one request of 3,000 tokens, 34 rows in 4 blocks: 15 us, in one 20).
+void kv8_attention_blocks(int rows, int64_t room, int* blocks, int* per_block) {
+  const int64_t least = (rows + kQMaxRows - 1) / kQMaxRows, most = (rows + 7) / 8;
+  *blocks = static_cast<int>(std::max(least, std::min(room, most)));
   *per_block = (rows + *blocks - 1) / *blocks;
+  *blocks = (rows + *per_block - 1) / *per_block;
 }
 
 template <int FMT, int RH, int H>
@@ -851,10 +856,8 @@ static cudaError_t launch_kv8_attention_f(const CUtensorMap& tmk, const CUtensor
   return launch_kv8_attention_t<FMT, kQMaxRows / 2, 2>(tmk, tmv, p, stream, pdl);
 }
 
-cudaError_t launch_kv8_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, KvAttnParams p, int format,
+cudaError_t launch_kv8_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, const KvAttnParams& p, int format,
                                  cudaStream_t stream, bool pdl) {
-  p.group = p.n_q_heads / p.n_kv_heads;
-  kv8_attention_blocks(p.group * p.K, &p.row_blocks, &p.rows_per_block);
   return format == GR_KV_E4M3 ? launch_kv8_attention_f<GR_KV_E4M3>(tmk, tmv, p, stream, pdl)
                               : launch_kv8_attention_f<GR_KV_INT8>(tmk, tmv, p, stream, pdl);
 }

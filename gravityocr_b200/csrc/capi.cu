@@ -922,7 +922,7 @@ int gr_kv8_attention_plan(int bs, int K, int max_len, int n_q_heads, int n_kv_he
   // part: no less than c = 8 sqrt(length).  One request of 3,000 tokens, 17 rows: 20 us at 384, 29 at 128; of 16,000: 32
   // at 1,024, 44 at 448; one row: 10 and 11, 14 and 16.  Whole tiles: 192 takes as long as 256, and joins more.
   int blocks, per_block;
-  kv8_attention_blocks(static_cast<int>(rows), &blocks, &per_block);
+  kv8_attention_blocks(static_cast<int>(rows), 1, &blocks, &per_block);
   const int64_t units = static_cast<int64_t>(bs) * n_kv_heads * blocks, wave = 2LL * num_sms();
   int64_t chunk = units < num_sms() ? (max_len + wave / units - 1) / (wave / units)
                                     : std::min<int64_t>({3200, max_len, (max_len * units + wave - 1) / wave});
@@ -946,9 +946,10 @@ int gr_kv8_attention(const void* q, const gr_kv_cache* cache, const int32_t* pag
     return GR_ERR_ARG;
   const int64_t rows = static_cast<int64_t>(n_q_heads / cache->n_kv_heads) * K;
   if (rows > kKv8MaxRows) return GR_ERR_UNSUPPORTED;
+  const int64_t pairs = static_cast<int64_t>(bs) * cache->n_kv_heads, wave = 2LL * num_sms();
   int blocks, per_block;
-  kv8_attention_blocks(static_cast<int>(rows), &blocks, &per_block);
-  if (static_cast<int64_t>(bs) * cache->n_kv_heads * blocks > kKv8TicketPairs || pt_stride > (INT32_MAX - 8192) / 16)
+  kv8_attention_blocks(static_cast<int>(rows), pairs > kKv8TicketPairs ? 1 : wave / (pairs * max_splits), &blocks, &per_block);
+  if (pairs > kKv8TicketPairs / blocks || pt_stride > (INT32_MAX - 8192) / 16)
     return GR_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(chunk) * max_splits < K) return GR_ERR_ARG;
   KvAttnParams p;
@@ -984,11 +985,14 @@ int gr_kv8_attention(const void* q, const gr_kv_cache* cache, const int32_t* pag
   p.n_kv_heads = cache->n_kv_heads;
   p.chunk = chunk;
   p.max_splits = max_splits;
+  p.group = n_q_heads / cache->n_kv_heads;
+  p.row_blocks = blocks;
+  p.rows_per_block = per_block;
   // More CTAs than run at once (two an SM): requests in order of length, longest first, so that no long one starts last.
   // 64 requests of 288-4,128 tokens, 17 rows: 95 us, 108-115 by index; 1.5 us more where all are of 1,000 tokens (57).  Up
   // to 16 rows CTAs wait for memory rather than for the last one's end: one row 52 us against 54, and 96 against 89 at 128
   // requests.
-  p.few = static_cast<int64_t>(bs) * cache->n_kv_heads * blocks * max_splits <= 2 * num_sms();
+  p.few = pairs * blocks * max_splits <= wave;
   p.longest_first = per_block > 16 && bs > 1 && bs <= kKv8MaxSort && !p.few;
   p.scale_log2 = (1.0f / sqrtf(128.0f)) * 1.4426950408889634f;
   p.status = status;

@@ -267,9 +267,9 @@ cudaError_t launch_penalty_cumulate(const SampleParams& p, cudaStream_t s);
 cudaError_t launch_qk_norm_rope_write(KvWriteParams p, int format, bool half, cudaStream_t s, bool pdl);
 cudaError_t launch_kv_read(const KvReadParams& p, int format, cudaStream_t s, bool pdl);
 size_t kv8_attention_ws_bytes(int bs, int rows, int n_kv_heads, int max_splits, size_t* o_off, size_t* ml_off);
-cudaError_t launch_kv8_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, KvAttnParams p, int format,
+cudaError_t launch_kv8_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, const KvAttnParams& p, int format,
                                  cudaStream_t stream, bool pdl);
-void kv8_attention_blocks(int rows, int* blocks, int* per_block);
+void kv8_attention_blocks(int rows, int64_t room, int* blocks, int* per_block);
 constexpr int kKv8TicketPairs = 16384;  // (request, K/V head, row block) triples of one call
 constexpr int kKv8MaxSplits = 128;
 constexpr int kKv8MaxRows = 128;        // query heads of a K/V head times window rows
