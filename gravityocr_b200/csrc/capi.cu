@@ -919,13 +919,17 @@ int gr_kv8_attention_plan(int bs, int K, int max_len, int n_q_heads, int n_kv_he
   // 288-4,128 tokens, one row: 54 us at 3,200, 58 at 1,536, 54 unsplit; 17 rows: 95, 120, 99; 20 requests, one row: 29 us
   // at 3,200, 24 at 2,048; 64 of 100-16,000, one row: 167 us at 3,200, 181 at 8,192).
   // Pieces of c tokens cost c / 128 tiles in turn and a join of length / c parts by one CTA, which takes half a tile's time a
-  // part: no less than c = 8 sqrt(length).  One request of 3,000 tokens, 17 rows: 20 us at 384, 29 at 128; of 16,000: 32
-  // at 1,024, 44 at 448; one row: 10 and 11, 14 and 16.  Whole tiles: 192 takes as long as 256, and joins more.
+  // part: no less than c = 8 sqrt(length).  One request of 3,000 tokens, 8 window rows: 11 us at 384, 16 at 128; of 16,000:
+  // 21 at 1,024, 23 at 512; one row: 9.5 and 9.8, 14 and 13.5.  Whole tiles: 192 takes as long as 256, and joins more.
   int blocks, per_block;
   kv8_attention_blocks(static_cast<int>(rows), 1, &blocks, &per_block);
   const int64_t units = static_cast<int64_t>(bs) * n_kv_heads * blocks, wave = 2LL * num_sms();
   int64_t chunk = units < num_sms() ? (max_len + wave / units - 1) / (wave / units)
                                     : std::min<int64_t>({3200, max_len, (max_len * units + wave - 1) / wave});
+  // Pieces of up to 1,024 tokens leave room for row blocks of 16 rows instead, whose softmax and join are shorter (4 requests
+  // of 3,000 tokens, 34 rows: 20 us in 3 pieces and 3 blocks, 24 in 8 pieces).
+  const int64_t narrow = static_cast<int64_t>(bs) * n_kv_heads * ((rows + 15) / 16);
+  if (narrow < num_sms() && max_len <= 1024 * (wave / narrow)) chunk = (max_len + wave / narrow - 1) / (wave / narrow);
   const int64_t tiles = static_cast<int64_t>(8.0 * std::sqrt(static_cast<double>(max_len)) / 128 + 0.5);
   chunk = std::max({chunk, tiles * 128, (static_cast<int64_t>(max_len) + kKv8MaxSplits - 1) / kKv8MaxSplits});
   chunk = std::min<int64_t>((chunk + 127) / 128 * 128, kKv8MaxChunk);
@@ -948,7 +952,8 @@ int gr_kv8_attention(const void* q, const gr_kv_cache* cache, const int32_t* pag
   if (rows > kKv8MaxRows) return GR_ERR_UNSUPPORTED;
   const int64_t pairs = static_cast<int64_t>(bs) * cache->n_kv_heads, wave = 2LL * num_sms();
   int blocks, per_block;
-  kv8_attention_blocks(static_cast<int>(rows), pairs > kKv8TicketPairs ? 1 : wave / (pairs * max_splits), &blocks, &per_block);
+  kv8_attention_blocks(static_cast<int>(rows), pairs > kKv8TicketPairs ? 1 : wave / (pairs * max_splits), &blocks,
+                       &per_block);
   if (pairs > kKv8TicketPairs / blocks || pt_stride > (INT32_MAX - 8192) / 16)
     return GR_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(chunk) * max_splits < K) return GR_ERR_ARG;
