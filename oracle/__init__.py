@@ -9,6 +9,7 @@ Modules:
     full-draft round, AR greedy and teacher forcing.
   * ``commit_ref``: numpy restatement of the linear-chain accept, the reference's Triton commit kernel and the host
     commit rules.
+  * ``kv8_ref``: the 8-bit K/V cache's rows (quantising, reading back) and the attention over them in 64 bits.
 
 Pins: ``tests/golden/`` holds vectors generated by running the reference itself (natcache + teacher forcing through
 transformers' GLM-OCR, the Triton commit kernel under the Triton CPU interpreter, the commit-rules module), by the
