@@ -53,102 +53,154 @@ template <bool HALF>
 __device__ __forceinline__ int pair_slot(int i) {
   return HALF ? (i & 7) * 8 + (i >> 3) : (i & 3) * 16 + (i >> 2);
 }
-// This lane's k-th pair: of its elements 2k, 2k + 1, or (half-split) of its element k and its partner.
+// The slot of this lane's pair 0 (k further pairs at + k * 8 or k * 16): of its elements 2k, 2k + 1, or (half-split, hop lanes
+// between an element and its partner) of its element k and its partner.  Lanes past the rotation find (1, 0).
 template <bool HALF>
-__device__ __forceinline__ int lane_slot(int k, int l16, int hop) {
-  return HALF ? k * 8 + (l16 < hop ? l16 : (l16 - hop) & 7) : k * 16 + l16;
+__device__ __forceinline__ int lane_slot(int l16, int hop) {
+  return HALF ? (l16 < hop ? l16 : (l16 < 2 * hop ? l16 - hop : hop & 7)) : l16;
 }
-// Norm and rotation of a head in T (float or double): y = rope(x * w / sqrt(mean x^2 + eps)); cs(k): this lane's k-th pair.
-template <typename T, bool HALF, typename F>
-__device__ __forceinline__ void norm_rotate(const float (&x)[8], bool norm, const uint4& w, double eps, int rotary_dim,
-                                            int l16, T (&y)[8], F cs) {
+// 1 / sqrt(mean x^2 + eps) of a head.
+template <typename T>
+__device__ __forceinline__ T head_rms(const float (&x)[8], double eps) {
+  T ss = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss += static_cast<T>(x[i]) * static_cast<T>(x[i]);
+  ss = head_sum(ss);
+  return static_cast<T>(rsqrt(ss * static_cast<T>(1.0 / 128) + static_cast<T>(eps)));
+}
+// x * w: a product of two bf16 is exact in fp32.
+__device__ __forceinline__ void times_weight(float (&x)[8], const uint4& w) {
+  float wf[8];
+  unpack8(w, wf);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] *= wf[i];
+}
+
+// Norm and rotation of a head in fp32; cs(k): this lane's k-th pair.
+template <bool HALF, typename F>
+__device__ __forceinline__ void norm_rotate(float (&x)[8], bool norm, const uint4& w, double eps, int rotary_dim, int l16,
+                                            F cs) {
   if (norm) {
-    float wf[8];
-    unpack8(w, wf);
-    T ss = 0;
+    const float r = head_rms<float>(x, eps);
+    times_weight(x, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += static_cast<T>(x[i]) * static_cast<T>(x[i]);
-    ss = head_sum(ss);
-    const T r = static_cast<T>(rsqrt(ss * static_cast<T>(1.0 / 128) + static_cast<T>(eps)));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = static_cast<T>(x[i] * wf[i]) * r;  // a product of two bf16 is exact in fp32
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = x[i];
+    for (int i = 0; i < 8; ++i) x[i] *= r;
   }
   if (rotary_dim == 0) return;
   const bool rot = l16 * 8 < rotary_dim;
   if (HALF) {
-    const int hop = rotary_dim >> 4;  // lanes between an element and its partner
-    const bool low = l16 < hop;
-    const int src = (threadIdx.x & 16) | (!rot ? l16 : (low ? l16 + hop : l16 - hop));
+    const int hop = rotary_dim >> 4;
+    const int src = (threadIdx.x & 16) | (!rot ? l16 : (l16 < hop ? l16 + hop : l16 - hop));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const T z = __shfl_sync(0xffffffffu, y[i], src);
-      const auto c = cs(i);
-      if (rot) y[i] = y[i] * c.x + z * c.y;  // c.y has the sign of the element's half
+      const float z = __shfl_sync(0xffffffffu, x[i], src);
+      const float2 c = cs(i);
+      if (rot) x[i] = x[i] * c.x + z * c.y;  // c.y has the sign of the element's half
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const T a = y[2 * i], b = y[2 * i + 1];
-      const auto c = cs(i);
+      const float a = x[2 * i], b = x[2 * i + 1];
+      const float2 c = cs(i);
       if (rot) {
-        y[2 * i] = a * c.x - b * c.y;
-        y[2 * i + 1] = b * c.x + a * c.y;
+        x[2 * i] = a * c.x - b * c.y;
+        x[2 * i + 1] = b * c.x + a * c.y;
       }
     }
   }
 }
 
-// One 8-bit row: the head's 128 values to codes and exponent.
-template <int FMT, typename T>
-__device__ __forceinline__ void put_row(const T (&y)[8], int l16, bool store, uint8_t* codes, int8_t* exps) {
-  // the largest |y| by its bits (NaNs rank highest)
-  int raw;
-  if constexpr (sizeof(T) == 8) {
-    // the high words, one up where the low word is not zero: the exponent's border has zeros below the high word
-    uint32_t b = 0;
+__device__ __forceinline__ int clamp_exp(int raw) { return max(kKvExpMin, min(kKvExpMax, raw)); }
+// This lane's eight codes and, once a head, the exponent.
+__device__ __forceinline__ void store_row(uint2 c, int raw, int l16, bool store, uint8_t* codes, int8_t* exps) {
+  const bool bad = raw >= (1 << 20);
+  if (store) {
+    *reinterpret_cast<uint2*>(codes) = bad ? make_uint2(0u, 0u) : c;
+    if (l16 == 0) *exps = static_cast<int8_t>(bad ? kKvExpBad : clamp_exp(raw));
+  }
+}
+// An 8-bit v row: the head's bf16 values, scaled exactly, to codes and exponent.
+template <int FMT>
+__device__ __forceinline__ void put_v(const uint4& in, const float (&x)[8], int l16, bool store, uint8_t* codes,
+                                      int8_t* exps) {
+  // the largest |x| by its bits (NaNs rank highest)
+  constexpr uint32_t mag = 0x7fff7fffu;
+  const uint32_t m2 = __vmaxu2(__vmaxu2(in.x & mag, in.y & mag), __vmaxu2(in.z & mag, in.w & mag));
+  const int raw = kv_exp_of<FMT>(static_cast<uint32_t>(head_max(static_cast<int>(max(m2 << 16, m2 & 0xffff0000u)))));
+  const float f = exp2i(-clamp_exp(raw));
+  constexpr float top = FMT == GR_KV_E4M3 ? 448.f : 127.f;
+  float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      b = max(b, (static_cast<uint32_t>(__double2hiint(y[i])) & 0x7fffffffu) + (__double2loint(y[i]) != 0 ? 1u : 0u));
-    raw = kv_exp_of<FMT>(static_cast<long long>(static_cast<unsigned long long>(b) << 32));
+  for (int i = 0; i < 8; ++i) y[i] = x[i] * f;
+  if (raw > kKvExpMax) {  // past the exponents' range: saturate (a bad row's codes are dropped)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = y[i] > top ? top : (y[i] < -top ? -top : y[i]);
+  }
+  store_row(make_uint2(kv_pack<FMT>({y[0], y[1], y[2], y[3]}), kv_pack<FMT>({y[4], y[5], y[6], y[7]})), raw, l16, store,
+            codes, exps);
+}
+// An 8-bit k row: norm, rotation and rounding in fp64.  With a = x w (exact in fp32) and r = 1 / rms the row is r * (a c + z s):
+// the partners z travel as fp32, r goes with 2^-e into one factor, and the sum with the rounding constant (kv8_dev.cuh) is
+// fused with it: one multiplication an element is left of three.
+template <int FMT, bool HALF>
+__device__ __forceinline__ void put_k(float (&a)[8], bool norm, const uint4& w, double eps, int rotary_dim, int l16,
+                                      const double2* cs, bool store, uint8_t* codes, int8_t* exps) {
+  double r = 1.0;
+  if (norm) {
+    r = head_rms<double>(a, eps);
+    times_weight(a, w);
+  }
+  double y[8];
+  if (rotary_dim == 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = a[i];
+  } else if (HALF) {
+    const int hop = rotary_dim >> 4;
+    const int src = (threadIdx.x & 16) | (l16 >= 2 * hop ? l16 : (l16 < hop ? l16 + hop : l16 - hop));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float z = __shfl_sync(0xffffffffu, a[i], src);
+      const double2 c = cs[i * 8];  // c.y has the sign of the element's half
+      y[i] = static_cast<double>(a[i]) * c.x + static_cast<double>(z) * c.y;
+    }
   } else {
-    uint32_t b = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b = max(b, __float_as_uint(y[i]) & 0x7fffffffu);
-    raw = kv_exp_of<FMT>(b);
-  }
-  raw = head_max(raw);
-  const int e = max(kKvExpMin, min(kKvExpMax, raw));
-  T f;
-  if constexpr (sizeof(T) == 8) f = exp2i64(-e);
-  else f = exp2i(-e);
-  T lo[4], hi[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    lo[i] = y[i] * f;
-    hi[i] = y[4 + i] * f;
-  }
-  if (raw > kKvExpMax) {  // past the exponents' range: saturate (a bad row's codes are dropped below)
-    constexpr T top = FMT == GR_KV_E4M3 ? 448 : 127;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      lo[i] = lo[i] > top ? top : (lo[i] < -top ? -top : lo[i]);
-      hi[i] = hi[i] > top ? top : (hi[i] < -top ? -top : hi[i]);
+      const double u = a[2 * i], v = a[2 * i + 1];
+      const double2 c = cs[i * 16];
+      y[2 * i] = u * c.x - v * c.y;
+      y[2 * i + 1] = v * c.x + u * c.y;
     }
   }
-  const bool bad = raw >= (1 << 20);
-  const uint2 c = bad ? make_uint2(0u, 0u) : make_uint2(kv_pack<FMT>(lo), kv_pack<FMT>(hi));
-  if (store) {
-    *reinterpret_cast<uint2*>(codes + l16 * 8) = c;
-    if (l16 == 0) *exps = static_cast<int8_t>(bad ? kKvExpBad : e);
+  // the exponent from the high words; where their next value up would give another one, from the largest |y r| itself
+  int hi = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) hi = max(hi, __double2hiint(y[i]) & 0x7fffffff);
+  hi = head_max(hi);
+  auto exp_of = [](double v) { return max(kv_exp_of<FMT>(__double_as_longlong(fabs(v))), kKvExpMin); };
+  int raw = exp_of(__hiloint2double(hi, 0) * r);
+  if (__any_sync(0xffffffffu, raw != exp_of(__hiloint2double(hi + 1, 0) * r))) {
+    long long m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __double_as_longlong(y[i] * r) & 0x7fffffffffffffffll);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    raw = max(kv_exp_of<FMT>(m), kKvExpMin);
   }
+  const double f = r * exp2i64(-clamp_exp(raw));
+  if (raw > kKvExpMax) {
+    constexpr double top = FMT == GR_KV_E4M3 ? 448 : 127;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = y[i] * f > top ? top / f : (y[i] * f < -top ? -top / f : y[i]);
+  }
+  const uint2 c = make_uint2(kv_pack<FMT>({y[0], y[1], y[2], y[3]}, f), kv_pack<FMT>({y[4], y[5], y[6], y[7]}, f));
+  store_row(c, raw, l16, store, codes, exps);
 }
 
 template <int FMT, bool HALF>
 __global__ void __launch_bounds__(kWriteThreads, 7) qk_norm_rope_write_kernel(const KvWriteParams p) {
-  __shared__ double2 s_cs64[FMT != GR_KV_BF16 ? kWriteThreads / 32 : 1][64];
+  // for k: half-split rotations, with -s for the elements of the first half, and with s
+  __shared__ double2 s_cs64[FMT != GR_KV_BF16 ? kWriteThreads / 32 : 1][HALF ? 2 : 1][64];
   __shared__ float2 s_cs32[kWriteThreads / 32][64];
   if (threadIdx.x == 0) pdl_trigger();
   pdl_wait();
@@ -178,68 +230,85 @@ __global__ void __launch_bounds__(kWriteThreads, 7) qk_norm_rope_write_kernel(co
   uint4 next = make_uint4(0, 0, 0, 0);
   if (g < n_pairs) next = load(g);
 
-  double2* cs64 = s_cs64[FMT != GR_KV_BF16 ? threadIdx.x >> 5 : 0];
+  double2(*cs64)[64] = s_cs64[FMT != GR_KV_BF16 ? threadIdx.x >> 5 : 0];
   float2* cs32 = s_cs32[threadIdx.x >> 5];
-  for (int i = lane; i < (p.rotary_dim >> 1); i += 32) {
-    int pos;
-    if (p.row_pos3) pos = p.row_pos3[row * 3 + (i < p.mrope_s0 ? 0 : (i < p.mrope_s0 + p.mrope_s1 ? 1 : 2))];
-    else pos = p.row_pos[row];
-    // sincospi reduces exactly; the multiplication by 1 / pi is off by 2^-53 of the angle
-    double c, s;
-    sincospi(static_cast<double>(pos) * static_cast<double>(p.inv_freq[i]) * 0.31830988618379067154, &s, &c);
-    if (FMT != GR_KV_BF16) cs64[pair_slot<HALF>(i)] = make_double2(c, s);
-    cs32[pair_slot<HALF>(i)] = make_float2(static_cast<float>(c), static_cast<float>(s));
+  if (p.rotary_dim) {
+#pragma unroll 1
+    for (int i = lane; i < 64; i += 32) {
+      double c = 1.0, s = 0.0;
+      if (i < (p.rotary_dim >> 1)) {
+        int pos;
+        if (p.row_pos3) pos = p.row_pos3[row * 3 + (i < p.mrope_s0 ? 0 : (i < p.mrope_s0 + p.mrope_s1 ? 1 : 2))];
+        else pos = p.row_pos[row];
+        // sincospi reduces exactly; the multiplication by 1 / pi is off by 2^-53 of the angle
+        sincospi(static_cast<double>(pos) * static_cast<double>(p.inv_freq[i]) * 0.31830988618379067154, &s, &c);
+      }
+      const int at = pair_slot<HALF>(i);
+      if (FMT != GR_KV_BF16) {
+        cs64[0][at] = make_double2(c, HALF ? -s : s);
+        if (HALF) cs64[1][at] = make_double2(c, s);
+      }
+      cs32[at] = make_float2(static_cast<float>(c), static_cast<float>(s));
+    }
   }
   uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;
   if (p.q_norm) wq = __ldg(reinterpret_cast<const uint4*>(p.q_norm) + l16);
   if (p.k_norm) wk = __ldg(reinterpret_cast<const uint4*>(p.k_norm) + l16);
   __syncwarp();
   // q's pairs stay in registers, the fp64 ones are read when a k head comes
-  const int hop = p.rotary_dim >> 4;
+  const int hop = p.rotary_dim >> 4, slot0 = lane_slot<HALF>(l16, hop);
   float2 csf[HALF ? 8 : 4];
 #pragma unroll
   for (int k = 0; k < (HALF ? 8 : 4); ++k) {
-    csf[k] = cs32[lane_slot<HALF>(k, l16, hop)];
+    csf[k] = cs32[slot0 + k * (HALF ? 8 : 16)];
     if (HALF && l16 < hop) csf[k].y = -csf[k].y;
   }
   auto cs_f = [&](int k) { return csf[k]; };
-  auto cs_d = [&](int k) {
-    double2 c = cs64[lane_slot<HALF>(k, l16, hop)];
-    if (HALF && l16 < hop) c.y = -c.y;
-    return c;
-  };
+  const double2* cs_d = cs64[HALF && l16 >= hop ? 1 : 0] + slot0;
 
-  const int64_t cache_row = (slot >> 4) * p.n_kv_heads * 16 + (slot & 15);
-  for (int i = g; i < n_pairs; i += p.groups) {
-    float x[8];
-    unpack8(next, x);
+  int i = g;
+  // this lane's values of pair i; the next pair's are on their way
+  auto take = [&](float (&x)[8]) {
+    const uint4 v = next;
+    unpack8(v, x);
     if (i + p.groups < n_pairs) next = load(i + p.groups);
-    if (i < n_qp) {
-      const int h = 2 * i + sub;
-      float y[8];
-      norm_rotate<float, HALF>(x, p.q_norm != nullptr, wq, p.eps, p.rotary_dim, l16, y, cs_f);
-      if (h < p.n_q_heads) store8(p.q_out + (row * p.n_q_heads + h) * 128 + l16 * 8, y);
-      continue;
-    }
-    const bool is_k = i < n_qp + n_kp;
-    const int kvh = 2 * (i - n_qp - (is_k ? 0 : n_kp)) + sub;
-    const bool store = kvh < p.n_kv_heads;
-    const int64_t r = cache_row + kvh * 16;
+    return v;
+  };
+  __nv_bfloat16* q_row = p.q_out + row * p.n_q_heads * 128 + l16 * 8;
+  for (; i < n_qp; i += p.groups) {
+    float x[8];
+    take(x);
+    norm_rotate<HALF>(x, p.q_norm != nullptr, wq, p.eps, p.rotary_dim, l16, cs_f);
+    const int h = 2 * i + sub;
+    if (h < p.n_q_heads) store8(q_row + h * 128, x);
+  }
+  const int64_t cache_row = (slot >> 4) * p.n_kv_heads * 16 + (slot & 15);
+  constexpr int row_bytes = FMT == GR_KV_BF16 ? 256 : 128;
+  uint8_t* k_row = static_cast<uint8_t*>(p.k) + cache_row * row_bytes + l16 * (row_bytes / 16);
+  for (; i < n_qp + n_kp && i < n_pairs; i += p.groups) {
+    float x[8];
+    take(x);
+    const int h = 2 * (i - n_qp) + sub;
+    const bool store = h < p.n_kv_heads;
+    uint8_t* to = k_row + h * 16 * row_bytes;
     if (FMT == GR_KV_BF16) {
-      float y[8];
-      if (is_k) {
-        norm_rotate<float, HALF>(x, p.k_norm != nullptr, wk, p.eps, p.rotary_dim, l16, y, cs_f);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = x[e];
-      }
-      if (store) store8(static_cast<__nv_bfloat16*>(is_k ? p.k : p.v) + r * 128 + l16 * 8, y);
-    } else if (is_k) {
-      double y[8];
-      norm_rotate<double, HALF>(x, p.k_norm != nullptr, wk, p.eps, p.rotary_dim, l16, y, cs_d);
-      put_row<FMT>(y, l16, store, static_cast<uint8_t*>(p.k) + r * 128, p.k_exp + r);
+      norm_rotate<HALF>(x, p.k_norm != nullptr, wk, p.eps, p.rotary_dim, l16, cs_f);
+      if (store) store8(reinterpret_cast<__nv_bfloat16*>(to), x);
     } else {
-      put_row<FMT>(x, l16, store, static_cast<uint8_t*>(p.v) + r * 128, p.v_exp + r);
+      put_k<FMT, HALF>(x, p.k_norm != nullptr, wk, p.eps, p.rotary_dim, l16, cs_d, store, to, p.k_exp + cache_row + h * 16);
+    }
+  }
+  uint8_t* v_row = static_cast<uint8_t*>(p.v) + cache_row * row_bytes + l16 * (row_bytes / 16);
+  for (; i < n_pairs; i += p.groups) {
+    float x[8];
+    const uint4 in8 = take(x);
+    const int h = 2 * (i - n_qp - n_kp) + sub;
+    const bool store = h < p.n_kv_heads;
+    uint8_t* to = v_row + h * 16 * row_bytes;
+    if (FMT == GR_KV_BF16) {
+      if (store) *reinterpret_cast<uint4*>(to) = in8;
+    } else {
+      put_v<FMT>(in8, x, l16, store, to, p.v_exp + cache_row + h * 16);
     }
   }
 }

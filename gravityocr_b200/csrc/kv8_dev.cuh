@@ -63,23 +63,23 @@ __device__ __forceinline__ uint32_t kv_pack(const float (&y)[4]) {
   return low_bytes(__float_as_uint(y[0] + big), __float_as_uint(y[1] + big), __float_as_uint(y[2] + big),
                    __float_as_uint(y[3] + big));
 }
-// The same from fp64 values, rounded once.
+// Four fp64 values times f, rounded once: to the integer with the addition, or to e4m3 by way of fp32 rounded to odd (towards
+// zero, the last bit set where something was cut off), which keeps the second rounding's side.
 template <int FMT>
-__device__ __forceinline__ uint32_t kv_pack(const double (&y)[4]) {
+__device__ __forceinline__ uint32_t kv_pack(const double (&y)[4], double f) {
   if (FMT == GR_KV_E4M3) {
-    float f[4];
+    float o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      // the step of the value's binade: 2^(k - 3), k >= -6 (the subnormal step is 2^-9)
-      const int k = max(((__double2hiint(y[i]) >> 20) & 0x7ff) - 1023, -6);
-      const double c = __hiloint2double(((k - 3 + 52 + 1023) << 20) | 0x80000, 0);
-      f[i] = static_cast<float>(__dsub_rn(__dadd_rn(y[i], c), c));  // exact: a multiple of the step below 2^9
+      const double v = y[i] * f;
+      o[i] = __double2float_rz(v);
+      if (static_cast<double>(o[i]) != v) o[i] = __int_as_float(__float_as_int(o[i]) | 1);
     }
-    return kv_pack<FMT>(f);  // exact: the values are on the grid
+    return kv_pack<FMT>(o);
   }
   constexpr double big = 6755399441055744.0;
-  return low_bytes(__double2loint(__dadd_rn(y[0], big)), __double2loint(__dadd_rn(y[1], big)),
-                   __double2loint(__dadd_rn(y[2], big)), __double2loint(__dadd_rn(y[3], big)));
+  return low_bytes(__double2loint(__fma_rn(y[0], f, big)), __double2loint(__fma_rn(y[1], f, big)),
+                   __double2loint(__fma_rn(y[2], f, big)), __double2loint(__fma_rn(y[3], f, big)));
 }
 
 // Two codes in the low 16 bits -> two halves, exact.
