@@ -10,16 +10,17 @@
 // elements, and the cached codes would then depend on the kernel's operation order.
 // kv_read: rows by slot back to bf16, exact.
 //
-// Measured (16 q and 8 k / v heads, int8, norms, rotation of 128).  Write: 1,088 rows 7 us, 16,496 rows 77 us (237 MB, 3.1
-// TB/s), bound by its instructions: 3,562 a row, 394 of them for the 64-bit angles, 139 for each pair of q heads and 514 for
-// each pair of k heads with its pair of v heads; 71% of the issue slots.  A warp per row keeps angles, norms and maxima
-// within the warp; seven CTAs an SM cover its latencies (six: 82 us).  Read: 66,560 rows 66 us (411 MB, 6.2 TB/s, a copy's
+// Measured (16 q and 8 k / v heads, int8, norms, rotation of 128).  Write: 1,088 rows 7 us, 16,496 rows 55 us (237 MB, 4.3
+// TB/s), bound by its instructions: 2,911 a row, some 500 of them for the 64-bit angles, 115 for each pair of q heads and 371
+// for each pair of k heads with its pair of v heads; 70% of the issue slots.  A warp per row keeps angles, norms and maxima
+// within the warp.  Read: 66,560 rows 66 us (411 MB, 6.2 TB/s, a copy's
 // rate).
 #include "kv8_dev.cuh"
 
 namespace gr {
 
-constexpr int kWriteThreads = 128, kWriteCtas = 7;  // an SM: six 82 us for 16,496 rows, seven 77 (before the prefetch), eight spill
+constexpr int kWriteThreads = 128;
+constexpr int kWriteCtas = 7;  // an SM (16,496 rows without the prefetch: six 68 us, seven 62, eight 62)
 constexpr int kReadThreads = 128;
 constexpr int kReadItems = 4;
 
