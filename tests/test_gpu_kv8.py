@@ -84,6 +84,7 @@ WRITES = [
     (130, "int8", True, 96, True, False, 5, 1), (257, "int8", False, 0, True, False, 2, 2),
     (257, "e4m3", True, 16, True, True, 7, 7), (33, "int8", False, 8, True, True, 3, 1), (1000, "bf16", True, 128, False, False, 16, 2),
     (2500, "int8", False, 128, True, True, 12, 4), (2500, "e4m3", False, 64, True, False, 16, 8),
+    (4401, "int8", True, 64, True, False, 3, 1),   # more rows than run at once
 ]
 
 
@@ -164,6 +165,31 @@ def test_write_special_rows(fmt):
     L.kv_read(L.kv_cache(*cache), c["slots"].to(DEV), out[0], out[1])
     for o in out.cpu():
         assert torch.isnan(o[1:4].float()).all() and torch.isfinite(o[[0, *range(4, 12)]].float()).all()
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_write_k_maxima_next_to_the_exponents_border(fmt, half):
+    """Rotated k rows whose largest value is top 2^j (1 + d): d = 0, and within 10^-5 .. 10^-14 above and below, of both signs."""
+    d = [0.0] + [s * 10.0 ** -n for n in range(5, 15) for s in (1, -1)]
+    m = 2 * len(d)
+    c = _write_case(m, fmt, half, 128, False, False, 2, 2)
+    rows = torch.randn((m, 6, 128), generator=torch.Generator().manual_seed(5))
+    i, j = (0, 64) if half else (0, 1)
+    rows[:, :, i] = R.TOP[fmt] * (2.0 ** (torch.arange(m) % 7 - 3))[:, None]
+    rows[1::2, :, i] *= -1
+    rows[:, :, j] = -rows[:, :, i] / 128                # d moves it by the angle's 128th
+    c["qkv"] = rows.bfloat16().view(m, 768).to(DEV)
+    for k, x in enumerate(d):                            # y_i = x_i cos - x_j sin = x_i (1 + a / 128 - ..): a = 128 d
+        inv = torch.zeros(64)
+        inv[0] = 128 * x
+        c["inv"] = inv
+        c["pos"] = torch.ones(m, dtype=torch.int32)
+        cache = _cache(c["pages"], 2, fmt)
+        _write(c, cache)
+        want, e = R.quantise(_write_ref(c)[1], fmt)
+        assert torch.equal(_rows(cache[2], c["slots"]).long(), e), x
+        assert torch.equal(_rows(cache[0], c["slots"]).double(), want), x
 
 
 def test_write_row_does_not_depend_on_its_batch():
