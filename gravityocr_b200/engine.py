@@ -207,6 +207,7 @@ class Engine:
         self.status = torch.zeros((4,), dtype=torch.int32, device=dev)
         self.lin_ws = torch.zeros((self.linear_ws_bytes(max_rows),), dtype=torch.uint8, device=dev)
         self.attn_ws: Optional[torch.Tensor] = None
+        self._captured_scratch: List[torch.Tensor] = []   # what captured graphs point to: kept when the scratch grows
         self.sms = L.num_sms()
         self.graphs: Dict[Tuple[int, int], torch.cuda.CUDAGraph] = {}
 
@@ -245,8 +246,26 @@ class Engine:
         size = L.kv8_attention_workspace_bytes if self.kv8 else L.attention_workspace_bytes
         need = size(bs, K, self.cfg.n_q_heads, self.cfg.n_kv_heads, splits)
         if self.attn_ws is None or self.attn_ws.numel() < need:
+            if torch.cuda.is_current_stream_capturing():
+                # its zero-fill would be part of the graph, and eager calls before the first replay find other tickets
+                raise RuntimeError(f"attention workspace too small for {bs} x {K} rows in {splits} splits; run the forward "
+                                   "once before capture")
             self.attn_ws = torch.zeros((max(need, 256),), dtype=torch.uint8, device=self.device)
         return self.attn_ws
+
+    def _keep_captured(self, *scratch: Optional[torch.Tensor]) -> None:
+        """Scratch of a forward under capture lives as long as the engine: the graph holds its address, and a later, larger
+        call replaces the engine's own reference."""
+        if torch.cuda.is_current_stream_capturing():
+            for t in scratch:
+                if t is not None and not any(t is u for u in self._captured_scratch):
+                    self._captured_scratch.append(t)
+
+    def _reserve_round(self, rb: RoundBuffers) -> None:
+        """Every scratch buffer of a round over rb, before its capture."""
+        self.reserve(rb.bs * rb.K)
+        if rb.attn_splits > 1:
+            self._attn_workspace(rb.bs, rb.K, rb.attn_splits)
 
     def attention_plan(self, bs: int, K: int, max_len: int, avg_len: int) -> Tuple[int, int]:
         """(chunk, splits) of the attention over up to max_len committed tokens and the K window rows."""
@@ -282,6 +301,7 @@ class Engine:
                      row_pos=self.row_pos, row_slot=self.row_slot, row_ids=self.row_ids, rope_delta=rope_delta,
                      status=st)
         ws_attn = self._attn_workspace(bs, K, attn_splits) if attn_splits > 1 else None
+        self._keep_captured(self.lin_ws, self.y, ws_attn)
         draft = int(rows_mode == L.ROWS_DRAFT) if attn_draft is None else int(attn_draft)
         self._forward_body(rows_mode, bs, K, seq_lens, page_table, out_idx, out_top1, out_gap, attn_chunk,
                            attn_splits, st, head, order, ws_attn, draft, rope_pos3)
@@ -535,6 +555,7 @@ class Engine:
     def capture(self, rb: RoundBuffers, override: bool = False, warmup: int = 0) -> torch.cuda.CUDAGraph:
         """Capture one round (both forwards and the commit) into a CUDA graph; replays read the device-resident
         lengths, seeds and page tables, so one graph serves every round of this (B, batch) bucket."""
+        self._reserve_round(rb)
         g = torch.cuda.CUDAGraph()
         s = torch.cuda.Stream(device=self.device)
         s.wait_stream(torch.cuda.current_stream())
@@ -547,6 +568,7 @@ class Engine:
 
     def capture_split(self, rb: RoundBuffers, override: bool = False) -> Tuple[torch.cuda.CUDAGraph, torch.cuda.CUDAGraph]:
         """Two graphs per (B, batch): the draft forward, and the verify forward + commit (timed separately)."""
+        self._reserve_round(rb)
         gd, gv = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
         s = torch.cuda.Stream(device=self.device)
         s.wait_stream(torch.cuda.current_stream())
