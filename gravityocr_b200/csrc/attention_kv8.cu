@@ -23,7 +23,8 @@
 // P is measured from its own tile's maximum T_r, not the running one: its parts then resolve the tile's weights whatever the
 // rest of the sequence holds (a first token that takes most of the attention would otherwise push every later weight
 // below int8's two digits), and O and l take a tile in fp32 with the factor 2^(T_r - M_r).  M_r is the first tile's maximum,
-// raised only where a tile's is 2^64 above it: fp32 holds the rest, and the sums are hardly ever rescaled.
+// raised only where a tile's is 2^kQRaise above it: fp32 holds the rest, and the sums are hardly ever rescaled.  The largest l: a
+// token adds up to 2^15 (its weight in P's units) 2^40 (2^-ev) 2^48, and a split's 2^13 tokens 2^116 together.
 //
 // CTA: (split, K/V head and block of at most 40 rows, request).  A thread per token (then per dimension) and row group: one
 // group of four warps, or two that share the rows (launch_kv8_attention_f).  One warp issues the MMAs, one the TMA copies (8
@@ -48,6 +49,8 @@ constexpr int kQHalf = kQTile * 128;                        // K or V codes of a
 constexpr int kQStages = 2;                                 // K and V rings (the product barriers are as many)
 constexpr int kQExpStages = 4;                              // tiles' exponents
 constexpr int kQMaxRows = 40;                               // rows of a CTA
+constexpr float kQRaise = 48.f;                             // binades of a tile's maximum above the sums' reference
+static_assert(kKv8MaxChunk <= 1 << 13 && 15 - kKvExpMin + kQRaise + 13 < 127, "the softmax sum stays below 2^127");
 constexpr size_t kQTicketBytes = kKv8TicketPairs * sizeof(int);
 
 // H groups of RH rows, each padded to RP (a multiple of four; the padding has columns, but no arithmetic).  Columns: S has
@@ -540,8 +543,8 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
       bool raised = false;
       if (tid < RT) {
         const float mt = fmaxf(fmaxf(xm[tid], xm[RT + tid]), fmaxf(xm[2 * RT + tid], xm[3 * RT + tid]));
-        // mt = -inf: the row sees no token of this tile.  The sums' reference moves only when a tile is 2^64 above it.
-        raised = mt > m_row + 64.f;
+        // mt = -inf: the row sees no token of this tile.  The sums' reference moves only when a tile is 2^kQRaise above it.
+        raised = mt > m_row + kQRaise;
         alphas[tid] = raised ? ex2_approx(m_row - mt) : 1.f;  // 0 from -inf
         if (raised) m_row = mt;
         betas[tid] = mt == -INFINITY ? 1.f : ex2_approx(mt - m_row);

@@ -1,0 +1,51 @@
+"""8-bit cache attention at the ends of the exponents' range: tiles whose weights 2^(score + exponent) lie far apart, in one chunk
+and across splits, against the 64-bit oracle (scores and bounds as in test_gpu_kv8)."""
+import math
+
+import pytest
+import torch
+
+from oracle import kv8_ref as R
+from test_gpu_kv8 import DEV, DT, _attend, _attn_case, _check_attention, _status
+
+pytestmark = pytest.mark.gpu
+
+
+def _case(fmt, tokens, score):
+    """One request of len(tokens) tokens, one head.  tokens: (0 or 1, e): the key of score 0 or of about `score` (base 2), and a
+    value row of 0.8 top 2^e."""
+    n = len(tokens)
+    c = _attn_case(fmt, [n - 1], 1, 1, 1, spread=0.0)
+    k, v, ke, ve = c["cache"]
+    q = torch.zeros((1, 128))
+    q[0, 0] = score * math.sqrt(128) / (8 * math.log2(math.e))
+    c["q"] = q.bfloat16()
+    slots = c["slots"][0]
+    pages = k.shape[0]
+    rows_k, rows_v = (torch.zeros((pages * 16, 128), dtype=torch.float64) for _ in range(2))
+    loud = torch.tensor([t[0] for t in tokens], dtype=torch.float64)
+    e = torch.tensor([t[1] for t in tokens], dtype=torch.float64)
+    rows_k[slots, 0] = 8 * loud
+    # a row's values differ by dimension (the sign and the size), its largest decides the exponent
+    shape = torch.linspace(-1, 1, 128, dtype=torch.float64)
+    rows_v[slots] = (0.8 * R.TOP[fmt] * 2.0 ** e)[:, None] * shape
+    for rows, codes, exps, name in ((rows_k, k, ke, "k"), (rows_v, v, ve, "v")):
+        qc, ex = R.quantise(rows.view(pages, 1, 16, 128), fmt)
+        codes.copy_(qc.float().to(DT[fmt]))
+        exps.copy_(ex.to(torch.int8))
+        c[name] = R.values(qc, ex).transpose(1, 2).flatten(0, 1)
+    assert ve.cpu().transpose(1, 2).flatten()[slots].tolist() == e.int().tolist()
+    return c
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("score", [60, 87, 103, 130])
+@pytest.mark.parametrize("chunk", [8192, 2048])
+def test_a_sum_of_thousands_of_quiet_rows(fmt, score, chunk):
+    """A first tile of ordinary rows, then thousands of tokens with all the weight and the quietest values (2^-ev = 2^40 each in
+    the softmax sum): the sum stays finite, the output is their mean."""
+    c = _case(fmt, [(0, 0)] * 128 + [(1, -40)] * 7000, score)
+    st = _status()
+    out = _attend(c, chunk=chunk, status=st)
+    assert int(st) == 0
+    _check_attention(c, out)
