@@ -18,7 +18,9 @@
 //   (bf16 rounding of the output is 2^-9 relative.)
 // Scales: a row's q is brought to the parts' range by a factor that coef_r undoes; with a token's 2^ek, 2^ev:
 //   w = s * coef_r * 2^ek + ev (base 2),  p = 2^(w - M_r),  O = sum p code_v,  l = sum p 2^-ev,  out = O / l.
-// |ev| <= 40 keeps l: a token whose p underflows has a score 46 binades below the best.
+// |ev| <= 40 keeps l: a token whose p underflows within a tile, or whose tile lies 2^126 below M_r, has a score at least 46
+// binades below the best.  Sums from before a raise of M_r, and those of other splits, may hold most of l although their weights
+// lie 2^126 below: they are scaled in two steps of half the factor, and joined by l, not by their references.
 //
 // P is measured from its own tile's maximum T_r, not the running one: its parts then resolve the tile's weights whatever the
 // rest of the sequence holds (a first token that takes most of the attention would otherwise push every later weight
@@ -73,7 +75,7 @@ struct KvAttnShape {
   static constexpr int xm = exps + kQExpStages * 2 * kQTile;  // [4][RT] warp maxima of a tile; at the end, the sums l
   static constexpr int coef = xm + RT * 16;                 // [RT] score scale
   static constexpr int ref = coef + RT * 4;                 // [RT] off - T_r
-  static constexpr int alpha = ref + RT * 4;                // [RT] factor of the sums so far
+  static constexpr int alpha = ref + RT * 4;                // [RT] root of the factor of the sums so far
   static constexpr int beta = alpha + RT * 4;               // [RT] factor of the tile's sums
   static constexpr int lim = beta + RT * 4;                 // [RT] row limits
   static constexpr int pages = lim + RT * 4;                // [kKv8MaxChunk / 16] first code row of each page
@@ -166,6 +168,11 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+// The exponent of a softmax sum (2^-33 .. 2^116); 0 for none, and for NaN.
+__device__ __forceinline__ int sum_exp(float l) {
+  const int e = (__float_as_int(l) >> 23 & 0xff) - 127;
+  return e == -127 || e == 128 ? 0 : e;
 }
 __device__ __forceinline__ void named_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
@@ -545,7 +552,7 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
         const float mt = fmaxf(fmaxf(xm[tid], xm[RT + tid]), fmaxf(xm[2 * RT + tid], xm[3 * RT + tid]));
         // mt = -inf: the row sees no token of this tile.  The sums' reference moves only when a tile is 2^kQRaise above it.
         raised = mt > m_row + kQRaise;
-        alphas[tid] = raised ? ex2_approx(m_row - mt) : 1.f;  // 0 from -inf
+        alphas[tid] = raised ? ex2_approx(0.5f * (m_row - mt)) : 1.f;  // 0 from -inf
         if (raised) m_row = mt;
         betas[tid] = mt == -INFINITY ? 1.f : ex2_approx(mt - m_row);
         refs[tid] = off - (mt == -INFINITY ? 0.f : mt);
@@ -554,8 +561,9 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
       if (named_any(1, kSoft, raised)) {
 #pragma unroll
         for (int r = 0; r < RH; ++r) {
-          o[r] *= alphas[rb + r];
-          l[r] *= alphas[rb + r];
+          const float a = alphas[rb + r];
+          o[r] = o[r] * a * a;
+          l[r] = l[r] * a * a;
         }
       }
       // weights; P to shared memory, 16 (part, row) columns of a token in a vector
@@ -678,7 +686,7 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
       float* dst = p.ws_o + ((slot0 + split) * R_all + r0 + grp * RH) * 128 + t128;
 #pragma unroll
       for (int r = 0; r < RH; ++r)
-        if (grp * RH + r < R) __stcg(dst + r * 128, o[r]);
+        if (grp * RH + r < R) __stcg(dst + r * 128, o[r] * exp2i(-sum_exp(xm[rb + r])));
     }
     tc_fence_before();
   }
@@ -707,16 +715,22 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
   float* wgt = reinterpret_cast<float*>(smem + Sh::k);  // [rows][kKv8MaxSplits] weights / sum of the splits
   constexpr int per_warp = (RT + kMmaWarp - 1) / kMmaWarp;
   constexpr int per_lane = kKv8MaxSplits / 32;
+  // A split's softmax sum is y 2^x from its own reference x: with y = f 2^e, 1 <= f < 2, the splits' shares go by x + e, and its O
+  // is stored times 2^-e.
   auto weights = [&](int r, float2 (&x)[per_lane]) {
     float M = -INFINITY, sum = 0.f;
+    int e[per_lane];
 #pragma unroll
-    for (int k = 0; k < per_lane; ++k) M = fmaxf(M, x[k].x);
+    for (int k = 0; k < per_lane; ++k) {
+      e[k] = sum_exp(x[k].y);
+      M = fmaxf(M, x[k].x + static_cast<float>(e[k]));
+    }
     M = warp_max(M);
     if (M == -INFINITY) M = 0.f;
 #pragma unroll
     for (int k = 0; k < per_lane; ++k) {
-      x[k].x = ex2_approx(x[k].x - M);
-      sum += x[k].x * x[k].y;
+      x[k].x = ex2_approx((x[k].x - M) + static_cast<float>(e[k]));
+      sum += x[k].x * (x[k].y * exp2i(-e[k]));
     }
     sum = warp_sum(sum);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;

@@ -49,3 +49,32 @@ def test_a_sum_of_thousands_of_quiet_rows(fmt, score, chunk):
     out = _attend(c, chunk=chunk, status=st)
     assert int(st) == 0
     _check_attention(c, out)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("score", [70, 85, 87, 100, 127, 200])
+@pytest.mark.parametrize("chunk", [8192, 128, 256])
+@pytest.mark.parametrize("order", ["quiet first", "loud first"])
+def test_equal_scores_whose_values_are_80_binades_apart(fmt, score, chunk, order):
+    """Two tokens of the same score, in tiles of their own behind one of score 0: their weights 2^(score + e) are 2^80 apart, the
+    softmax has them equal.  One chunk (the sums' reference rises between them), a split each, and a split that holds the
+    quiet one beside the first tile."""
+    quiet = [(1, -40)] + [(0, -40)] * 127
+    loud = [(1, 40)] + [(0, 0)] * 127
+    first = [(0, 0)] * 128
+    tiles = [first, quiet, loud] if order == "quiet first" else [loud, first, quiet]
+    c = _case(fmt, [t for tile in tiles for t in tile], score)
+    st = _status()
+    out = _attend(c, chunk=chunk, status=st)
+    assert int(st) == 0
+    _check_attention(c, out)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("chunk", [8192, 384])
+def test_many_quiet_tokens_behind_a_raise(fmt, chunk):
+    """A thousand quiet tokens 39 binades below one loud weight hold the softmax sum between them, before and after it."""
+    quiet, loud = [(1, -40)] * 512, [(1, 40)] + [(0, 0)] * 127
+    for tokens in ([(0, 0)] * 128 + quiet + loud + quiet, loud + quiet + [(0, 0)] * 300 + quiet):
+        c = _case(fmt, tokens, 87)
+        _check_attention(c, _attend(c, chunk=chunk))
