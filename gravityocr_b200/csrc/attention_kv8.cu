@@ -53,7 +53,10 @@ constexpr int kQExpStages = 4;                              // tiles' exponents
 constexpr int kQMaxRows = 40;                               // rows of a CTA
 constexpr float kQRaise = 48.f;                             // binades of a tile's maximum above the sums' reference
 static_assert(kKv8MaxChunk <= 1 << 13 && 15 - kKvExpMin + kQRaise + 13 < 127, "the softmax sum stays below 2^127");
-constexpr size_t kQTicketBytes = kKv8TicketPairs * sizeof(int);
+
+// A ticket a (request, K/V head, row block): the fewest blocks that hold the rows, or more of them for at most two CTAs an SM in
+// all.  The same place for every shape: a workspace serves calls of different ones, and only tickets are zero between calls.
+constexpr size_t kQTicketBytes = static_cast<size_t>(kKv8MaxPairs) * ((kKv8MaxRows + kQMaxRows - 1) / kQMaxRows) * sizeof(int);
 
 // H groups of RH rows, each padded to RP (a multiple of four; the padding has columns, but no arithmetic).  Columns: S has
 // part k of a group's row r at group * 2 * RP + k * RP + r, P likewise with every group padded to 16 columns.

@@ -899,20 +899,27 @@ int gr_kv_read(const gr_kv_cache* cache, const int64_t* slots, int64_t n, void* 
                                                                                                   : GR_ERR_CUDA;
 }
 
+// Shapes that the plan, the workspace size and the call take alike; rows: query rows of a K/V head.
+static bool kv8_shape_ok(int bs, int K, int n_q_heads, int n_kv_heads, int* rows) {
+  const int64_t r = static_cast<int64_t>(n_q_heads / n_kv_heads) * K;
+  *rows = static_cast<int>(std::min<int64_t>(r, INT32_MAX));
+  return r <= kKv8MaxRows && static_cast<int64_t>(bs) * n_kv_heads <= kKv8MaxPairs;
+}
+
 size_t gr_kv8_attention_workspace_bytes(int bs, int K, int n_q_heads, int n_kv_heads, int max_splits) {
+  int rows;
   if (bs <= 0 || K <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads || max_splits <= 0 ||
-      static_cast<int64_t>(n_q_heads / n_kv_heads) * K > kKv8MaxRows || max_splits > kKv8MaxSplits ||
-      static_cast<int64_t>(bs) * n_kv_heads > kKv8TicketPairs)
+      max_splits > kKv8MaxSplits || !kv8_shape_ok(bs, K, n_q_heads, n_kv_heads, &rows))
     return 0;
-  return kv8_attention_ws_bytes(bs, n_q_heads / n_kv_heads * K, n_kv_heads, max_splits, nullptr, nullptr);
+  return kv8_attention_ws_bytes(bs, rows, n_kv_heads, max_splits, nullptr, nullptr);
 }
 
 int gr_kv8_attention_plan(int bs, int K, int max_len, int n_q_heads, int n_kv_heads, int32_t* out) {
   if (!out || bs <= 0 || K <= 0 || max_len <= 0 || max_len > kKv8MaxChunk * kKv8MaxSplits || n_kv_heads <= 0 ||
       n_q_heads <= 0 || n_q_heads % n_kv_heads)
     return GR_ERR_ARG;
-  const int64_t rows = static_cast<int64_t>(n_q_heads / n_kv_heads) * K;
-  if (rows > kKv8MaxRows || static_cast<int64_t>(bs) * n_kv_heads > kKv8TicketPairs) return GR_ERR_UNSUPPORTED;
+  int rows;
+  if (!kv8_shape_ok(bs, K, n_q_heads, n_kv_heads, &rows)) return GR_ERR_UNSUPPORTED;
   // The (request, head, row block) triples times the splits of the longest request make about one wave of two CTAs an SM
   // (131,071 tokens of one request: 37 splits 52 us, 55 splits 55 us).  Where the triples alone fill the SMs, lengths are
   // taken to be mixed: pieces of at most 3,200 tokens, shorter where that leaves SMs without a second CTA (64 requests of
@@ -922,7 +929,7 @@ int gr_kv8_attention_plan(int bs, int K, int max_len, int n_q_heads, int n_kv_he
   // part: no less than c = 8 sqrt(length).  One request of 3,000 tokens, 8 window rows: 11 us at 384, 16 at 128; of 16,000:
   // 21 at 1,024, 23 at 512; one row: 9.5 and 9.8, 14 and 13.5.  Whole tiles: 192 takes as long as 256, and joins more.
   int blocks, per_block;
-  kv8_attention_blocks(static_cast<int>(rows), 1, &blocks, &per_block);
+  kv8_attention_blocks(rows, 1, &blocks, &per_block);
   const int64_t units = static_cast<int64_t>(bs) * n_kv_heads * blocks, wave = 2LL * num_sms();
   int64_t chunk = units < num_sms() ? (max_len + wave / units - 1) / (wave / units)
                                     : std::min<int64_t>({3200, max_len, (max_len * units + wave - 1) / wave});
@@ -948,20 +955,18 @@ int gr_kv8_attention(const void* q, const gr_kv_cache* cache, const int32_t* pag
       n_q_heads % cache->n_kv_heads || draft < 0 || draft > 2 || chunk <= 0 || chunk % 32 || chunk > kKv8MaxChunk ||
       max_splits <= 0 || max_splits > kKv8MaxSplits || !aligned(q, 16) || !aligned(out, 16))
     return GR_ERR_ARG;
-  const int64_t rows = static_cast<int64_t>(n_q_heads / cache->n_kv_heads) * K;
-  if (rows > kKv8MaxRows) return GR_ERR_UNSUPPORTED;
+  int rows;
+  if (!kv8_shape_ok(bs, K, n_q_heads, cache->n_kv_heads, &rows) || pt_stride > (INT32_MAX - 8192) / 16)
+    return GR_ERR_UNSUPPORTED;
   const int64_t pairs = static_cast<int64_t>(bs) * cache->n_kv_heads, wave = 2LL * num_sms();
   int blocks, per_block;
-  kv8_attention_blocks(static_cast<int>(rows), pairs > kKv8TicketPairs ? 1 : wave / (pairs * max_splits), &blocks,
-                       &per_block);
-  if (pairs > kKv8TicketPairs / blocks || pt_stride > (INT32_MAX - 8192) / 16)
-    return GR_ERR_UNSUPPORTED;
+  kv8_attention_blocks(rows, wave / (pairs * max_splits), &blocks, &per_block);
   if (static_cast<int64_t>(chunk) * max_splits < K) return GR_ERR_ARG;
   KvAttnParams p;
   std::memset(&p, 0, sizeof(p));
   if (max_splits > 1) {
     size_t o_off, ml_off;
-    const size_t need = kv8_attention_ws_bytes(bs, static_cast<int>(rows), cache->n_kv_heads, max_splits, &o_off, &ml_off);
+    const size_t need = kv8_attention_ws_bytes(bs, rows, cache->n_kv_heads, max_splits, &o_off, &ml_off);
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16)) return GR_ERR_ARG;
     uint8_t* w = static_cast<uint8_t*>(workspace);
     p.ws_ticket = reinterpret_cast<int*>(w);

@@ -270,7 +270,7 @@ size_t kv8_attention_ws_bytes(int bs, int rows, int n_kv_heads, int max_splits, 
 cudaError_t launch_kv8_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, const KvAttnParams& p, int format,
                                  cudaStream_t stream, bool pdl);
 void kv8_attention_blocks(int rows, int64_t room, int* blocks, int* per_block);
-constexpr int kKv8TicketPairs = 16384;  // (request, K/V head, row block) triples of one call
+constexpr int kKv8MaxPairs = 16384;     // (request, K/V head) pairs of one call
 constexpr int kKv8MaxSplits = 128;
 constexpr int kKv8MaxRows = 128;        // query heads of a K/V head times window rows
 constexpr int kKv8MaxSort = 256;       // requests that the attention orders by length

@@ -314,9 +314,10 @@ int gr_kv_read(const gr_kv_cache* cache, const int64_t* slots, int64_t n, void* 
  * (draft 0, 1, 2) and page tables.  K = 1 is one decode token.  A row that sees nothing (seq_lens[b] + base_add + j < 0: a
  * padding request has seq_lens -K - base_add) gives zeros.  Lengths past the page table, and page ids past the cache, set
  * GR_ERR_BAD_PAGE; lengths past chunk * max_splits set GR_ERR_ARG (the rest is not seen).  Query heads per K/V head times K
- * at most 128.  chunk: a multiple of 32, at most 8192; max_splits <= 128; chunk * max_splits >= the longest length + K.
- * workspace: gr_kv8_attention_workspace_bytes (0: a shape that is not supported), zero-filled once (needed for max_splits >
- * 1), one call at a time. */
+ * at most 128, bs times K/V heads at most 16,384 (the plan, the workspace size and the call agree on both).  chunk: a
+ * multiple of 32, at most 8192; max_splits <= 128; chunk * max_splits >= the longest length + K.  workspace:
+ * gr_kv8_attention_workspace_bytes (0: a shape that is not supported), zero-filled once (needed for max_splits > 1), one
+ * call at a time. */
 size_t gr_kv8_attention_workspace_bytes(int bs, int K, int n_q_heads, int n_kv_heads, int max_splits);
 int gr_kv8_attention(const void* q, const gr_kv_cache* cache, const int32_t* page_table, int pt_stride,
                      const int64_t* seq_lens, int bs, int K, int draft, int base_add, int n_q_heads, int chunk,

@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from gravityocr_b200 import _lib as L
 from oracle import kv8_ref as R
 from test_gpu_kv8 import DEV, DT, _attend, _attn_case, _check_attention, _status
 
@@ -78,3 +79,28 @@ def test_many_quiet_tokens_behind_a_raise(fmt, chunk):
     for tokens in ([(0, 0)] * 128 + quiet + loud + quiet, loud + quiet + [(0, 0)] * 300 + quiet):
         c = _case(fmt, tokens, 87)
         _check_attention(c, _attend(c, chunk=chunk))
+
+
+@pytest.mark.parametrize("splits", [1, 2])
+def test_more_row_blocks_than_16384(splits):
+    """600 requests' prompt chunks of 64 rows: 4,800 (request, head) pairs of four row blocks, each with a ticket of its own."""
+    bs, K, nq, nkv = 600, 64, 16, 8
+    c = _attn_case("int8", [0, 60, 17, 1, 40, 5, 33, 58], K, nq, nkv)    # eight different ones, over and over
+    g = torch.Generator().manual_seed(1)
+    lens, slots = c["lens"] * 75, c["slots"] * 75
+    c.update(bs=bs, lens=lens, slots=slots, pt=c["pt"].repeat(75, 1),
+             q=torch.randn((bs * K, nq * 128), generator=g).bfloat16())
+    chunk = 128 // splits
+    ws = torch.zeros((L.kv8_attention_workspace_bytes(bs, K, nq, nkv, splits),), dtype=torch.uint8, device=DEV)
+    st = _status()
+    # a small call first: its partial results lie behind the tickets, whatever the shape
+    small = dict(c, pt=c["pt"][:8].contiguous(), q=c["q"][: 8 * K], lens=lens[:8], slots=slots[:8], bs=8)
+    _check_attention(small, _attend(small, chunk=32, splits=4, ws=ws, status=st))
+    out = _attend(c, chunk=chunk, splits=splits, ws=ws, status=st)
+    again = _attend(c, chunk=chunk, splits=splits, ws=ws, status=st)
+    assert int(st) == 0 and torch.equal(out, again)
+    tickets = 4 * bs * nkv * 4
+    assert int(ws[:tickets].sum()) == 0
+    for b in (0, 1, 300, 555, 599):
+        one = dict(c, pt=c["pt"][b: b + 1].contiguous(), q=c["q"][b * K: (b + 1) * K], lens=[lens[b]], bs=1, slots=slots[b: b + 1])
+        _check_attention(one, out[b * K: (b + 1) * K])
