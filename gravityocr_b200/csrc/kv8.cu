@@ -60,32 +60,33 @@ template <bool HALF>
 __device__ __forceinline__ int lane_slot(int l16, int hop) {
   return HALF ? (l16 < hop ? l16 : (l16 < 2 * hop ? l16 - hop : hop & 7)) : l16;
 }
-// 1 / sqrt(mean x^2 + eps) of a head.
+// mean x^2 + eps of a head.
 template <typename T>
-__device__ __forceinline__ T head_rms(const float (&x)[8], double eps) {
+__device__ __forceinline__ T head_square(const float (&x)[8], double eps) {
   T ss = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ss += static_cast<T>(x[i]) * static_cast<T>(x[i]);
-  ss = head_sum(ss);
-  return static_cast<T>(rsqrt(ss * static_cast<T>(1.0 / 128) + static_cast<T>(eps)));
-}
-// x * w: a product of two bf16 is exact in fp32.
-__device__ __forceinline__ void times_weight(float (&x)[8], const uint4& w) {
-  float wf[8];
-  unpack8(w, wf);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] *= wf[i];
+  return head_sum(ss) * static_cast<T>(1.0 / 128) + static_cast<T>(eps);
 }
 
-// Norm and rotation of a head in fp32; cs(k): this lane's k-th pair.
-template <bool HALF, typename F>
+// Norm and rotation of a head in fp32; cs(k): this lane's k-th pair.  x r stays within sqrt(128) whatever the size of x and w, its
+// squares may not: `odd` where they leave fp32 or its normal numbers (WIDE: a norm in fp64 for such heads).
+template <bool HALF, bool WIDE, typename F>
 __device__ __forceinline__ void norm_rotate(float (&x)[8], bool norm, const uint4& w, double eps, int rotary_dim, int l16,
-                                            F cs) {
+                                            F cs, volatile int* odd) {
   if (norm) {
-    const float r = head_rms<float>(x, eps);
-    times_weight(x, w);
+    float wf[8];
+    unpack8(w, wf);
+    if (WIDE) {
+      const double r = rsqrt(head_square<double>(x, eps));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= r;
+      for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(static_cast<double>(x[i]) * r) * wf[i];
+    } else {
+      const float sq = head_square<float>(x, eps), r = rsqrtf(sq);
+      if (!(sq > 0x1p-100f && sq < 0x1p120f)) *odd = 1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = x[i] * r * wf[i];
+    }
   }
   if (rotary_dim == 0) return;
   const bool rot = l16 * 8 < rotary_dim;
@@ -140,18 +141,9 @@ __device__ __forceinline__ void put_v(const uint4& in, const float (&x)[8], int 
   store_row(make_uint2(kv_pack<FMT>({y[0], y[1], y[2], y[3]}), kv_pack<FMT>({y[4], y[5], y[6], y[7]})), raw, l16, store,
             codes, exps);
 }
-// An 8-bit k row: norm, rotation and rounding in fp64.  With a = x w (exact in fp32) and r = 1 / rms the row is r * (a c + z s):
-// the partners z travel as fp32, r goes with 2^-e into one factor, and the sum with the rounding constant (kv8_dev.cuh) is
-// fused with it: one multiplication an element is left of three.
-template <int FMT, bool HALF>
-__device__ __forceinline__ void put_k(float (&a)[8], bool norm, const uint4& w, double eps, int rotary_dim, int l16,
-                                      const double2* cs, bool store, uint8_t* codes, int8_t* exps) {
-  double r = 1.0;
-  if (norm) {
-    r = head_rms<double>(a, eps);
-    times_weight(a, w);
-  }
-  double y[8];
+// The rotation of a k row in fp64; a: fp32 or fp64.
+template <bool HALF, typename T>
+__device__ __forceinline__ void rotate64(double (&y)[8], const T (&a)[8], int rotary_dim, int l16, const double2* cs) {
   if (rotary_dim == 0) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = a[i];
@@ -160,7 +152,7 @@ __device__ __forceinline__ void put_k(float (&a)[8], bool norm, const uint4& w, 
     const int src = (threadIdx.x & 16) | (l16 >= 2 * hop ? l16 : (l16 < hop ? l16 + hop : l16 - hop));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float z = __shfl_sync(0xffffffffu, a[i], src);
+      const T z = __shfl_sync(0xffffffffu, a[i], src);
       const double2 c = cs[i * 8];  // c.y has the sign of the element's half
       y[i] = static_cast<double>(a[i]) * c.x + static_cast<double>(z) * c.y;
     }
@@ -173,7 +165,11 @@ __device__ __forceinline__ void put_k(float (&a)[8], bool norm, const uint4& w, 
       y[2 * i + 1] = v * c.x + u * c.y;
     }
   }
-  // the exponent from the high words; where their next value up would give another one, from the largest |y r| itself
+}
+// Exponent of the row y r, not clamped from above: from the high words; where their next value up would give another one, from
+// the largest |y r| itself.
+template <int FMT>
+__device__ __forceinline__ int exp_of_row(const double (&y)[8], double r) {
   int hi = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) hi = max(hi, __double2hiint(y[i]) & 0x7fffffff);
@@ -188,6 +184,36 @@ __device__ __forceinline__ void put_k(float (&a)[8], bool norm, const uint4& w, 
     for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     raw = max(kv_exp_of<FMT>(m), kKvExpMin);
   }
+  return raw;
+}
+// An 8-bit k row: norm, rotation and rounding in fp64.  With a = x w and r = 1 / rms the row is r * (a c + z s): a and the
+// partners z are fp32, where a product of two bf16 is exact while it is a normal number; r goes with 2^-e into one factor, and
+// the sum with the rounding constant (kv8_dev.cuh) is fused with it: one multiplication an element is left of three.
+// A product past fp32 gives a bad row, one below its normal numbers is off by 2^-150, which only an r above 2^40 brings near the
+// codes' steps (2^-49 and up): `odd` for such heads (WIDE: fp64 products).
+template <int FMT, bool HALF, bool WIDE>
+__device__ __forceinline__ void put_k(float (&a)[8], bool norm, const uint4& w, double eps, int rotary_dim, int l16,
+                                      const double2* cs, bool store, uint8_t* codes, int8_t* exps, volatile int* odd) {
+  double r = 1.0, y[8];
+  float wf[8];
+  if (norm) {
+    r = rsqrt(head_square<double>(a, eps));
+    unpack8(w, wf);
+  }
+  if (WIDE && norm) {
+    double d[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[i] = static_cast<double>(a[i]) * static_cast<double>(wf[i]);
+    rotate64<HALF>(y, d, rotary_dim, l16, cs);
+  } else {
+    if (norm) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] *= wf[i];
+    }
+    rotate64<HALF>(y, a, rotary_dim, l16, cs);
+  }
+  const int raw = exp_of_row<FMT>(y, r);
+  if (!WIDE && norm && (raw >= (1 << 20) || r > 0x1p40)) *odd = 1;
   const double f = r * exp2i64(-clamp_exp(raw));
   if (raw > kKvExpMax) {
     constexpr double top = FMT == GR_KV_E4M3 ? 448 : 127;
@@ -198,11 +224,62 @@ __device__ __forceinline__ void put_k(float (&a)[8], bool norm, const uint4& w, 
   store_row(c, raw, l16, store, codes, exps);
 }
 
+// This lane's head of pair i, from the row's start (an odd count's last pair has one head: its other half repeats it).  Pairs of
+// heads: n_qp of q, n_kp of k, n_kp of v.
+__device__ __forceinline__ int head_of_pair(const KvWriteParams& p, int i, int n_qp, int n_kp, int sub) {
+  if (i < n_qp) return min(2 * i + sub, p.n_q_heads - 1);
+  i -= n_qp;
+  if (i < n_kp) return p.n_q_heads + min(2 * i + sub, p.n_kv_heads - 1);
+  return p.n_q_heads + p.n_kv_heads + min(2 * (i - n_kp) + sub, p.n_kv_heads - 1);
+}
+
+// A warp's q and k heads once more, with norms in fp64: each lane over what it wrote.  Rare, and out of line behind the warp's
+// loops: within them it costs every row registers (write and read of 16,496 rows 88 us, so 82).
 template <int FMT, bool HALF>
-__global__ void __launch_bounds__(kWriteThreads, kWriteCtas) qk_norm_rope_write_kernel(const KvWriteParams p) {
+__device__ __noinline__ void wide_heads(const KvWriteParams& p, const double2* all64, const float2* all32) {
+  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kWriteThreads + threadIdx.x) >> 5, row = unit / p.groups;
+  const int g = static_cast<int>(unit - row * p.groups);
+  int64_t slot = p.row_slot[row];
+  if (slot >= p.n_slots) slot = -1;
+  const double2* cs64 = all64 + (threadIdx.x >> 5) * (HALF ? 128 : 64);
+  const float2* cs32 = all32 + (threadIdx.x >> 5) * 64;
+  const int l16 = threadIdx.x & 15, sub = (threadIdx.x >> 4) & 1;
+  const int hop = p.rotary_dim >> 4, slot0 = lane_slot<HALF>(l16, hop);
+  const int n_qp = (p.n_q_heads + 1) >> 1, n_kp = slot < 0 ? 0 : (p.n_kv_heads + 1) >> 1;
+  const int64_t cache_row = (slot >> 4) * p.n_kv_heads * 16 + (slot & 15);
+  constexpr int row_bytes = FMT == GR_KV_BF16 ? 256 : 128;
+  auto cs = [&](int k) {
+    float2 c = cs32[slot0 + k * (HALF ? 8 : 16)];
+    if (HALF && l16 < hop) c.y = -c.y;
+    return c;
+  };
+#pragma unroll 1
+  for (int i = g; i < n_qp + n_kp; i += p.groups) {
+    const bool is_q = i < n_qp;
+    const __nv_bfloat16* norm = is_q ? p.q_norm : p.k_norm;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (norm) w = __ldg(reinterpret_cast<const uint4*>(norm) + l16);
+    float x[8];
+    unpack8(__ldg(reinterpret_cast<const uint4*>(p.qkv + row * p.ld_qkv + head_of_pair(p, i, n_qp, n_kp, sub) * 128) + l16), x);
+    const int h = 2 * (is_q ? i : i - n_qp) + sub;
+    const bool store = h < (is_q ? p.n_q_heads : p.n_kv_heads);
+    uint8_t* k_row = static_cast<uint8_t*>(p.k) + (cache_row + h * 16) * row_bytes + l16 * (row_bytes / 16);
+    if (is_q || FMT == GR_KV_BF16) {
+      norm_rotate<HALF, true>(x, norm != nullptr, w, p.eps, p.rotary_dim, l16, cs, nullptr);
+      if (store) store8(is_q ? p.q_out + (row * p.n_q_heads + h) * 128 + l16 * 8 : reinterpret_cast<__nv_bfloat16*>(k_row), x);
+    } else {
+      put_k<FMT, HALF, true>(x, norm != nullptr, w, p.eps, p.rotary_dim, l16, cs64 + (HALF && l16 >= hop ? 64 : 0) + slot0, store,
+                             k_row, p.k_exp + cache_row + h * 16, nullptr);
+    }
+  }
+}
+
+template <int FMT, bool HALF>
+__global__ void __launch_bounds__(kWriteThreads, kWriteCtas) qk_norm_rope_write_kernel(const __grid_constant__ KvWriteParams p) {
   // for k: half-split rotations, with -s for the elements of the first half, and with s
   __shared__ double2 s_cs64[FMT != GR_KV_BF16 ? kWriteThreads / 32 : 1][HALF ? 2 : 1][64];
   __shared__ float2 s_cs32[kWriteThreads / 32][64];
+  __shared__ int s_odd[kWriteThreads / 32];  // a head of the warp's needs its norm in fp64
   if (threadIdx.x == 0) pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31, l16 = lane & 15, sub = lane >> 4;
@@ -220,14 +297,7 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteCtas) qk_norm_rope_write_
   }
   const int n_pairs = slot < 0 ? n_qp : n_qp + 2 * n_kp;
   const __nv_bfloat16* in = p.qkv + row * p.ld_qkv + l16 * 8;
-  // this lane's head of pair i, from the row's start (an odd count's last pair has one head: its other half repeats it)
-  auto head_of = [&](int i) {
-    if (i < n_qp) return min(2 * i + sub, p.n_q_heads - 1);
-    i -= n_qp;
-    if (i < n_kp) return p.n_q_heads + min(2 * i + sub, p.n_kv_heads - 1);
-    return p.n_q_heads + p.n_kv_heads + min(2 * (i - n_kp) + sub, p.n_kv_heads - 1);
-  };
-  auto load = [&](int i) { return __ldg(reinterpret_cast<const uint4*>(in + (even ? 2 * i + sub : head_of(i)) * 128)); };
+  auto load = [&](int i) { return __ldg(reinterpret_cast<const uint4*>(in + (even ? 2 * i + sub : head_of_pair(p, i, n_qp, n_kp, sub)) * 128)); };
   uint4 next = make_uint4(0, 0, 0, 0);
   if (g < n_pairs) next = load(g);
   // More rows than run at once: a row's later heads come to L2 at its start, beside other rows' work (16,496 rows: 55 us, 62
@@ -235,6 +305,8 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteCtas) qk_norm_rope_write_
   if (lane == 0 && p.m > p.sms * kWriteCtas * (kWriteThreads / 32))
     l2_prefetch(p.qkv + row * p.ld_qkv, static_cast<uint32_t>(p.n_q_heads + 2 * p.n_kv_heads) * 256);
 
+  volatile int* odd = s_odd + (threadIdx.x >> 5);
+  if (lane == 0) *odd = 0;
   double2(*cs64)[64] = s_cs64[FMT != GR_KV_BF16 ? threadIdx.x >> 5 : 0];
   float2* cs32 = s_cs32[threadIdx.x >> 5];
   if (p.rotary_dim) {
@@ -283,7 +355,7 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteCtas) qk_norm_rope_write_
   for (; i < n_qp; i += p.groups) {
     float x[8];
     take(x);
-    norm_rotate<HALF>(x, p.q_norm != nullptr, wq, p.eps, p.rotary_dim, l16, cs_f);
+    norm_rotate<HALF, false>(x, p.q_norm != nullptr, wq, p.eps, p.rotary_dim, l16, cs_f, odd);
     const int h = 2 * i + sub;
     if (h < p.n_q_heads) store8(q_row + h * 128, x);
   }
@@ -297,10 +369,11 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteCtas) qk_norm_rope_write_
     const bool store = h < p.n_kv_heads;
     uint8_t* to = k_row + h * 16 * row_bytes;
     if (FMT == GR_KV_BF16) {
-      norm_rotate<HALF>(x, p.k_norm != nullptr, wk, p.eps, p.rotary_dim, l16, cs_f);
+      norm_rotate<HALF, false>(x, p.k_norm != nullptr, wk, p.eps, p.rotary_dim, l16, cs_f, odd);
       if (store) store8(reinterpret_cast<__nv_bfloat16*>(to), x);
     } else {
-      put_k<FMT, HALF>(x, p.k_norm != nullptr, wk, p.eps, p.rotary_dim, l16, cs_d, store, to, p.k_exp + cache_row + h * 16);
+      put_k<FMT, HALF, false>(x, p.k_norm != nullptr, wk, p.eps, p.rotary_dim, l16, cs_d, store, to,
+                              p.k_exp + cache_row + h * 16, odd);
     }
   }
   uint8_t* v_row = static_cast<uint8_t*>(p.v) + cache_row * row_bytes + l16 * (row_bytes / 16);
@@ -316,6 +389,8 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteCtas) qk_norm_rope_write_
       put_v<FMT>(in8, x, l16, store, to, p.v_exp + cache_row + h * 16);
     }
   }
+  __syncwarp();
+  if (s_odd[threadIdx.x >> 5]) wide_heads<FMT, HALF>(p, s_cs64[0][0], s_cs32[0]);
 }
 
 // A warp reads one row's K or V; a lane takes 8 elements (a warp's stores cover whole lines) of kReadItems pairs of heads at a

@@ -1,0 +1,49 @@
+"""8-bit cache write and attention on values far from one: norms whose sums or products leave fp32, query rows of the largest and
+smallest sizes; against the 64-bit oracle, codes equal, outputs within the bounds of test_gpu_kv8."""
+import pytest
+import torch
+
+from gravityocr_b200 import _lib as L
+from oracle import kv8_ref as R
+from test_gpu_kv8 import DEV, _attend, _attn_case, _cache, _check_attention, _close_bf16, _rows, _status
+
+pytestmark = pytest.mark.gpu
+
+# (size of the rows, size of the weights, eps): squares, sums or products beyond fp32 or below its normal numbers
+SIZES = [(1.0, 1.0, 1e-6), (2.0 ** 110, 2.0 ** 30, 1e-6), (2.0 ** 120, 2.0 ** -20, 1e-6), (2.0 ** 66, 1.0, 0.0),
+         (2.0 ** 30, 2.0 ** 100, 1e-6), (2.0 ** -110, 2.0 ** -18, 0.0), (2.0 ** -70, 1.0, 0.0), (2.0 ** -70, 1.0, 1e-6),
+         (2.0 ** -120, 2.0 ** 30, 0.0), (2.0 ** -40, 2.0 ** -20, 0.0), (2.0 ** 62, 2.0 ** 62, 1e-30)]
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("half,rd", [(False, 64), (True, 128), (False, 0)])
+@pytest.mark.parametrize("size,weight,eps", SIZES)
+def test_norms_of_any_size(fmt, half, rd, size, weight, eps):
+    m, nq, nkv = 21, 5, 3
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn((m, (nq + 2 * nkv) * 128), generator=g) * size
+    x[3] = 0.0 if eps else x[3]                         # (0 / 0 otherwise)
+    x[5, ::7] = torch.randn((x.shape[1] + 6) // 7, generator=g)    # two sizes in a row
+    x = x.bfloat16()
+    w = [((1 + 0.2 * torch.randn(128, generator=g)) * weight).bfloat16() for _ in range(2)]
+    w[0][9], w[1][17] = 0.0, 0.0
+    inv = (1.0 / 10000.0 ** (torch.arange(0, rd, 2, dtype=torch.float64) / max(rd, 1))).float()
+    pos = torch.randint(0, 4096, (m,), generator=g, dtype=torch.int32)
+    slots = torch.randperm(64, generator=g)[:m]
+    cache, st = _cache(4, nkv, fmt), _status()
+    q = torch.zeros((m, nq * 128), dtype=torch.bfloat16, device=DEV)
+    L.qk_norm_rope_write(x.to(DEV), nq, L.kv_cache(*cache), slots.to(DEV), q, inv.to(DEV), rd, row_pos=pos.to(DEV),
+                         rope_half=half, q_norm=w[0].to(DEV), k_norm=w[1].to(DEV), eps=eps, status=st)
+    assert int(st) == 0
+    y = x.double().view(m, -1, 128)
+    ang = R.angles(inv, pos) if rd else None
+    rq = R.norm_rotate(y[:, :nq], w[0], eps, ang, half)
+    rk = R.norm_rotate(y[:, nq: nq + nkv], w[1], eps, ang, half)
+    assert torch.isfinite(rq).all() and float(rq.abs().max()) < 1e38
+    _close_bf16(q, rq)
+    if fmt == "bf16":
+        _close_bf16(_rows(cache[0], slots), rk)
+    else:
+        want, e = R.quantise(rk, fmt)
+        assert torch.equal(_rows(cache[2], slots).long(), e)
+        assert torch.equal(_rows(cache[0], slots).double(), want)
