@@ -77,7 +77,7 @@ struct KvAttnShape {
   static constexpr int exps = p + n2 * 128;                 // [kQExpStages][K, V][128]
   static constexpr int xm = exps + kQExpStages * 2 * kQTile;  // [4][RT] warp maxima of a tile; at the end, the sums l
   static constexpr int coef = xm + RT * 16;                 // [RT] score scale
-  static constexpr int ref = coef + RT * 4;                 // [RT] off - T_r
+  static constexpr int ref = coef + RT * 4;                 // [RT] (weights' top) - T_r
   static constexpr int alpha = ref + RT * 4;                // [RT] root of the factor of the sums so far
   static constexpr int beta = alpha + RT * 4;               // [RT] factor of the tile's sums
   static constexpr int lim = beta + RT * 4;                 // [RT] row limits
@@ -165,11 +165,6 @@ __device__ __forceinline__ float warp_max(float v) {
   float r;
   // NaNs are ignored; volatile: every lane has to take part, wherever the result is used
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 // The exponent of a softmax sum (2^-33 .. 2^116); 0 for none, and for NaN.
@@ -490,7 +485,6 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t t_s = t_lane + grp * 2 * RP, t_o = t_lane + Sh::n1 + grp * Sh::p_cols;
     uint8_t* ps = smem + Sh::p + grp * Sh::p_cols * kQTile;
-    constexpr float off = FMT == GR_KV_E4M3 ? 8.f : 14.994309f;  // weights up to 2^8, or 32639 (two digits' largest)
     const int min_lim = min(kv_end, p.draft == 2 ? base + p.K : base + 1);
     float o[RH], l[RH];
 #pragma unroll
@@ -558,7 +552,9 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
         alphas[tid] = raised ? ex2_approx(0.5f * (m_row - mt)) : 1.f;  // 0 from -inf
         if (raised) m_row = mt;
         betas[tid] = mt == -INFINITY ? 1.f : ex2_approx(mt - m_row);
-        refs[tid] = off - (mt == -INFINITY ? 0.f : mt);
+        // e4m3 weights go up to 2^8, which comes with the reference while fp32 holds both (beyond, a score's step is half a binade);
+        // int8's up to 1, brought to the digits as they are rounded
+        refs[tid] = (FMT == GR_KV_E4M3 && fabsf(mt) < 0x1p22f ? 8.f : 0.f) - (mt == -INFINITY ? 0.f : mt);
       }
       __syncwarp();
       if (named_any(1, kSoft, raised)) {
@@ -583,7 +579,6 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
         for (int e = 0; e < 4; ++e) {
           if (r + e >= RH) break;
           x[e] = ex2_approx(w[r + e] + rfs[e]);
-          if (FMT == GR_KV_INT8) x[e] = min_nan(x[e], 32639.f);  // the exponent is rounded: past 32639 the digits would wrap
           // a hidden token's exponent may be that of a bad row, or of no row: its weight is 0, and 2^-ev is finite
           l[r + e] = fmaf(x[e] * unv, bts[e], l[r + e]);
         }
@@ -604,10 +599,11 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
             }
           }
         } else {
-          // two signed digits: the low 16 bits of x + 2^23 + 0x8080 are x + 0x8080, each byte less 0x80 a digit
+          // x to 32639 (two digits' largest) and to two signed digits: the low 16 bits of that + 2^23 + 0x8080 are that + 0x8080, each
+          // byte less 0x80 a digit
           uint32_t t[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) t[k] = __float_as_uint(x[k] + 8421504.f);
+          for (int k = 0; k < 4; ++k) t[k] = __float_as_uint(fmaf(x[k], 32639.f, 8421504.f));
           const uint32_t a = __byte_perm(t[0], t[1], 0x5140), c = __byte_perm(t[2], t[3], 0x5140);  // lo lo hi hi
           pw[r / 4] = __byte_perm(a, c, 0x7632) ^ 0x80808080u;
           pw[(RP + r) / 4] = __byte_perm(a, c, 0x5410) ^ 0x80808080u;
@@ -652,7 +648,7 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
     const int64_t slot0 = (static_cast<int64_t>(b) * p.n_kv_heads + kvh) * p.max_splits;
     float* part = reinterpret_cast<float*>(smem + Sh::k);  // [RT][128]; the last tile's scores are done with the ring
 #pragma unroll
-    for (int r = 0; r < RH; ++r) part[(rb + r) * kQTile + t128] = l[r];
+    for (int r = 0; r < RH; ++r) part[(rb + r) * kQTile + t128] = FMT == GR_KV_INT8 ? l[r] * 32639.f : l[r];  // O's units
     named_sync(1, kSoft);
     {
       constexpr int per_warp = (RT + kMmaWarp - 1) / kMmaWarp;

@@ -47,3 +47,45 @@ def test_norms_of_any_size(fmt, half, rd, size, weight, eps):
         want, e = R.quantise(rk, fmt)
         assert torch.equal(_rows(cache[2], slots).long(), e)
         assert torch.equal(_rows(cache[0], slots).double(), want)
+
+
+def _sized(fmt, K, size, back):
+    """Query rows of size `size`, keys of size 2^back."""
+    c = _attn_case(fmt, [300, 90], K, 4, 2, spread=0.0)
+    ke = c["cache"][2]
+    ke += back
+    assert int(ke.min()) >= -40 and int(ke.max()) <= 40
+    c["k"] = c["k"] * 2.0 ** back
+    q = c["q"].float()
+    c["q"] = (q / q.abs().max() * (1.9 * size)).bfloat16()
+    return c
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("K", [1, 9])
+@pytest.mark.parametrize("size", [2.0 ** -30, 2.0 ** -60, 2.0 ** -110, 2.0 ** -126])
+def test_attention_of_small_query_rows(fmt, K, size):
+    c = _sized(fmt, K, size, 33)
+    _check_attention(c, _attend(c))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("K", [1, 9])
+@pytest.mark.parametrize("size", [2.0 ** n for n in (48, 52, 54, 56, 57, 58, 59, 60, 64, 80)])
+def test_attention_of_large_query_rows(fmt, K, size):
+    """Scores from 10^4 up, where a score's fp32 step passes one, then the weights' whole range: they are finite in fp32, and a row
+    attends to its largest alone (where that is larger by 2^-8 of it, far more than any rounding)."""
+    c = _sized(fmt, K, size, -33)
+    out = _attend(c).double().cpu().view(2, K, 4, 128)
+    for b in range(2):
+        q = c["q"][b * K: (b + 1) * K].double().view(K, 4, 128)
+        k, v = c["k"][c["slots"][b]], c["v"][c["slots"][b]]
+        s = torch.einsum("jhd,thd->jht", q, k.repeat_interleave(2, 1)) / 128 ** 0.5
+        lim = torch.tensor(R.row_limits(0, c["lens"][b], K))
+        s[(torch.arange(k.shape[0])[None] >= lim[:, None])[:, None].expand(s.shape)] = -float("inf")
+        top = torch.topk(s, 2, -1)
+        sure = top.values[..., 0] - top.values[..., 1] > 2.0 ** -8 * top.values[..., 0].abs()
+        assert sure.float().mean() > 0.5                  # of the inputs
+        want = v.repeat_interleave(2, 1).transpose(0, 1)[torch.arange(4)[None], top.indices[..., 0]]
+        err = (out[b] - want).abs()[sure]
+        assert (err <= 2.0 ** -8 * want.abs()[sure] + 2.0 ** -14 * want.abs().amax(-1, keepdim=True).expand(want.shape)[sure]).all()
