@@ -364,12 +364,12 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
       // e4m3: the largest |q| to [2^7, 2^8), exactly; int8: to 32639, two digits' largest, rounded with the digits.  A row
       // with a NaN or an infinity scores NaN.
       if (FMT == GR_KV_E4M3) {
-        const int sh = max(-100, min(100, static_cast<int>(am >> 23) - 127 - 7));
+        const int sh = max(-120, static_cast<int>(am >> 23) - 127 - 7);  // at most 120
         f[u] = exp2i(-sh);
         back[u] = exp2i(sh);
       } else {
         const float a = fmaxf(__uint_as_float(am), 1e-30f);
-        f[u] = __fdividef(32639.f, a) * 0.9999995f;  // not above 32639 after its rounding
+        f[u] = 32639.f / a * 0.9999995f;  // not above 32639 after its rounding
         back[u] = 1.f / f[u];
       }
       if (am >= 0x7f800000u) {

@@ -312,7 +312,7 @@ int gr_kv_read(const gr_kv_cache* cache, const int64_t* slots, int64_t n, void* 
 
 /* gr_bd_attention over an 8-bit cache (GR_KV_BF16 is GR_ERR_UNSUPPORTED: gr_bd_attention reads that): the same rows, masks
  * (draft 0, 1, 2) and page tables.  K = 1 is one decode token.  A row that sees nothing (seq_lens[b] + base_add + j < 0: a
- * padding request has seq_lens -K - base_add) gives zeros.  Lengths past the page table, and page ids past the cache, set
+ * padding request has seq_lens -K - base_add) gives zeros; one with a score past fp32, or that sees a bad row, gives NaN.  Lengths past the page table, and page ids past the cache, set
  * GR_ERR_BAD_PAGE; lengths past chunk * max_splits set GR_ERR_ARG (the rest is not seen).  Query heads per K/V head times K
  * at most 128, bs times K/V heads at most 16,384 (the plan, the workspace size and the call agree on both).  chunk: a
  * multiple of 32, at most 8192; max_splits <= 128; chunk * max_splits >= the longest length + K.  workspace:

@@ -89,3 +89,11 @@ def test_attention_of_large_query_rows(fmt, K, size):
         want = v.repeat_interleave(2, 1).transpose(0, 1)[torch.arange(4)[None], top.indices[..., 0]]
         err = (out[b] - want).abs()[sure]
         assert (err <= 2.0 ** -8 * want.abs()[sure] + 2.0 ** -14 * want.abs().amax(-1, keepdim=True).expand(want.shape)[sure]).all()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("K", [1, 9])
+@pytest.mark.parametrize("size", [2.0 ** 100, 2.0 ** 107, 2.0 ** 110, 2.0 ** 125, 2.0 ** 126, 2.0 ** 127])
+def test_attention_of_the_largest_query_rows(fmt, K, size):
+    """Up to bf16's largest number."""
+    test_attention_of_large_query_rows(fmt, K, size)
