@@ -39,7 +39,7 @@ struct LpState {
 
 // e^{(a - b) / T} with a <= b; 0 for a = -inf.  k = log2(e) / T.
 __device__ __forceinline__ float lp_shift(float a, float b, float k, float& d) {
-  d = fmaxf((a - b) * k, -1e30f);  // -1e30 instead of -inf: d * 0 stays 0
+  d = fmaxf((a - b) * k, -1e20f);  // -1e20 instead of -inf: times any sum it stays a number
   return ex2_approx(d);
 }
 __device__ __forceinline__ LpState lp_join(const LpState& a, const LpState& b, float k) {
@@ -173,7 +173,7 @@ __device__ __forceinline__ void lp_move(float& S, float& W, float ref, float to,
   S *= f;
 }
 __device__ __forceinline__ void lp_add(float x, float ref, float k, float& S, float& W) {
-  const float d = max_nan((x - ref) * k, -1e30f);  // a masked token: e = 0, and e d = 0 stays a number
+  const float d = max_nan((x - ref) * k, -1e20f);  // a masked token: e = 0, and e d = 0 stays a number
   const float e = ex2_approx(d);
   S += e;
   W = fmaf(e, d, W);
@@ -210,8 +210,8 @@ __device__ __forceinline__ float lp_batch(LpThread& t, const uint4 (&raw)[LpVec<
     for (int i = 0; i < V::N; i += 2) {
       float d0, d1;
       f2_unpack(f2_mul(f2_add(f2_pack(V::get(raw[u], i), V::get(raw[u], i + 1)), minus), kk), d0, d1);
-      d0 = max_nan(d0, -1e30f);  // a masked token: e = 0, and e d = 0 stays a number
-      d1 = max_nan(d1, -1e30f);
+      d0 = max_nan(d0, -1e20f);  // a masked token: e = 0, and e d = 0 stays a number
+      d1 = max_nan(d1, -1e20f);
       const uint64_t e = f2_pack(ex2_approx(d0), ex2_approx(d1));
       S2 = f2_add(S2, e);
       W2 = f2_fma(e, f2_pack(d0, d1), W2);
