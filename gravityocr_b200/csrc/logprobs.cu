@@ -304,7 +304,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const Log
     for (int u = 0; u < V::B; ++u) next[u] = __ldg(vec + v_beg + tid + u * NT);
   }
   const float temp = p.temperature ? p.temperature[row] : 1.f;
-  const float k = 1.4426950408889634f / temp;
+  const bool warm = temp >= 0x1p-126f;  // (log2(e) / T is finite for normal T)
+  const float k = fmaxf(1.4426950408889634f / temp, 1e-45f);  // above 0 for T = inf, too: a masked token's -inf stays -inf
   const int64_t want = p.ids[row];
   const bool asked = want >= 0 && want < p.vocab;
   const int my_id = asked ? static_cast<int>(want) : -1;
@@ -506,21 +507,22 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const Log
     before += static_cast<int>(b >> 32);
     s = lp_join(s, x, k);
   }
-  const bool ok = s.m > -INFINITY && s.m < INFINITY && s.R == s.R && temp > 0.f;
+  const bool ok = s.m > -INFINITY && s.m < INFINITY && s.R == s.R && warm;
   const float lse = log1pf(s.R);
   const float nan = __int_as_float(0x7fc00000);
+  auto log_p = [&](float x) { return x == -INFINITY ? x : (x - s.m) / temp - lse; };
   if (tid == 0) {
     const bool known = ok && asked;
-    p.logprob[row] = known ? (mine - s.m) / temp - lse : nan;
+    p.logprob[row] = known ? log_p(mine) : nan;
     p.rank[row] = known ? before + 1 : 0;
     p.entropy[row] = ok ? lse - s.W * 0.69314718055994531f / (1.f + s.R) : nan;
-    if (!ok) report(p.status, temp > 0.f ? GR_ERR_NO_TOKEN : GR_ERR_ARG);
+    if (!ok) report(p.status, warm ? GR_ERR_NO_TOKEN : GR_ERR_ARG);
     else if (!asked && want != -1) report(p.status, GR_ERR_BAD_ID);
   }
   float* top = p.top_logprob + row * n;
   int32_t* top_ids = p.top_ids + row * n;
   auto put_top = [&](int at, uint64_t key) {
-    top[at] = ok ? (lp_key_logit(key) - s.m) / temp - lse : nan;
+    top[at] = ok ? log_p(lp_key_logit(key)) : nan;
     top_ids[at] = ok ? lp_key_id(key) : -1;
   };
   if (ctas == 1) {

@@ -312,12 +312,12 @@ int gr_kv_read(const gr_kv_cache* cache, const int64_t* slots, int64_t n, void* 
 
 /* gr_bd_attention over an 8-bit cache (GR_KV_BF16 is GR_ERR_UNSUPPORTED: gr_bd_attention reads that): the same rows, masks
  * (draft 0, 1, 2) and page tables.  K = 1 is one decode token.  A row that sees nothing (seq_lens[b] + base_add + j < 0: a
- * padding request has seq_lens -K - base_add) gives zeros; one with a score past fp32, or that sees a bad row, gives NaN.  Lengths past the page table, and page ids past the cache, set
- * GR_ERR_BAD_PAGE; lengths past chunk * max_splits set GR_ERR_ARG (the rest is not seen).  Query heads per K/V head times K
- * at most 128, bs times K/V heads at most 16,384 (the plan, the workspace size and the call agree on both).  chunk: a
- * multiple of 32, at most 8192; max_splits <= 128; chunk * max_splits >= the longest length + K.  workspace:
- * gr_kv8_attention_workspace_bytes (0: a shape that is not supported), zero-filled once (needed for max_splits > 1), one
- * call at a time. */
+ * padding request has seq_lens -K - base_add) gives zeros; one with a score past fp32, or that sees a bad row, gives NaN.
+ * Lengths past the page table, and page ids past the cache, set GR_ERR_BAD_PAGE; lengths past chunk * max_splits set
+ * GR_ERR_ARG (the rest is not seen).  Query heads per K/V head times K at most 128, bs times K/V heads at most 16,384 (the
+ * plan, the workspace size and the call agree on both).  chunk: a multiple of 32, at most 8192; max_splits <= 128; chunk *
+ * max_splits >= the longest length + K.  workspace: gr_kv8_attention_workspace_bytes (0: a shape that is not supported),
+ * zero-filled once (needed for max_splits > 1), one call at a time. */
 size_t gr_kv8_attention_workspace_bytes(int bs, int K, int n_q_heads, int n_kv_heads, int max_splits);
 int gr_kv8_attention(const void* q, const gr_kv_cache* cache, const int32_t* page_table, int pt_stride,
                      const int64_t* seq_lens, int bs, int K, int draft, int base_add, int n_q_heads, int chunk,
@@ -327,10 +327,11 @@ int gr_kv8_attention_plan(int bs, int K, int max_len, int n_q_heads, int n_kv_he
 
 /* Log probabilities of ids [rows] under softmax(logits / temperature): logprob [rows], rank [rows] (1 + the tokens that come
  * before it, by logit, then by id), entropy [rows] (nats), and the n_top (0..64, <= vocab) best tokens, equal logits by id:
- * top_logprob / top_ids [rows, n_top].  logits: fp32, or bf16 when is_bf16, [rows, ld], ld >= vocab; temperature [rows] > 0,
- * or NULL for 1.  -inf logits (masked tokens) have probability 0.  id -1: no token asked (NaN, rank 0); any other id outside
+ * top_logprob / top_ids [rows, n_top].  logits: fp32, or bf16 when is_bf16, [rows, ld], ld >= vocab; temperature [rows], at
+ * least 2^-126, inf for the uniform distribution, or NULL for 1.  -inf logits (masked tokens), and those further below the
+ * largest than fp32's largest number, have probability 0.  id -1: no token asked (NaN, rank 0); any other id outside
  * the vocabulary sets GR_ERR_BAD_ID.  A row with a NaN or +inf logit, or with every logit -inf, has no distribution: its
- * outputs are NaN, rank 0, ids -1, and GR_ERR_NO_TOKEN is set; a temperature that is not > 0 gives the same with GR_ERR_ARG.
+ * outputs are NaN, rank 0, ids -1, and GR_ERR_NO_TOKEN is set; a temperature below 2^-126 or NaN gives the same with GR_ERR_ARG.
  * The reference refuses requests that ask for log probabilities. */
 int gr_token_logprobs(const void* logits, int is_bf16, int64_t ld, int rows, int vocab, const int64_t* ids,
                       const float* temperature, int n_top, float* logprob, float* entropy, int32_t* rank,
