@@ -3,8 +3,9 @@
     python -m gravityocr_b200.build [--verbose] [--ptxas-info] [--timeline]
 
 Objects go to ``gravityocr_b200/_build/``; the shared library lands next to this file, where ``_lib.py`` loads it.
-``--timeline`` builds ``libgravity_b200_timeline.so`` instead: the same kernels compiled with ``-DGR_TIMELINE``, which
-record per-CTA globaltimer stamps for ``bench.py case timeline`` (load it with ``GRAVITY_B200_LIB``).
+``--timeline`` builds ``libgravity_b200_timeline.so`` instead: the same kernels compiled with ``-DGR_TIMELINE``; those of
+a bf16 round (not the 8-bit cache's and the log probabilities') record per-CTA globaltimer stamps for ``bench.py case
+timeline`` (load it with ``GRAVITY_B200_LIB``).
 The CUDA runtime is linked shared so the library uses the same runtime (current device, streams) as PyTorch.
 """
 from __future__ import annotations

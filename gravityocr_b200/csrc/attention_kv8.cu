@@ -36,8 +36,8 @@
 // latencies.
 //
 // Measured (8 K/V heads of 2 query heads).  One row: 131,071 tokens of one request 50 us, 283 MB, 5.6 TB/s, where a plain
-// sum of as many bytes takes 49.5; 64 requests of 288-4,128 tokens 53 us (291 MB): bound by the memory.  17 rows of these 64:
-// 99 us int8, 115 e4m3, bound by the softmax threads: their instructions fill half of the issue slots, and a tile's chain
+// sum of as many bytes takes 49.5; 64 requests of 288-4,128 tokens 54 us (291 MB): bound by the memory.  17 rows of these 64:
+// 100 us int8, 116 e4m3, bound by the softmax threads: their instructions fill half of the issue slots, and a tile's chain
 // (scores, maxima, weights, P, O) the time between.
 #include <algorithm>
 #include <type_traits>

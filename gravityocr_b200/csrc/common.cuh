@@ -43,7 +43,7 @@ __device__ __forceinline__ void report(int* status, int code) {
 }
 
 // ------------------------------------------------------------------ launch timeline (timeline build only)
-// Built with -DGR_TIMELINE (python -m gravityocr_b200.build --timeline): thread 0 of every CTA of every round kernel
+// Built with -DGR_TIMELINE (python -m gravityocr_b200.build --timeline): thread 0 of every CTA of a bf16 round's kernels
 // appends (kind, block, entry, exit) globaltimer stamps to its translation unit's record array, and a (0, block, t, t)
 // record when griddepcontrol.wait returns; the host reads them with gr_timeline_read_<unit>.  This shows each
 // launch's dependency release and its CTAs' critical path as the graphs replay, which a serialising profiler does

@@ -10,17 +10,17 @@
 // elements, and the cached codes would then depend on the kernel's operation order.
 // kv_read: rows by slot back to bf16, exact.
 //
-// Measured (16 q and 8 k / v heads, int8, norms, rotation of 128).  Write: 1,088 rows 7 us, 16,496 rows 55 us (237 MB, 4.3
-// TB/s), bound by its instructions: 2,911 a row, some 500 of them for the 64-bit angles, 115 for each pair of q heads and 371
-// for each pair of k heads with its pair of v heads; 70% of the issue slots.  A warp per row keeps angles, norms and maxima
-// within the warp.  Read: 66,560 rows 66 us (411 MB, 6.2 TB/s, a copy's
-// rate).
+// Measured (16 q and 8 k / v heads, int8, norms, rotation of 128; launches one behind the other in a graph, on inputs in turn).
+// Write: one row 2.5 us, 1,088 rows 7.7, 16,496 rows 65 (237 MB, 3.7 TB/s; e4m3 67, a bf16 cache 52), bound by its
+// instructions: 3,010 a row, some 500 of them for the 64-bit angles, 120 for each pair of q heads and 380 for each pair of k heads
+// with its pair of v heads; 71% of the issue slots.  A warp per row keeps angles, norms and maxima within the warp; at 1,088
+// rows three warps share a row, each with all of its angles.  Read: 66,560 rows 66 us (411 MB, 6.2 TB/s, a copy's rate).
 #include "kv8_dev.cuh"
 
 namespace gr {
 
 constexpr int kWriteThreads = 128;
-constexpr int kWriteCtas = 7;  // an SM (16,496 rows without the prefetch: six 68 us, seven 62, eight 62)
+constexpr int kWriteCtas = 7;  // an SM (16,496 rows: six 68 us, seven 65, eight 67)
 constexpr int kReadThreads = 128;
 constexpr int kReadItems = 4;
 
@@ -300,8 +300,8 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteCtas) qk_norm_rope_write_
   auto load = [&](int i) { return __ldg(reinterpret_cast<const uint4*>(in + (even ? 2 * i + sub : head_of_pair(p, i, n_qp, n_kp, sub)) * 128)); };
   uint4 next = make_uint4(0, 0, 0, 0);
   if (g < n_pairs) next = load(g);
-  // More rows than run at once: a row's later heads come to L2 at its start, beside other rows' work (16,496 rows: 55 us, 62
-  // without).  A single wave only asks for everything at the same time (4,000 rows: 18.4 us, 17.7 without).
+  // More rows than run at once: a row's later heads come to L2 at its start, beside other rows' work (16,496 rows: 65 us, 68
+  // without).  A single wave only asks for everything at the same time (4,000 rows: 20.7 us, 19.9 without).
   if (lane == 0 && p.m > p.sms * kWriteCtas * (kWriteThreads / 32))
     l2_prefetch(p.qkv + row * p.ld_qkv, static_cast<uint32_t>(p.n_q_heads + 2 * p.n_kv_heads) * 256);
 

@@ -15,8 +15,9 @@
 // logits of 64 groups of threads bounds the row's n-th best from below, so only cells that reach the bound are read
 // again, and what is found above it is ranked by counting.  (Cells, not threads, because 592 rows in flight outgrow the L2:
 // reading every such thread's logits again cost 20% more DRAM traffic.)
-// Bound: reading the row (1,088 rows of 59,392 fp32 logits, the 20 best: 52 us, 258 MB, 5.0 TB/s; bf16: 46 us, by its
-// instructions).  Few rows (64 bf16: 12 us, one: 9) wait for the chain of phases: stream, maxima, bound, cells, ranks.  They
+// Bound: reading the row (1,088 rows of 59,392 fp32 logits, the 20 best: 51 us, 55 on another machine; 258 MB, 5.0 TB/s; bf16:
+// 45 us, by its instructions).  Rows with fewer tokens than alternatives are slow: every masked token is a candidate (three of
+// 59,392 left, the 20 best: one row 64 us, 1,088 rows 446).  Few rows (64 bf16: 12 us, one: 9) wait for the chain of phases: stream, maxima, bound, cells, ranks.  They
 // are shared between the CTAs of a cluster, whose states, counts and best lists the first one joins through distributed
 // shared memory.
 #include <type_traits>

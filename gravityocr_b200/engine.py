@@ -269,7 +269,7 @@ class Engine:
 
     def attention_plan(self, bs: int, K: int, max_len: int, avg_len: int) -> Tuple[int, int]:
         """(chunk, splits) of the attention over up to max_len committed tokens and the K window rows."""
-        if self.kv8:
+        if self.kv8:  # for the longest request the buffers hold: a graph serves every length up to it
             return L.kv8_attention_split(bs, K, max_len + K + 1, self.cfg.n_q_heads, self.cfg.n_kv_heads)
         return attention_split(bs, K, max_len, avg_len, self.cfg.n_kv_heads, self.sms)
 
@@ -374,7 +374,9 @@ class Engine:
 
     def _qkv_attention_8bit(self, l, d, bs, K, seq_lens, page_table, attn_chunk, attn_splits, st, ws_attn, draft, base_add,
                             rope_pos3) -> None:
-        """Layer l's projection, rotation with the quantised cache write, and attention over the 8-bit cache."""
+        """Layer l's projection, rotation with the quantised cache write, and attention over the 8-bit cache.  The projected rows
+        are rounded to bf16 on their way (the write is a kernel of its own, and a cached row a function of them alone), q once
+        more after its rotation; the bf16 engine rotates the projection's fp32 accumulators."""
         cfg, M = self.cfg, bs * K
         e = L.Epilogue()
         e.mode = L.EPI_STORE_BF16
