@@ -19,14 +19,14 @@
 // Scales: a row's q is brought to the parts' range by a factor that coef_r undoes; with a token's 2^ek, 2^ev:
 //   w = s * coef_r * 2^ek + ev (base 2),  p = 2^(w - M_r),  O = sum p code_v,  l = sum p 2^-ev,  out = O / l.
 // |ev| <= 40 keeps l: a token whose p underflows within a tile, or whose tile lies 2^126 below M_r, has a score at least 46
-// binades below the best.  Sums from before a raise of M_r, and those of other splits, may hold most of l although their weights
-// lie 2^126 below: they are scaled in two steps of half the factor, and joined by l, not by their references.
+// binades below the best.  Sums from before a raise of M_r, and those of other splits, may hold most of l although their
+// weights lie 2^126 below: they are scaled in two steps of half the factor, and joined by l, not by their references.
 //
 // P is measured from its own tile's maximum T_r, not the running one: its parts then resolve the tile's weights whatever the
 // rest of the sequence holds (a first token that takes most of the attention would otherwise push every later weight
 // below int8's two digits), and O and l take a tile in fp32 with the factor 2^(T_r - M_r).  M_r is the first tile's maximum,
-// raised only where a tile's is 2^kQRaise above it: fp32 holds the rest, and the sums are hardly ever rescaled.  The largest l: a
-// token adds up to 2^15 (its weight in P's units) 2^40 (2^-ev) 2^48, and a split's 2^13 tokens 2^116 together.
+// raised only where a tile's is 2^kQRaise above it: fp32 holds the rest, and the sums are hardly ever rescaled.  The largest
+// l: a token adds up to 2^15 (its weight in P's units) 2^40 (2^-ev) 2^48, and a split's 2^13 tokens 2^116 together.
 //
 // CTA: (split, K/V head and block of at most 40 rows, request).  A thread per token (then per dimension) and row group: one
 // group of four warps, or two that share the rows (launch_kv8_attention_f).  One warp issues the MMAs, one the TMA copies (8
@@ -54,8 +54,8 @@ constexpr int kQMaxRows = 40;                               // rows of a CTA
 constexpr float kQRaise = 48.f;                             // binades of a tile's maximum above the sums' reference
 static_assert(kKv8MaxChunk <= 1 << 13 && 15 - kKvExpMin + kQRaise + 13 < 127, "the softmax sum stays below 2^127");
 
-// A ticket a (request, K/V head, row block): the fewest blocks that hold the rows, or more of them for at most two CTAs an SM in
-// all.  The same place for every shape: a workspace serves calls of different ones, and only tickets are zero between calls.
+// A ticket a (request, K/V head, row block): the fewest blocks that hold the rows, or more of them for at most two CTAs an SM
+// in all.  The same place for every shape: a workspace serves calls of different ones, and only tickets are zero between calls.
 constexpr size_t kQTicketBytes = static_cast<size_t>(kKv8MaxPairs) * ((kKv8MaxRows + kQMaxRows - 1) / kQMaxRows) * sizeof(int);
 
 // H groups of RH rows, each padded to RP (a multiple of four; the padding has columns, but no arithmetic).  Columns: S has
@@ -552,8 +552,8 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
         alphas[tid] = raised ? ex2_approx(0.5f * (m_row - mt)) : 1.f;  // 0 from -inf
         if (raised) m_row = mt;
         betas[tid] = mt == -INFINITY ? 1.f : ex2_approx(mt - m_row);
-        // e4m3 weights go up to 2^8, which comes with the reference while fp32 holds both (beyond, a score's step is half a binade);
-        // int8's up to 1, brought to the digits as they are rounded
+        // e4m3 weights go up to 2^8, which comes with the reference while fp32 holds both (beyond, a score's step is half a
+        // binade); int8's up to 1, brought to the digits as they are rounded
         refs[tid] = (FMT == GR_KV_E4M3 && fabsf(mt) < 0x1p22f ? 8.f : 0.f) - (mt == -INFINITY ? 0.f : mt);
       }
       __syncwarp();
@@ -599,8 +599,8 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
             }
           }
         } else {
-          // x to 32639 (two digits' largest) and to two signed digits: the low 16 bits of that + 2^23 + 0x8080 are that + 0x8080, each
-          // byte less 0x80 a digit
+          // x times 32639 (two digits' largest) to two signed digits: the low 16 bits of that + 2^23 + 0x8080 are that + 0x8080,
+          // each byte less 0x80 a digit
           uint32_t t[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) t[k] = __float_as_uint(fmaf(x[k], 32639.f, 8421504.f));
@@ -714,8 +714,8 @@ __global__ void __launch_bounds__(128 * H + 64, H == 2 ? 2 : 3) kv8_attention_ke
   float* wgt = reinterpret_cast<float*>(smem + Sh::k);  // [rows][kKv8MaxSplits] weights / sum of the splits
   constexpr int per_warp = (RT + kMmaWarp - 1) / kMmaWarp;
   constexpr int per_lane = kKv8MaxSplits / 32;
-  // A split's softmax sum is y 2^x from its own reference x: with y = f 2^e, 1 <= f < 2, the splits' shares go by x + e, and its O
-  // is stored times 2^-e.
+  // A split's softmax sum is y 2^x from its own reference x: with y = f 2^e, 1 <= f < 2, the splits' shares go by x + e, and its
+  // O is stored times 2^-e.
   auto weights = [&](int r, float2 (&x)[per_lane]) {
     float M = -INFINITY, sum = 0.f;
     int e[per_lane];

@@ -12,9 +12,9 @@
 //
 // Measured (16 q and 8 k / v heads, int8, norms, rotation of 128; launches one behind the other in a graph, on inputs in turn).
 // Write: one row 2.5 us, 1,088 rows 7.7, 16,496 rows 65 (237 MB, 3.7 TB/s; e4m3 67, a bf16 cache 52), bound by its
-// instructions: 3,010 a row, some 500 of them for the 64-bit angles, 120 for each pair of q heads and 380 for each pair of k heads
-// with its pair of v heads; 71% of the issue slots.  A warp per row keeps angles, norms and maxima within the warp; at 1,088
-// rows three warps share a row, each with all of its angles.  Read: 66,560 rows 66 us (411 MB, 6.2 TB/s, a copy's rate).
+// instructions: 3,010 a row, some 500 of them for the 64-bit angles, 120 for each pair of q heads and 380 for each pair of k
+// heads with its pair of v heads; 71% of the issue slots.  A warp per row keeps angles, norms and maxima within the warp; at
+// 1,088 rows three warps share a row, each with all of its angles.  Read: 66,560 rows 66 us (411 MB, 6.2 TB/s, a copy's rate).
 #include "kv8_dev.cuh"
 
 namespace gr {
@@ -69,8 +69,8 @@ __device__ __forceinline__ T head_square(const float (&x)[8], double eps) {
   return head_sum(ss) * static_cast<T>(1.0 / 128) + static_cast<T>(eps);
 }
 
-// Norm and rotation of a head in fp32; cs(k): this lane's k-th pair.  x r stays within sqrt(128) whatever the size of x and w, its
-// squares may not: `odd` where they leave fp32 or its normal numbers (WIDE: a norm in fp64 for such heads).
+// Norm and rotation of a head in fp32; cs(k): this lane's k-th pair.  x r stays within sqrt(128) whatever the size of x and w,
+// its squares may not: `odd` where they leave fp32 or its normal numbers (WIDE: a norm in fp64 for such heads).
 template <bool HALF, bool WIDE, typename F>
 __device__ __forceinline__ void norm_rotate(float (&x)[8], bool norm, const uint4& w, double eps, int rotary_dim, int l16,
                                             F cs, volatile int* odd) {
@@ -189,8 +189,8 @@ __device__ __forceinline__ int exp_of_row(const double (&y)[8], double r) {
 // An 8-bit k row: norm, rotation and rounding in fp64.  With a = x w and r = 1 / rms the row is r * (a c + z s): a and the
 // partners z are fp32, where a product of two bf16 is exact while it is a normal number; r goes with 2^-e into one factor, and
 // the sum with the rounding constant (kv8_dev.cuh) is fused with it: one multiplication an element is left of three.
-// A product past fp32 gives a bad row, one below its normal numbers is off by 2^-150, which only an r above 2^40 brings near the
-// codes' steps (2^-49 and up): `odd` for such heads (WIDE: fp64 products).
+// A product past fp32 gives a bad row, one below its normal numbers is off by 2^-150, which only an r above 2^40 brings near
+// the codes' steps (2^-49 and up): `odd` for such heads (WIDE: fp64 products).
 template <int FMT, bool HALF, bool WIDE>
 __device__ __forceinline__ void put_k(float (&a)[8], bool norm, const uint4& w, double eps, int rotary_dim, int l16,
                                       const double2* cs, bool store, uint8_t* codes, int8_t* exps, volatile int* odd) {
@@ -224,8 +224,8 @@ __device__ __forceinline__ void put_k(float (&a)[8], bool norm, const uint4& w, 
   store_row(c, raw, l16, store, codes, exps);
 }
 
-// This lane's head of pair i, from the row's start (an odd count's last pair has one head: its other half repeats it).  Pairs of
-// heads: n_qp of q, n_kp of k, n_kp of v.
+// This lane's head of pair i, from the row's start (an odd count's last pair has one head: its other half repeats it).  Pairs
+// of heads: n_qp of q, n_kp of k, n_kp of v.
 __device__ __forceinline__ int head_of_pair(const KvWriteParams& p, int i, int n_qp, int n_kp, int sub) {
   if (i < n_qp) return min(2 * i + sub, p.n_q_heads - 1);
   i -= n_qp;
@@ -268,14 +268,15 @@ __device__ __noinline__ void wide_heads(const KvWriteParams& p, const double2* a
       norm_rotate<HALF, true>(x, norm != nullptr, w, p.eps, p.rotary_dim, l16, cs, nullptr);
       if (store) store8(is_q ? p.q_out + (row * p.n_q_heads + h) * 128 + l16 * 8 : reinterpret_cast<__nv_bfloat16*>(k_row), x);
     } else {
-      put_k<FMT, HALF, true>(x, norm != nullptr, w, p.eps, p.rotary_dim, l16, cs64 + (HALF && l16 >= hop ? 64 : 0) + slot0, store,
-                             k_row, p.k_exp + cache_row + h * 16, nullptr);
+      put_k<FMT, HALF, true>(x, norm != nullptr, w, p.eps, p.rotary_dim, l16, cs64 + (HALF && l16 >= hop ? 64 : 0) + slot0,
+                             store, k_row, p.k_exp + cache_row + h * 16, nullptr);
     }
   }
 }
 
 template <int FMT, bool HALF>
-__global__ void __launch_bounds__(kWriteThreads, kWriteCtas) qk_norm_rope_write_kernel(const __grid_constant__ KvWriteParams p) {
+__global__ void __launch_bounds__(kWriteThreads, kWriteCtas) qk_norm_rope_write_kernel(
+    const __grid_constant__ KvWriteParams p) {
   // for k: half-split rotations, with -s for the elements of the first half, and with s
   __shared__ double2 s_cs64[FMT != GR_KV_BF16 ? kWriteThreads / 32 : 1][HALF ? 2 : 1][64];
   __shared__ float2 s_cs32[kWriteThreads / 32][64];
@@ -297,7 +298,9 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteCtas) qk_norm_rope_write_
   }
   const int n_pairs = slot < 0 ? n_qp : n_qp + 2 * n_kp;
   const __nv_bfloat16* in = p.qkv + row * p.ld_qkv + l16 * 8;
-  auto load = [&](int i) { return __ldg(reinterpret_cast<const uint4*>(in + (even ? 2 * i + sub : head_of_pair(p, i, n_qp, n_kp, sub)) * 128)); };
+  auto load = [&](int i) {
+    return __ldg(reinterpret_cast<const uint4*>(in + (even ? 2 * i + sub : head_of_pair(p, i, n_qp, n_kp, sub)) * 128));
+  };
   uint4 next = make_uint4(0, 0, 0, 0);
   if (g < n_pairs) next = load(g);
   // More rows than run at once: a row's later heads come to L2 at its start, beside other rows' work (16,496 rows: 65 us, 68

@@ -16,10 +16,10 @@
 // again, and what is found above it is ranked by counting.  (Cells, not threads, because 592 rows in flight outgrow the L2:
 // reading every such thread's logits again cost 20% more DRAM traffic.)
 // Bound: reading the row (1,088 rows of 59,392 fp32 logits, the 20 best: 51 us, 55 on another machine; 258 MB, 5.0 TB/s; bf16:
-// 45 us, by its instructions).  Rows with fewer tokens than alternatives are slow: every masked token is a candidate (three of
-// 59,392 left, the 20 best: one row 64 us, 1,088 rows 446).  Few rows (64 bf16: 12 us, one: 9) wait for the chain of phases: stream, maxima, bound, cells, ranks.  They
-// are shared between the CTAs of a cluster, whose states, counts and best lists the first one joins through distributed
-// shared memory.
+// 45 us, by its instructions).  Few rows (64 bf16: 12 us, one: 9) wait for the chain of phases: stream, maxima, bound, cells,
+// ranks.  They are shared between the CTAs of a cluster, whose states, counts and best lists the first one joins through
+// distributed shared memory.  Rows with fewer tokens than alternatives are slow, since every masked token is a candidate (three
+// of 59,392 left, the 20 best: one row 64 us, 1,088 rows 446).
 #include <type_traits>
 
 #include "params.cuh"
@@ -563,8 +563,9 @@ static cudaError_t launch_token_logprobs_t(const LogprobParams& p, int ctas, cud
 }
 
 // 1,024 threads an SM, in CTAs of 512, 256 or 128, a CTA a row: as many rows in flight as there are, since a row's
-// selection (about 6 us) leaves the memory to the other rows' reading.  1,088 rows of 59,392 fp32 logits: 52 us in CTAs of
-// 128 (one wave), 57 in CTAs of 256 (two); 600 rows: 46 / 44; 150 rows: 23 / 17.  Fewer rows than SMs are shared by clusters.
+// selection (about 6 us) leaves the memory to the other rows' reading.  Rows of 59,392 fp32 logits in CTAs of 128, 256 and 512:
+// 1,088 rows 51, 57 and 67 us; 580 rows 39, 31 and 36; 290 rows 36, 25 and 19 (just past a border the larger CTAs would still
+// be better: 600 rows 50 and 44).  Fewer rows than SMs are shared by clusters.
 cudaError_t launch_token_logprobs(LogprobParams p, bool bf16, cudaStream_t stream, bool pdl) {
   auto go = [&](auto nt, int ctas) {
     constexpr int NT = decltype(nt)::value;

@@ -374,9 +374,9 @@ class Engine:
 
     def _qkv_attention_8bit(self, l, d, bs, K, seq_lens, page_table, attn_chunk, attn_splits, st, ws_attn, draft, base_add,
                             rope_pos3) -> None:
-        """Layer l's projection, rotation with the quantised cache write, and attention over the 8-bit cache.  The projected rows
-        are rounded to bf16 on their way (the write is a kernel of its own, and a cached row a function of them alone), q once
-        more after its rotation; the bf16 engine rotates the projection's fp32 accumulators."""
+        """Layer l's projection, rotation with the quantised cache write, and attention over the 8-bit cache.  The projected
+        rows are rounded to bf16 on their way (the write is a kernel of its own, and a cached row a function of them alone),
+        q once more after its rotation; the bf16 engine rotates the projection's fp32 accumulators."""
         cfg, M = self.cfg, bs * K
         e = L.Epilogue()
         e.mode = L.EPI_STORE_BF16

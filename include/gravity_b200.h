@@ -331,8 +331,8 @@ int gr_kv8_attention_plan(int bs, int K, int max_len, int n_q_heads, int n_kv_he
  * least 2^-126, inf for the uniform distribution, or NULL for 1.  -inf logits (masked tokens), and those further below the
  * largest than fp32's largest number, have probability 0.  id -1: no token asked (NaN, rank 0); any other id outside
  * the vocabulary sets GR_ERR_BAD_ID.  A row with a NaN or +inf logit, or with every logit -inf, has no distribution: its
- * outputs are NaN, rank 0, ids -1, and GR_ERR_NO_TOKEN is set; a temperature below 2^-126 or NaN gives the same with GR_ERR_ARG.
- * The reference refuses requests that ask for log probabilities. */
+ * outputs are NaN, rank 0, ids -1, and GR_ERR_NO_TOKEN is set; a temperature below 2^-126 or NaN gives the same with
+ * GR_ERR_ARG.  The reference refuses requests that ask for log probabilities. */
 int gr_token_logprobs(const void* logits, int is_bf16, int64_t ld, int rows, int vocab, const int64_t* ids,
                       const float* temperature, int n_top, float* logprob, float* entropy, int32_t* rank,
                       float* top_logprob, int32_t* top_ids, int32_t* status, void* stream);
