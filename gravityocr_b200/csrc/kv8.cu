@@ -70,25 +70,27 @@ __device__ __forceinline__ T head_square(const float (&x)[8], double eps) {
 }
 
 // Norm and rotation of a head in fp32; cs(k): this lane's k-th pair.  x r stays within sqrt(128) whatever the size of x and w,
-// its squares may not: `odd` where they leave fp32 or its normal numbers (WIDE: a norm in fp64 for such heads).
+// its squares may not: true where they leave fp32 or its normal numbers (WIDE: with a norm in fp64, for such heads).
 template <bool HALF, bool WIDE, typename F>
-__device__ __forceinline__ void norm_rotate(float (&x)[8], bool norm, const uint4& w, double eps, int rotary_dim, int l16,
-                                            F cs, volatile int* odd) {
+__device__ __forceinline__ bool norm_rotate(float (&x)[8], bool norm, const uint4& w, double eps, int rotary_dim, int l16,
+                                            F cs) {
+  bool odd = false;
   if (norm) {
     float wf[8];
     unpack8(w, wf);
+    const float sq = head_square<float>(x, eps);
+    odd = !(sq > 0x1p-100f && sq < 0x1p120f);
     if (WIDE) {
       const double r = rsqrt(head_square<double>(x, eps));
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(static_cast<double>(x[i]) * r) * wf[i];
     } else {
-      const float sq = head_square<float>(x, eps), r = rsqrtf(sq);
-      if (!(sq > 0x1p-100f && sq < 0x1p120f)) *odd = 1;
+      const float r = rsqrtf(sq);
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = x[i] * r * wf[i];
     }
   }
-  if (rotary_dim == 0) return;
+  if (rotary_dim == 0) return odd;
   const bool rot = l16 * 8 < rotary_dim;
   if (HALF) {
     const int hop = rotary_dim >> 4;
@@ -110,6 +112,7 @@ __device__ __forceinline__ void norm_rotate(float (&x)[8], bool norm, const uint
       }
     }
   }
+  return odd;
 }
 
 __device__ __forceinline__ int clamp_exp(int raw) { return max(kKvExpMin, min(kKvExpMax, raw)); }
@@ -233,8 +236,9 @@ __device__ __forceinline__ int head_of_pair(const KvWriteParams& p, int i, int n
   return p.n_q_heads + p.n_kv_heads + min(2 * (i - n_kp) + sub, p.n_kv_heads - 1);
 }
 
-// A warp's q and k heads once more, with norms in fp64: each lane over what it wrote.  Rare, and out of line behind the warp's
-// loops: within them it costs every row registers (write and read of 16,496 rows 88 us, so 82).
+// A warp's q and k heads once more, those whose norm needs fp64 over what the lanes wrote (the others stay: an 8-bit k row
+// comes out the same).  Rare, and out of line behind the warp's loops: within them it costs every row registers (write and read of
+// 16,496 rows 88 us, so 82).
 template <int FMT, bool HALF>
 __device__ __noinline__ void wide_heads(const KvWriteParams& p, const double2* all64, const float2* all32) {
   const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kWriteThreads + threadIdx.x) >> 5, row = unit / p.groups;
@@ -265,8 +269,10 @@ __device__ __noinline__ void wide_heads(const KvWriteParams& p, const double2* a
     const bool store = h < (is_q ? p.n_q_heads : p.n_kv_heads);
     uint8_t* k_row = static_cast<uint8_t*>(p.k) + (cache_row + h * 16) * row_bytes + l16 * (row_bytes / 16);
     if (is_q || FMT == GR_KV_BF16) {
-      norm_rotate<HALF, true>(x, norm != nullptr, w, p.eps, p.rotary_dim, l16, cs, nullptr);
-      if (store) store8(is_q ? p.q_out + (row * p.n_q_heads + h) * 128 + l16 * 8 : reinterpret_cast<__nv_bfloat16*>(k_row), x);
+      const bool odd = norm_rotate<HALF, true>(x, norm != nullptr, w, p.eps, p.rotary_dim, l16, cs);
+      __nv_bfloat16* to =
+          is_q ? p.q_out + (row * p.n_q_heads + h) * 128 + l16 * 8 : reinterpret_cast<__nv_bfloat16*>(k_row);
+      if (store && odd) store8(to, x);
     } else {
       put_k<FMT, HALF, true>(x, norm != nullptr, w, p.eps, p.rotary_dim, l16, cs64 + (HALF && l16 >= hop ? 64 : 0) + slot0,
                              store, k_row, p.k_exp + cache_row + h * 16, nullptr);
@@ -358,7 +364,7 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteCtas) qk_norm_rope_write_
   for (; i < n_qp; i += p.groups) {
     float x[8];
     take(x);
-    norm_rotate<HALF, false>(x, p.q_norm != nullptr, wq, p.eps, p.rotary_dim, l16, cs_f, odd);
+    if (norm_rotate<HALF, false>(x, p.q_norm != nullptr, wq, p.eps, p.rotary_dim, l16, cs_f)) *odd = 1;
     const int h = 2 * i + sub;
     if (h < p.n_q_heads) store8(q_row + h * 128, x);
   }
@@ -372,7 +378,7 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteCtas) qk_norm_rope_write_
     const bool store = h < p.n_kv_heads;
     uint8_t* to = k_row + h * 16 * row_bytes;
     if (FMT == GR_KV_BF16) {
-      norm_rotate<HALF, false>(x, p.k_norm != nullptr, wk, p.eps, p.rotary_dim, l16, cs_f, odd);
+      if (norm_rotate<HALF, false>(x, p.k_norm != nullptr, wk, p.eps, p.rotary_dim, l16, cs_f)) *odd = 1;
       if (store) store8(reinterpret_cast<__nv_bfloat16*>(to), x);
     } else {
       put_k<FMT, HALF, false>(x, p.k_norm != nullptr, wk, p.eps, p.rotary_dim, l16, cs_d, store, to,

@@ -97,3 +97,36 @@ def test_attention_of_large_query_rows(fmt, K, size):
 def test_attention_of_the_largest_query_rows(fmt, K, size):
     """Up to bf16's largest number."""
     test_attention_of_large_query_rows(fmt, K, size)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_an_odd_head_changes_no_other(fmt):
+    """Rows with one head whose norm leaves fp32: its neighbours' outputs are those of the row without it, whether a warp or many
+    share the row."""
+    nq, nkv, m = 16, 8, 2600
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn((m, (nq + 2 * nkv) * 128), generator=g).bfloat16()
+    y = x.clone().view(m, -1, 128)
+    for h in (2, nq + 1):
+        y[:, h] *= 2.0 ** 80
+    w = [(1 + 0.2 * torch.randn(128, generator=g)).bfloat16().to(DEV) for _ in range(2)]
+    inv = (1.0 / 10000.0 ** (torch.arange(0, 64, 2, dtype=torch.float64) / 64)).float().to(DEV)
+    pos = torch.randint(0, 4096, (m,), generator=g, dtype=torch.int32).to(DEV)
+
+    def run(rows, lo, hi):
+        n = hi - lo
+        cache = _cache(n // 16 + 1, nkv, fmt)
+        q = torch.zeros((n, nq * 128), dtype=torch.bfloat16, device=DEV)
+        L.qk_norm_rope_write(rows.view(m, -1)[lo:hi].to(DEV), nq, L.kv_cache(*cache), torch.arange(n, device=DEV), q, inv, 64,
+                             row_pos=pos[lo:hi], q_norm=w[0], k_norm=w[1], eps=1e-6)
+        return [q.cpu().view(n, nq, 128)] + [_rows(t, torch.arange(n)) for t in cache if t is not None]
+
+    plain, loud = run(x, 0, m), run(y, 0, m)
+    others = [h for h in range(nq) if h != 2]
+    assert torch.equal(plain[0][:, others], loud[0][:, others])
+    others = [h for h in range(nkv) if h != 1]
+    for a, b in zip(plain[1:], loud[1:]):
+        assert torch.equal(a[:, others], b[:, others])
+    for lo, hi in ((0, 1), (7, 20)):
+        for a, b in zip(loud, run(y, lo, hi)):
+            assert torch.equal(a[lo:hi], b)
