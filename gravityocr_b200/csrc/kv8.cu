@@ -237,8 +237,8 @@ __device__ __forceinline__ int head_of_pair(const KvWriteParams& p, int i, int n
 }
 
 // A warp's q and k heads once more, those whose norm needs fp64 over what the lanes wrote (the others stay: an 8-bit k row
-// comes out the same).  Rare, and out of line behind the warp's loops: within them it costs every row registers (write and read of
-// 16,496 rows 88 us, so 82).
+// comes out the same).  Rare, and out of line behind the warp's loops: within them it costs every row registers (write and
+// read of 16,496 rows 88 us, so 82).
 template <int FMT, bool HALF>
 __device__ __noinline__ void wide_heads(const KvWriteParams& p, const double2* all64, const float2* all32) {
   const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kWriteThreads + threadIdx.x) >> 5, row = unit / p.groups;
